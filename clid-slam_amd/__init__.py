@@ -3,7 +3,8 @@ inner loop behind the reference's own Python call signatures.
 
     from clid_slam_amd import NeuralPoints, Decoder, Mapper        # drop-ins for model/*.py, utils/mapper.py
     from clid_slam_amd import LocalPointCloudMap, DataSampler     # ... model/local_point_cloud_map.py, utils/data_sampler.py
-    from clid_slam_amd.loss import sdf_bce_loss
+    from clid_slam_amd.loss import sdf_bce_loss, linear_cross_entropy
+    from clid_slam_amd.linear import linear_act, linear_label    # dense layers and class heads of any width
     from clid_slam_amd.tools import get_gradient, setup_optimizer
 
 The compute lives in libclid_native.so (include/clid_native.h); see DESIGN.md / INTEGRATION.md.

@@ -17,12 +17,19 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.path.join(LIBDIR, "libclid_native.so")
 SOURCES = ["api.hip", "comm.hip", "p2p.hip", "table.hip", "celldir.hip", "query.hip", "query_tile.hip", "track_tile.hip", "train.hip", "train_analytic.hip", "train_wf0.hip", "train_tile.hip", "mlp.hip", "sampler.hip", "mapops.hip"]
-HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "train_common.hpp"), os.path.join(CSRC, "search8.hpp"), os.path.join(HERE, "..", "include", "clid_native.h")]
+DENSE = sorted(os.listdir(os.path.join(CSRC, "dense")))  # the dense operators: sources and headers of a folder of their own
+SOURCES += [os.path.join("dense", f) for f in DENSE if f.endswith(".hip")]
+HEADERS = [os.path.join(CSRC, "common.hpp"), os.path.join(CSRC, "train_common.hpp"), os.path.join(CSRC, "search8.hpp"), os.path.join(HERE, "..", "include", "clid_native.h"),
+           os.path.join(HERE, "..", "include", "clid_dense.h")]
+HEADERS += [os.path.join(CSRC, "dense", f) for f in DENSE if f.endswith(".hpp")]
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     "-munsafe-fp-atomics",      # global_atomic_add_f32 instead of a CAS loop
     "-ffp-contract=on",         # FMA only inside one expression; exact-order code uses __f*_rn
     "-Wno-unused-result", "-Wno-unused-value",
+    # no packed fp32 arithmetic: some of its forms have given wrong results on this hardware (hipcc's host pass warns that it does
+    # not know the feature)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     # the leading scalar / pointer arguments of a kernel arrive in SGPRs with the wave instead of through an s_load of the
     # kernel-argument segment (decode 11.75 -> 11.5 us: the record request goes out earlier; profiles/r05_kernarg_ab.jsonl)
     "-mllvm", "-amdgpu-kernarg-preload-count=16",
@@ -53,11 +60,11 @@ def build_variant(name: str, extra_flags) -> str:
     hipcc = _hipcc()
 
     def one(src):
-        obj = os.path.join(objdir, src.replace(".hip", ".o"))
+        obj = os.path.join(objdir, os.path.basename(src).replace(".hip", ".o"))
         subprocess.run([hipcc, *FLAGS, *extra_flags, "-c", os.path.join(CSRC, src), "-o", obj], check=True)
         return obj
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 8)) as ex:
         objs = list(ex.map(one, SOURCES))
     subprocess.run([hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-ldl", "-o", out], check=True)
     return out
@@ -75,7 +82,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
     os.makedirs(objdir, exist_ok=True)
 
     def compile_one(src: str) -> str:
-        obj = os.path.join(objdir, src.replace(".hip", ".o"))
+        obj = os.path.join(objdir, os.path.basename(src).replace(".hip", ".o"))
         cmd = [hipcc, *FLAGS, "-c", os.path.join(CSRC, src), "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
@@ -84,7 +91,7 @@ def build(force: bool = False, verbose: bool = True) -> str:
             print(r.stderr, file=sys.stderr)
         return obj
 
-    with ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with ThreadPoolExecutor(max_workers=min(len(SOURCES), os.cpu_count() or 8)) as ex:
         objs = list(ex.map(compile_one, SOURCES))
     cmd = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", *objs, "-ldl", "-o", LIB]
     r = subprocess.run(cmd, capture_output=True, text=True)

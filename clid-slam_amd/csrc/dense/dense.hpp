@@ -1,0 +1,109 @@
+// What the dense operators (layer, cross entropy of a class head, label of each row) share: element types, activations, the
+// running softmax statistics, argument checks.
+//
+// Softmax statistics.  A row's statistics over a set of columns are (m, r): the largest z and r = sum over the OTHER columns of
+// exp(z - m).  log sum exp = m + log1p(r), so the log-probability of the largest column is -log1p(r) and the loss of a target t
+// is (m - z_t) + log1p(r): a confident row keeps its relative accuracy where m + log(1 + r) would round it away.  Two sets
+// join as: the larger m wins, r = r_win + (1 + r_lose) exp(m_lose - m_win).  A set without a finite value has m = -inf, r = 0.
+#pragma once
+#include <hip/hip_bf16.h>
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "../../../include/clid_dense.h"
+#include "../../../include/clid_native.h"
+
+extern "C" void clid_set_error(const char* fmt, ...);
+
+namespace clid_dense {
+
+using bf16 = __hip_bfloat16;
+using f16 = __half;
+
+__device__ __forceinline__ float up(float v) { return v; }
+__device__ __forceinline__ float up(bf16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float up(f16 v) { return __half2float(v); }
+template <typename T> __device__ __forceinline__ T down(float v);
+template <> __device__ __forceinline__ float down<float>(float v) { return v; }
+template <> __device__ __forceinline__ bf16 down<bf16>(float v) { return __float2bfloat16(v); }
+template <> __device__ __forceinline__ f16 down<f16>(float v) { return __float2half(v); }
+
+__device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
+
+// ---- activations: act(z) and its slope, in fp32 ------------------------------------------------------------------------
+__device__ __forceinline__ float act_value(float z, int act) {
+  switch (act) {
+    case CLID_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
+    case CLID_ACT_LEAKY_RELU: return z > 0.f ? z : 0.01f * z;
+    case CLID_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
+    case CLID_ACT_SILU: return z / (1.f + expf(-z));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_slope(float z, int act) {
+  switch (act) {
+    case CLID_ACT_RELU: return z > 0.f ? 1.f : 0.f;
+    case CLID_ACT_LEAKY_RELU: return z > 0.f ? 1.f : 0.01f;
+    case CLID_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.3989422804014327f;
+    case CLID_ACT_SILU: {
+      const float p = 1.f / (1.f + expf(-z));
+      return p * (1.f + z * (1.f - p));
+    }
+    default: return 1.f;
+  }
+}
+
+// z as the backward pass gets it (clid_linear_args.z_out): rounding to 16 bits must not turn a slope of 1 into one of 0 (a tiny z
+// becoming 0) nor a finite z into an infinity (z p (1 - p) of silu is inf * 0 there)
+template <typename T> __device__ __forceinline__ T keep_z(float z);
+template <> __device__ __forceinline__ float keep_z<float>(float z) { return z; }
+template <> __device__ __forceinline__ bf16 keep_z<bf16>(float z) {
+  bf16 h = down<bf16>(z);
+  const float b = up(h);
+  if (b == 0.f && z != 0.f) h = down<bf16>(copysignf(9.1835496e-41f, z));             // 2^-133, the smallest bf16
+  if (fabsf(b) > 3.3895314e38f && fabsf(z) <= 3.4028235e38f) h = down<bf16>(copysignf(3.3895314e38f, z));  // its largest
+  return h;
+}
+template <> __device__ __forceinline__ f16 keep_z<f16>(float z) {
+  f16 h = down<f16>(z);
+  const float b = up(h);
+  if (b == 0.f && z != 0.f) h = down<f16>(copysignf(5.9604645e-8f, z));               // 2^-24, the smallest fp16
+  if (fabsf(b) > 65504.f && fabsf(z) <= 3.4028235e38f) h = down<f16>(copysignf(65504.f, z));
+  return h;
+}
+
+// ---- softmax statistics ---------------------------------------------------------------------------------------------------
+struct Stat {
+  float m, r;
+  int at;  // the lowest column that holds m (labels only)
+};
+// does (m, at) come before (n, bt)?  A NaN counts as largest, then the larger value, then the lower column.
+__device__ __forceinline__ bool ahead(float m, int at, float n, int bt) {
+  const bool mn = m != m, nn = n != n;
+  if (mn || nn) return mn && (!nn || at < bt);
+  return m > n || (m == n && at < bt);
+}
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+  const bool first = ahead(a.m, a.at, b.m, b.at);
+  const Stat w = first ? a : b, l = first ? b : a;
+  return {w.m, w.r + (l.m == neg_inf() ? 0.f : (1.f + l.r) * expf(l.m - w.m)), w.at};
+}
+
+// ---- host: argument checks ----------------------------------------------------------------------------------------------
+inline bool sizes_ok(int64_t rows, int32_t k, int32_t n) {
+  return rows >= 0 && rows < (int64_t(1) << 31) && k >= 1 && n >= 1 && k < (1 << 24) && n < (1 << 24) &&
+         rows * (k > n ? k : n) <= (int64_t(1) << 40) && int64_t(k) * n <= (int64_t(1) << 40);
+}
+inline int64_t up256(int64_t v) { return (v + 255) & ~int64_t(255); }
+
+}  // namespace clid_dense
+
+#define DENSE_CHECK_LAUNCH(what)                                              \
+  do {                                                                        \
+    hipError_t e__ = hipGetLastError();                                       \
+    if (e__ != hipSuccess) {                                                  \
+      clid_set_error("%s: HIP error: %s", what, hipGetErrorString(e__));      \
+      return CLID_E_HIP;                                                      \
+    }                                                                         \
+  } while (0)

@@ -1,15 +1,17 @@
 """`Decoder` with the reference's interface (model/decoder.py:12), HIP-backed `mlp` / `sdf`.
 
 Parameters stay inside child modules (`layers: ModuleList[nn.Linear]`, `lout: nn.Linear`) so that
-`freeze_model` (utils/tools.py:314-317), `state_dict()` and `vis_pin_map.py` keep working.  The
-compiled shape is the one every shipped config uses: one hidden layer 11 -> 64 -> 1, bias, ReLU.
+`freeze_model` (utils/tools.py:314-317), `state_dict()` and `vis_pin_map.py` keep working.  The shape every shipped config uses (one hidden
+layer 11 -> 64 -> 1, bias, ReLU) has fused kernels of its own; any other width, depth and output count, the semantic head's among
+them, runs layer by layer on the dense operators (linear.py).
 """
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
 
-from . import _lib
+from . import _lib, linear
+from .loss import linear_cross_entropy
 
 
 class _MlpSdf(torch.autograd.Function):
@@ -92,17 +94,28 @@ class Decoder(nn.Module):
     def _require_native(self):
         if not self._native_shape:
             raise NotImplementedError(
-                "libclid_native is compiled for the geometry decoder of the shipped configs "
-                "(1 hidden layer, 11 -> 64 -> 1, bias, ReLU); semantic/colour heads are outside the hot-path scope"
+                "the fused kernels are compiled for the geometry decoder of the shipped configs "
+                "(1 hidden layer, 11 -> 64 -> 1, bias, ReLU); other shapes run through mlp / sdf / sem_label_prob / sem_label / sem_loss"
             )
 
+    def _hidden(self, features):
+        """The activations that `lout` reads: one `linear_act` a layer."""
+        act = "leaky_relu" if self.use_leaky_relu else "relu"
+        for layer in self.layers:
+            features = linear.linear_act(features, layer.weight, layer.bias, activation=act)
+        return features
+
     def mlp(self, features):
-        """model/decoder.py:58-76: [..., 11] -> [..., 1]."""
+        """model/decoder.py:58-76: [..., 11] -> [..., 1], or whatever widths the decoder was built with."""
+        if not self._native_shape:
+            return linear.linear_act(self._hidden(features), self.lout.weight, self.lout.bias)
         W1, b1, W2, b2 = self.flat_params()
         return _MlpSdf.apply(features, W1, b1, W2, b2, 1.0).unsqueeze(-1)
 
     def sdf(self, features):
         """model/decoder.py:80-82: mlp(features).squeeze(1) * sdf_scale."""
+        if not self._native_shape:
+            return self.mlp(features).squeeze(1) * self.sdf_scale
         W1, b1, W2, b2 = self.flat_params()
         out = _MlpSdf.apply(features, W1, b1, W2, b2, float(self.sdf_scale))
         # the reference squeezes dim 1 of [N,1] ([N,K,1] keeps its last dim when weighted_first is off)
@@ -112,7 +125,16 @@ class Decoder(nn.Module):
         return torch.sigmoid(self.sdf(features) / -self.sdf_scale)
 
     def sem_label_prob(self, features):
-        raise NotImplementedError("semantic head is outside the hot-path scope (semantic_on is off in all shipped configs)")
+        """model/decoder.py:84-95: log-probabilities of the classes, [..., out_dim]."""
+        return torch.log_softmax(self.mlp(features), dim=-1)
+
+    def sem_label(self, features):
+        """The class of each row, [...] int64: argmax of `sem_label_prob`, whose logits are never stored."""
+        return linear.linear_label(self._hidden(features), self.lout.weight, self.lout.bias)[0]
+
+    def sem_loss(self, features, label, ignore_index: int = -100, reduction: str = "mean"):
+        """NLL loss of `sem_label_prob(features)` against `label`, whose logits are never stored (loss.linear_cross_entropy)."""
+        return linear_cross_entropy(self._hidden(features), self.lout.weight, self.lout.bias, label, ignore_index, reduction)
 
     def regress_color(self, features):
         raise NotImplementedError("colour head is outside the hot-path scope (color_on is off in all shipped configs)")

@@ -1,9 +1,10 @@
-"""utils/loss.py counterpart: `sdf_bce_loss` (:44-62), HIP-backed (clid_loss_fwd_bwd)."""
+"""utils/loss.py counterpart: `sdf_bce_loss` (:44-62), HIP-backed (clid_loss_fwd_bwd), and the class head's softmax cross
+entropy without its logits (clid_ce_fwd / clid_ce_bwd)."""
 from __future__ import annotations
 
 import torch
 
-from . import _lib
+from . import _lib, linear
 
 
 class _BceLoss(torch.autograd.Function):
@@ -36,3 +37,65 @@ def sdf_bce_loss(pred, label, sigma, weight, weighted=False, bce_reduction="mean
     if bce_reduction != "mean":
         raise NotImplementedError("sdf_bce_loss: only bce_reduction='mean' is used by the mapping loop")
     return _BceLoss.apply(pred, label, sigma, weight, weighted)
+
+
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, target, ignore_index, reduction):
+        n, k = weight.shape
+        x2, w = linear.rows_of(x, k), linear.rows_of(weight, k)
+        b = None if bias is None else bias.detach().contiguous()
+        t = target.detach().reshape(-1).to(torch.int64).contiguous()
+        rows, dev = x2.shape[0], x.device
+        stat = torch.empty((rows, 4), dtype=torch.float32, device=dev)
+        total = torch.empty(2, dtype=torch.float32, device=dev)
+        loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
+        if rows or reduction != 0:
+            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(stat), _lib.ptr(total), _lib.ptr(loss),
+                                 None, None, None, None, linear.ld_of(x2), linear.ld_of(w), rows, ignore_index, k, n,
+                                 linear.DTYPES[x.dtype], reduction)
+            linear.call("clid_ce_fwd", "clid_ce_workspace", args, dev)
+        ctx.ignore_index, ctx.reduction, ctx.has_bias = ignore_index, reduction, bias is not None
+        ctx.save_for_backward(x, weight, t, stat, total, *(() if bias is None else (bias,)))
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight, t, stat, total, *rest = ctx.saved_tensors
+        n, k = weight.shape
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
+        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_w else None
+        db = torch.empty(n, dtype=x.dtype, device=x.device) if need_b else None
+        x2, w = linear.rows_of(x, k), linear.rows_of(weight, k)
+        if x2.shape[0] == 0:
+            for v in (dw, db):
+                if v is not None:
+                    v.zero_()
+        else:
+            b = rest[0].detach().contiguous() if rest else None
+            g = g.detach().reshape(-1).to(torch.float32).contiguous()
+            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(stat), _lib.ptr(total), None, _lib.ptr(g),
+                                 _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), linear.ld_of(x2), linear.ld_of(w), x2.shape[0], ctx.ignore_index,
+                                 k, n, linear.DTYPES[x.dtype], ctx.reduction)
+            linear.call("clid_ce_bwd", "clid_ce_bwd_workspace", args, x.device)
+        return dx, dw, db, None, None, None
+
+
+def linear_cross_entropy(x, weight, bias, target, ignore_index: int = -100, reduction: str = "mean"):
+    """Softmax cross entropy of the logits x weight^T + bias against `target`, with its gradients, never storing the logits: they
+    are made a piece of the classes at a time, in the forward pass for their running maximum and sum, in the backward pass again.
+
+    x [..., k], weight [n, k], bias [n] or None of one type (float32, bfloat16, float16) on one GPU; target [...] int64 or int32
+    class numbers.  The loss is fp32: a value, or [...] with reduction="none".  Rows with target == ignore_index count for nothing,
+    whatever they hold; "mean" divides by the rows that count and is 0 where there are none.  Any other target outside [0, n)
+    makes its row's loss and the gradients that it reaches NaN.  Differentiates once."""
+    if reduction not in linear.REDUCTIONS:
+        raise NotImplementedError(f"linear_cross_entropy: reduction must be mean, sum or none, got {reduction!r}")
+    linear.check_operands("linear_cross_entropy", x, weight, bias)
+    if not isinstance(target, torch.Tensor) or target.dtype not in (torch.int64, torch.int32) or target.device != x.device:
+        raise RuntimeError(f"linear_cross_entropy: target must be int64 or int32 on {x.device}")
+    if target.shape != x.shape[:-1]:
+        raise RuntimeError(f"linear_cross_entropy: target must have shape {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
+    return _LinearCrossEntropy.apply(x, weight, bias, target, int(ignore_index), linear.REDUCTIONS[reduction])

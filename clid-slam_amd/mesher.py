@@ -12,11 +12,14 @@ from . import _lib
 
 
 def query_points(neural_points, sdf_mlp, config, coord, bs=None, query_sdf=True, query_sem=False, query_color=False,
-                 query_mask=True, query_locally=False, mask_min_nn_count: int = 4, out_torch: bool = True):
-    """Same 4-tuple as the reference method: (sdf_pred [N], None, None, mc_mask [N]); `out_torch=False`
-    returns numpy arrays.  Semantic / colour heads are outside the hot-path scope."""
-    if query_sem or query_color:
-        raise NotImplementedError("semantic / colour queries are outside the hot-path scope")
+                 query_mask=True, query_locally=False, mask_min_nn_count: int = 4, out_torch: bool = True, sem_mlp=None):
+    """Same 4-tuple as the reference method: (sdf_pred [N], sem_pred [N] int64 or None, None, mc_mask [N]); `out_torch=False`
+    returns numpy arrays.  `query_sem` asks `sem_mlp` for the class of each point (0 where it has no neighbour).  The colour head
+    is outside the hot-path scope."""
+    if query_color:
+        raise NotImplementedError("colour queries are outside the hot-path scope")
+    if query_sem and sem_mlp is None:
+        raise RuntimeError("query_sem needs a semantic decoder")
     lib = _lib.load()
     bs = int(bs or config.infer_bs)
     n = coord.shape[0]
@@ -35,11 +38,25 @@ def query_points(neural_points, sdf_mlp, config, coord, bs=None, query_sdf=True,
             "clid_sdf_query",
         )
     sdf_pred = sdf if query_sdf else None
+    sem_pred = torch.zeros(n, device=dev, dtype=torch.int64) if query_sem else None
+    for i in range(math.ceil(n / bs) if query_sem else 0):
+        at = slice(i * bs, (i + 1) * bs)
+        sem_pred[at] = torch.where(nn_cnt[at] >= 1, _labels(neural_points, sem_mlp, config, coord[at].to(dev, torch.float32), query_locally), 0)
     mc_mask = (nn_cnt >= mask_min_nn_count).to(torch.float32) if query_mask else None
     if not out_torch:
         sdf_pred = None if sdf_pred is None else sdf_pred.cpu().numpy().astype("float64")
+        sem_pred = None if sem_pred is None else sem_pred.cpu().numpy()
         mc_mask = None if mc_mask is None else mc_mask.cpu().numpy().astype("float64")
-    return sdf_pred, None, None, mc_mask
+    return sdf_pred, sem_pred, None, mc_mask
+
+
+@torch.no_grad()
+def _labels(neural_points, sem_mlp, config, coord, query_locally):
+    """Classes of one chunk of points (utils/mesher.py:118-131)."""
+    feature, _, weight, _, _ = neural_points.query_feature(coord, training_mode=False, query_locally=bool(query_locally))
+    if config.weighted_first:
+        return sem_mlp.sem_label(feature)
+    return (sem_mlp.sem_label_prob(feature) * weight).sum(dim=1).argmax(dim=1)  # the neighbours' log-probabilities, blended
 
 
 class Mesher:
@@ -62,7 +79,7 @@ class Mesher:
                      query_locally=False, mask_min_nn_count: int = 4, out_torch: bool = False):
         """utils/mesher.py:38-163: (sdf_pred, sem_pred, color_pred, mc_mask)."""
         return query_points(self.neural_points, self.sdf_mlp, self.config, coord, bs, query_sdf, query_sem, query_color,
-                            query_mask, query_locally, mask_min_nn_count, out_torch)
+                            query_mask, query_locally, mask_min_nn_count, out_torch, self.sem_mlp)
 
     def recon_aabb_mesh(self, *args, **kwargs):
         raise NotImplementedError("marching cubes / mesh export (utils/mesher.py:371-667) need skimage + open3d: out of scope")
