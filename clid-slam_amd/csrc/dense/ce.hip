@@ -1,0 +1,401 @@
+// Softmax cross entropy of a class head and the class of each row, without the logits (include/clid_dense.h).
+//
+// Rows that count are brought together first (their numbers in `order`, the rows themselves copied without gaps), so a row that does
+// not count costs nothing in the products and what it holds reaches none of them.
+#include "stage.hpp"
+
+using namespace clid_dense;
+
+namespace {
+
+constexpr int kRowsPer = 8192;  // rows a block of k_count / k_order looks at, 8 a thread
+constexpr int kJoinRows = 64;   // rows a block of k_loss_rows joins
+
+__device__ __forceinline__ int block_scan(int v, int* total) {  // exclusive, 1024 threads
+  __shared__ int wsum[16];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  int s = v;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int o = __shfl_up(s, d, 64);
+    if (lane >= d) s += o;
+  }
+  if (lane == 63) wsum[wave] = s;
+  __syncthreads();
+  int before = 0, all = 0;
+  for (int i = 0; i < 16; ++i) {
+    if (i < wave) before += wsum[i];
+    all += wsum[i];
+  }
+  *total = all;
+  return before + s - v;
+}
+
+// counts[block] = rows of the block that count
+__global__ void __launch_bounds__(1024) k_count(const int64_t* target, int64_t rows, int64_t ignore, int* counts) {
+  int c = 0;
+  const int64_t at = (int64_t)blockIdx.x * kRowsPer + threadIdx.x * 8;
+  for (int i = 0; i < 8; ++i) c += at + i < rows && target[at + i] != ignore;
+  int total;
+  block_scan(c, &total);
+  if (threadIdx.x == 0) counts[blockIdx.x] = total;
+}
+// order[0 ..) = the rows that count, in their order; order[rows] = how many; the others' loss
+__global__ void __launch_bounds__(1024) k_order(const int64_t* target, int64_t rows, int64_t ignore, const int* counts, int32_t* order, float* loss_none) {
+  const int64_t at = (int64_t)blockIdx.x * kRowsPer + threadIdx.x * 8;
+  int before = 0, total;
+  for (int b = threadIdx.x; b < (int)blockIdx.x; b += 1024) before += counts[b];
+  block_scan(before, &total);
+  before = total;
+  __syncthreads();
+  int on[8], c = 0;
+  for (int i = 0; i < 8; ++i) {
+    on[i] = at + i < rows && target[at + i] != ignore;
+    c += on[i];
+    if (loss_none && at + i < rows && !on[i]) loss_none[at + i] = 0.f;
+  }
+  int to = before + block_scan(c, &total);
+  for (int i = 0; i < 8; ++i)
+    if (on[i]) order[to++] = (int32_t)(at + i);
+  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) order[rows] = before + total;
+}
+
+// a row's strips joined: 64 rows a block, 16 threads a row; the block's sum of losses
+__global__ void __launch_bounds__(1024) k_loss_rows(const float2* part, int strips, const float* zt, const int64_t* target, const int32_t* order,
+                                                    int64_t rows, int n, float4* stat, float* loss_none, double* sums) {
+  __shared__ float pm[16][kJoinRows], pr[16][kJoinRows];
+  const int64_t live = order[rows];
+  const int row = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int64_t j = (int64_t)blockIdx.x * kJoinRows + row;
+  if ((int64_t)blockIdx.x * kJoinRows >= live) {
+    if (threadIdx.x == 0) sums[blockIdx.x] = 0.0;
+    return;
+  }
+  Stat s = {neg_inf(), 0.f, 0};
+  if (j < live)
+    for (int i = g; i < strips; i += 16) {
+      const float2 p = part[(int64_t)i * rows + j];
+      s = join(s, {p.x, p.y, 0});
+    }
+  pm[g][row] = s.m;
+  pr[g][row] = s.r;
+  __syncthreads();
+  if (g) return;
+  double sum = 0.0;
+  if (j < live) {
+    for (int i = 1; i < 16; ++i) s = join(s, {pm[i][row], pr[i][row], 0});
+    const int64_t m = order[j], t = target[m];
+    const float loss = t >= 0 && t < n ? (s.m - zt[j]) + log1pf(s.r) : __builtin_nanf("");
+    stat[j] = {s.m, 1.f / (1.f + s.r), expm1f(-loss), loss};
+    if (loss_none) loss_none[m] = loss;
+    sum = loss;
+  }
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  if (threadIdx.x == 0) sums[blockIdx.x] = sum;
+}
+__global__ void __launch_bounds__(1024) k_loss_total(const double* sums, int blocks, const int32_t* live, int reduction, float* total, float* loss_out) {
+  __shared__ double ps[16];
+  double s = 0.0;
+  for (int b = threadIdx.x; b < blocks; b += 1024) s += sums[b];
+  for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d, 64);
+  if ((threadIdx.x & 63) == 0) ps[threadIdx.x >> 6] = s;
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = 0.0;
+  for (int i = 0; i < 16; ++i) s += ps[i];
+  const int c = live ? *live : 0;
+  total[0] = (float)s;
+  total[1] = (float)c;
+  if (reduction == CLID_REDUCE_MEAN) loss_out[0] = c ? (float)(s / c) : 0.f;
+  if (reduction == CLID_REDUCE_SUM) loss_out[0] = (float)s;
+}
+
+__global__ void __launch_bounds__(256) k_label_join(const float2* part, const int32_t* part_at, int strips, int64_t rows, int64_t* label, float* log_prob) {
+  __shared__ float pm[16][16], pr[16][16];
+  __shared__ int pa[16][16];
+  const int row = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t m = (int64_t)blockIdx.x * 16 + row;
+  Stat s = {neg_inf(), 0.f, 0x7fffffff};
+  if (m < rows)
+    for (int i = g; i < strips; i += 16) {
+      const float2 p = part[(int64_t)i * rows + m];
+      s = join(s, {p.x, p.y, part_at[(int64_t)i * rows + m]});
+    }
+  pm[g][row] = s.m;
+  pr[g][row] = s.r;
+  pa[g][row] = s.at;
+  __syncthreads();
+  if (g || m >= rows) return;
+  for (int i = 1; i < 16; ++i) s = join(s, {pm[i][row], pr[i][row], pa[i][row]});
+  label[m] = s.at;
+  log_prob[m] = s.m == neg_inf() ? __builtin_nanf("") : -log1pf(s.r);
+}
+
+// scale[0]: what dz is multiplied by as it is stored, scale[1]: what its products are multiplied by.  mean and sum: the one factor
+// belongs to the products, and fp16's dz = p - onehot is stored times 2^10 so that small p keep their bits (|dz| <= 1).  none: the
+// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10.
+__global__ void __launch_bounds__(1024) k_scale(const float* g, const float* total, int64_t rows, int reduction, int half, float* scale) {
+  __shared__ float ps[16];
+  if (reduction != CLID_REDUCE_NONE) {
+    if (threadIdx.x == 0) {
+      const float f = half ? 1024.f : 1.f;
+      scale[0] = f;
+      scale[1] = (reduction == CLID_REDUCE_MEAN ? g[0] / fmaxf(total[1], 1.f) : g[0]) / f;
+    }
+    return;
+  }
+  float top = 0.f;
+  if (half)
+    for (int64_t m = threadIdx.x; m < rows; m += 1024) {
+      const float v = fabsf(g[m]);
+      top = v <= 3.4028235e38f ? fmaxf(top, v) : top;
+    }
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if ((threadIdx.x & 63) == 0) ps[threadIdx.x >> 6] = top;
+  __syncthreads();
+  if (threadIdx.x) return;
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, ps[i]);
+  int e = 0;
+  if (top > 0.f) frexpf(top, &e);  // top < 2^e
+  const int by = half && top > 0.f ? (10 - e > 100 ? 100 : 10 - e < -100 ? -100 : 10 - e) : 0;
+  scale[0] = ldexpf(1.f, by);
+  scale[1] = ldexpf(1.f, -by);
+}
+
+// gradients of the rows that do not count
+template <typename T>
+__global__ void __launch_bounds__(256) k_clear_rows(const int64_t* target, int64_t rows, int64_t ignore, int k, T* dx) {
+  for (int64_t m = blockIdx.x; m < rows; m += gridDim.x)
+    if (target[m] == ignore)
+      for (int c = threadIdx.x; c < k; c += 256) dx[m * k + c] = down<T>(0.f);
+}
+
+template <typename T, int SIZE> constexpr int strip_of() { return Tile<Kind<T>::NP, SIZE>::BN / Tile<Kind<T>::NP, SIZE>::WN; }
+template <typename T>
+int strip_width(int size) { return size == 2 ? strip_of<T, 2>() : size == 1 ? strip_of<T, 1>() : strip_of<T, 0>(); }
+
+template <typename T, bool LABEL>
+int launch_stat(const Product& g, int size, const T* bias, const int64_t* target, const int32_t* order, float2* part, int32_t* part_at, float* zt, hipStream_t s) {
+  constexpr int NP = Kind<T>::NP;
+  if (size == 2) return launch_one<T, 2, false, false>(g, EpiStat<T, Tile<NP, 2>::BN, strip_of<T, 2>(), LABEL>{bias, target, order, part, part_at, zt, g.m, g.n}, s);
+  if (size == 1) return launch_one<T, 1, false, false>(g, EpiStat<T, Tile<NP, 1>::BN, strip_of<T, 1>(), LABEL>{bias, target, order, part, part_at, zt, g.m, g.n}, s);
+  return launch_one<T, 0, false, false>(g, EpiStat<T, Tile<NP, 0>::BN, strip_of<T, 0>(), LABEL>{bias, target, order, part, part_at, zt, g.m, g.n}, s);
+}
+template <typename T>
+int launch_dz(const Product& g, int size, const EpiDz<T, 0, Kind<T>::NP>& e, hipStream_t s) {
+  constexpr int NP = Kind<T>::NP;
+#define DZ(S) launch_one<T, S, false, false>(g, EpiDz<T, Tile<NP, S>::BN, NP>{e.bias, e.target, e.order, e.stat, e.scale, e.g, e.dz, e.v0, e.n, e.ld, e.plane}, s)
+  return size == 2 ? DZ(2) : size == 1 ? DZ(1) : DZ(0);
+#undef DZ
+}
+
+bool ce_ok(const clid_ce_args* a) {
+  return a && sizes_ok(a->rows, a->k, a->n) && dtype_ok(a->dtype) && a->reduction >= 0 && a->reduction <= CLID_REDUCE_SUM;
+}
+
+template <typename T>
+struct CeFwd {
+  Plan p;
+  int strips, joins;
+  char *x, *w, *counts, *part, *zt, *sums;
+  int64_t bytes;
+  explicit CeFwd(const clid_ce_args* a) {
+    Ws ws(a->ws);
+    p = plan<Kind<T>::NP>(a->rows, a->n, a->k, false);
+    strips = (a->n + strip_width<T>(p.size) - 1) / strip_width<T>(p.size);
+    joins = (int)((a->rows + kJoinRows - 1) / kJoinRows);
+    x = ws.take(stage_bytes<T>(a->x, a->ldx, a->rows, a->k, true));
+    w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
+    counts = ws.take((a->rows + kRowsPer - 1) / kRowsPer * 4);
+    part = ws.take((int64_t)strips * a->rows * 8);
+    zt = ws.take(a->rows * 4);
+    sums = ws.take((int64_t)joins * 8);
+    bytes = ws.used;
+  }
+};
+
+template <typename T>
+int ce_fwd(const clid_ce_args* a, hipStream_t s) {
+  const CeFwd<T> f(a);
+  float* none = a->reduction == CLID_REDUCE_NONE ? a->loss_out : nullptr;
+  if (a->rows) {
+    const int blocks = (int)((a->rows + kRowsPer - 1) / kRowsPer);
+    if (blocks > 1) hipLaunchKernelGGL(k_count, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (int*)f.counts);
+    hipLaunchKernelGGL(k_order, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (const int*)f.counts, a->order, none);
+    const int32_t* live = a->order + a->rows;
+    Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, a->order, live), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), live, 0, 1, 0, 0};
+    const int rc = launch_stat<T, false>(g, f.p.size, (const T*)a->bias, a->target, a->order, (float2*)f.part, nullptr, (float*)f.zt, s);
+    if (rc != CLID_OK) return rc;
+    hipLaunchKernelGGL(k_loss_rows, dim3(f.joins), dim3(1024), 0, s, (const float2*)f.part, f.strips, (const float*)f.zt, a->target, a->order, a->rows, a->n,
+                       (float4*)a->stat, none, (double*)f.sums);
+  }
+  hipLaunchKernelGGL(k_loss_total, dim3(1), dim3(1024), 0, s, (const double*)f.sums, f.joins, a->rows ? a->order + a->rows : nullptr, a->reduction, a->total, a->loss_out);
+  return CLID_OK;
+}
+
+// classes per piece: 512 MB of dz, in whole tiles
+template <typename T>
+int64_t piece_of(const clid_ce_args* a) {
+  int64_t p = (int64_t(512) << 20) / (2 * Kind<T>::NP * (a->rows > 0 ? a->rows : 1)) / 256 * 256;
+  if (p < 256) p = 256;
+  return p < a->n ? p : a->n;
+}
+
+template <typename T>
+struct CeBwd {
+  int64_t piece, ld;
+  int blocks;
+  Plan pz, px, pw;
+  char *x, *w, *dz, *sum, *part, *sums, *scale;
+  int64_t bytes;
+  explicit CeBwd(const clid_ce_args* a) {
+    constexpr int NP = Kind<T>::NP;
+    Ws ws(a->ws);
+    piece = piece_of<T>(a);
+    ld = up8(piece);
+    pz = plan<NP>(a->rows, piece, a->k, false);
+    px = plan<NP>(a->rows, a->k, piece, true);
+    pw = plan<NP>(piece, a->k, a->rows, true);
+    x = ws.take(stage_bytes<T>(a->x, a->ldx, a->rows, a->k, true));
+    w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
+    dz = ws.take(NP * a->rows * ld * 2);
+    sum = ws.take(a->dx && piece < a->n ? a->rows * a->k * 4 : 0);
+    const int64_t bx = a->dx ? part_bytes<NP>(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes<NP>(pw, piece, a->k) : 0;
+    part = ws.take(bx > bw ? bx : bw);
+    blocks = row_blocks(a->rows, (int)piece);
+    sums = ws.take(a->db ? blocks * piece * 4 : 0);
+    scale = ws.take(8);
+    bytes = ws.used;
+  }
+};
+
+template <typename T>
+int ce_bwd(const clid_ce_args* a, hipStream_t s) {
+  constexpr int NP = Kind<T>::NP;
+  const CeBwd<T> f(a);
+  const int32_t* live = a->order + a->rows;
+  float* scale = (float*)f.scale;
+  hipLaunchKernelGGL(k_scale, dim3(1), dim3(1024), 0, s, a->g, a->total, a->rows, a->reduction, (int)Kind<T>::F16, scale);
+  if (a->dx)
+    hipLaunchKernelGGL(k_clear_rows<T>, dim3((unsigned)(a->rows < 2048 ? a->rows : 2048)), dim3(256), 0, s, a->target, a->rows, a->ignore_index, a->k, (T*)a->dx);
+  const Operand x = stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, a->order, live);
+  const Operand w = stage<T>(a->w, a->ldw, a->n, a->k, f.w, s);
+  const int wide = a->k % 4 == 0, four = 4 * sizeof(T);
+  for (int64_t v0 = 0; v0 < a->n; v0 += f.piece) {
+    const int64_t nv = a->n - v0 < f.piece ? a->n - v0 : f.piece, ld = up8(nv);
+    Operand wv = w;
+    wv.p += v0 * w.ld;
+    const Operand dz = {(const uint16_t*)f.dz, ld, a->rows * ld};
+    Product gz = {x, wv, a->rows, nv, up8(a->k), live, 0, 1, 0, 0};
+    int rc = launch_dz<T>(gz, f.pz.size, {a->bias ? (const T*)a->bias + v0 : nullptr, a->target, a->order, (const float4*)a->stat, scale,
+                                          a->reduction == CLID_REDUCE_NONE ? a->g : nullptr, (uint16_t*)f.dz, v0, nv, ld, a->rows * ld}, s);
+    if (rc != CLID_OK) return rc;
+    if (a->dx) {
+      const bool last = v0 + nv == a->n;
+      Product g = {dz, wv, a->rows, a->k, nv, live, 0, 1, 0, 0};
+      const float* before = v0 ? (const float*)f.sum : nullptr;
+      if (last)
+        rc = launch_out<T, StoreOut<T>, false, true, EpiStore, T>(g, f.px, {(T*)a->dx, before, scale + 1, a->order, a->k, wide && (uintptr_t)a->dx % four == 0},
+                                                                 (float*)f.part, (const T*)nullptr, s);
+      else
+        rc = launch_out<T, StoreOut<float>, false, true, EpiStore, float>(g, f.px, {(float*)f.sum, before, nullptr, nullptr, a->k, wide}, (float*)f.part, (const float*)nullptr, s);
+      if (rc != CLID_OK) return rc;
+    }
+    if (a->dw) {
+      T* to = (T*)a->dw + v0 * a->k;
+      Product g = {dz, x, nv, a->k, a->rows, live, 1, 1, 0, 0};
+      rc = launch_out<T, StoreOut<T>, true, true, EpiStore, T>(g, f.pw, {to, nullptr, scale + 1, nullptr, a->k, wide && (uintptr_t)to % four == 0}, (float*)f.part, (const T*)nullptr, s);
+      if (rc != CLID_OK) return rc;
+    }
+    if (a->db) {
+      hipLaunchKernelGGL(k_colsum<T>, dim3((unsigned)((ld + 255) / 256), f.blocks), dim3(256), 0, s, (const uint16_t*)f.dz, a->rows, live, (int)nv, (int)ld, a->rows * ld, (float*)f.sums);
+      hipLaunchKernelGGL(k_colsum_join<T>, dim3((unsigned)((nv + 63) / 64)), dim3(256), 0, s, (const float*)f.sums, f.blocks, (int)nv, (const float*)(scale + 1), (T*)a->db + v0);
+    }
+  }
+  return CLID_OK;
+}
+
+bool label_ok(const clid_label_args* a) { return a && sizes_ok(a->rows, a->k, a->n) && dtype_ok(a->dtype); }
+
+template <typename T>
+struct Label {
+  Plan p;
+  int strips;
+  char *x, *w, *part, *at;
+  int64_t bytes;
+  explicit Label(const clid_label_args* a) {
+    Ws ws(a->ws);
+    p = plan<Kind<T>::NP>(a->rows, a->n, a->k, false);
+    strips = (a->n + strip_width<T>(p.size) - 1) / strip_width<T>(p.size);
+    x = ws.take(stage_bytes<T>(a->x, a->ldx, a->rows, a->k));
+    w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
+    part = ws.take((int64_t)strips * a->rows * 8);
+    at = ws.take((int64_t)strips * a->rows * 4);
+    bytes = ws.used;
+  }
+};
+template <typename T>
+int label(const clid_label_args* a, hipStream_t s) {
+  const Label<T> f(a);
+  Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
+  const int rc = launch_stat<T, true>(g, f.p.size, (const T*)a->bias, nullptr, nullptr, (float2*)f.part, (int32_t*)f.at, nullptr, s);
+  if (rc != CLID_OK) return rc;
+  hipLaunchKernelGGL(k_label_join, dim3((unsigned)((a->rows + 15) / 16)), dim3(256), 0, s, (const float2*)f.part, (const int32_t*)f.at, f.strips, a->rows, a->label, a->log_prob);
+  return CLID_OK;
+}
+
+}  // namespace
+
+extern "C" int64_t clid_ce_workspace(const clid_ce_args* a) {
+  if (!ce_ok(a)) return bad("clid_ce_workspace", "bad argument");
+  BY_DTYPE(a->dtype, return CeFwd<T>(a).bytes;);
+}
+extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
+  const char* me = "clid_ce_fwd";
+  if (!ce_ok(a)) return bad(me, "bad argument");
+  if (!a->total || (a->rows && (!a->x || !a->w || !a->target || !a->stat || !a->order || a->ldx < a->k || a->ldw < a->k)) ||
+      (!a->loss_out && !(a->reduction == CLID_REDUCE_NONE && a->rows == 0)))
+    return bad(me, "bad pointer or row stride");
+  const int64_t need = clid_ce_workspace(a);
+  if (a->rows && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  int rc = CLID_OK;
+  BY_DTYPE(a->dtype, rc = ce_fwd<T>(a, (hipStream_t)stream););
+  if (rc != CLID_OK) return rc;
+  DENSE_CHECK_LAUNCH(me);
+  return CLID_OK;
+}
+extern "C" int64_t clid_ce_bwd_workspace(const clid_ce_args* a) {
+  if (!ce_ok(a)) return bad("clid_ce_bwd_workspace", "bad argument");
+  BY_DTYPE(a->dtype, return CeBwd<T>(a).bytes;);
+}
+extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
+  const char* me = "clid_ce_bwd";
+  if (!ce_ok(a)) return bad(me, "bad argument");
+  if (a->rows == 0) return bad(me, "no rows");
+  if (!a->x || !a->w || !a->target || !a->stat || !a->total || !a->order || !a->g || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
+  const int64_t need = clid_ce_bwd_workspace(a);
+  if (!a->ws || a->ws_bytes < need) return bad(me, "workspace too small");
+  int rc = CLID_OK;
+  BY_DTYPE(a->dtype, rc = ce_bwd<T>(a, (hipStream_t)stream););
+  if (rc != CLID_OK) return rc;
+  DENSE_CHECK_LAUNCH(me);
+  return CLID_OK;
+}
+
+extern "C" int64_t clid_label_workspace(const clid_label_args* a) {
+  if (!label_ok(a)) return bad("clid_label_workspace", "bad argument");
+  BY_DTYPE(a->dtype, return Label<T>(a).bytes;);
+}
+extern "C" int clid_label_fwd(const clid_label_args* a, void* stream) {
+  const char* me = "clid_label_fwd";
+  if (!label_ok(a)) return bad(me, "bad argument");
+  if (a->rows == 0) return CLID_OK;
+  if (!a->x || !a->w || !a->label || !a->log_prob || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
+  const int64_t need = clid_label_workspace(a);
+  if (!a->ws || a->ws_bytes < need) return bad(me, "workspace too small");
+  int rc = CLID_OK;
+  BY_DTYPE(a->dtype, rc = label<T>(a, (hipStream_t)stream););
+  if (rc != CLID_OK) return rc;
+  DENSE_CHECK_LAUNCH(me);
+  return CLID_OK;
+}

@@ -4,7 +4,8 @@
 // Softmax statistics.  A row's statistics over a set of columns are (m, r): the largest z and r = sum over the OTHER columns of
 // exp(z - m).  log sum exp = m + log1p(r), so the log-probability of the largest column is -log1p(r) and the loss of a target t
 // is (m - z_t) + log1p(r): a confident row keeps its relative accuracy where m + log(1 + r) would round it away.  Two sets
-// join as: the larger m wins, r = r_win + (1 + r_lose) exp(m_lose - m_win).  A set without a finite value has m = -inf, r = 0.
+// join as: the larger m wins, r = r_win + (1 + r_lose) exp(m_lose - m_win).  A set of -inf alone has m = -inf, r = 0; one that holds a NaN has
+// r = NaN.
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
@@ -87,12 +88,12 @@ __device__ __forceinline__ bool ahead(float m, int at, float n, int bt) {
 __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
   const bool first = ahead(a.m, a.at, b.m, b.at);
   const Stat w = first ? a : b, l = first ? b : a;
-  return {w.m, w.r + (l.m == neg_inf() ? 0.f : (1.f + l.r) * expf(l.m - w.m)), w.at};
+  return {w.m, w.r + (l.m == neg_inf() ? l.r : (1.f + l.r) * expf(l.m - w.m)), w.at};
 }
 
 // ---- host: argument checks ----------------------------------------------------------------------------------------------
 inline bool sizes_ok(int64_t rows, int32_t k, int32_t n) {
-  return rows >= 0 && rows < (int64_t(1) << 31) && k >= 1 && n >= 1 && k < (1 << 24) && n < (1 << 24) &&
+  return rows >= 0 && rows < (int64_t(1) << 31) && k >= 1 && n >= 1 && k < (1 << 22) && n < (1 << 22) &&
          rows * (k > n ? k : n) <= (int64_t(1) << 40) && int64_t(k) * n <= (int64_t(1) << 40);
 }
 inline int64_t up256(int64_t v) { return (v + 255) & ~int64_t(255); }

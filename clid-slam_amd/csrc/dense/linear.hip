@@ -1,0 +1,129 @@
+// A layer: y = act(x w^T + bias) + residual, and its gradients (include/clid_dense.h).
+#include "stage.hpp"
+
+using namespace clid_dense;
+
+namespace {
+
+template <typename T>
+struct Fwd {
+  Plan p;
+  char *x, *w, *part;
+  int64_t bytes;
+  explicit Fwd(const clid_linear_args* a) {
+    Ws ws(a->ws);
+    // both copies or neither where k is odd: their rows are padded alike
+    x = ws.take(stage_bytes<T>(a->x, a->ldx, a->rows, a->k));
+    w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
+    p = plan<Kind<T>::NP>(a->rows, a->n, a->k, true);
+    part = ws.take(part_bytes<Kind<T>::NP>(p, a->rows, a->n));
+    bytes = ws.used;
+  }
+};
+
+template <typename T>
+int fwd(const clid_linear_args* a, hipStream_t s) {
+  const Fwd<T> f(a);
+  Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
+  const int64_t four = 4 * sizeof(T);
+  LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (T*)a->z_out, a->ldr, a->n, a->act,
+                    a->n % 4 == 0 && (uintptr_t)a->y % four == 0 && (uintptr_t)a->z_out % four == 0, a->ldr % 4 == 0 && (uintptr_t)a->residual % four == 0};
+  return launch_out<T, LinearOut<T>, false, false, EpiLinear, T>(g, f.p, o, (float*)f.part, (const T*)a->bias, s);
+}
+
+template <typename T>
+struct Bwd {
+  bool own_dz;  // dz is not dy itself
+  int blocks;
+  Plan px, pw;
+  char *dz, *w, *x, *sums, *part;
+  int64_t bytes;
+  explicit Bwd(const clid_linear_bwd_args* a) {
+    Ws ws(a->ws);
+    own_dz = (a->dx || a->dw) && (a->act != CLID_ACT_NONE || !direct<T>(a->dy, a->lddy, a->n));
+    dz = ws.take(own_dz ? Kind<T>::NP * a->rows * up8(a->n) * 2 : 0);
+    w = ws.take(a->dx ? stage_bytes<T>(a->w, a->ldw, a->n, a->k) : 0);
+    x = ws.take(a->dw ? stage_bytes<T>(a->x, a->ldx, a->rows, a->k) : 0);
+    blocks = row_blocks(a->rows, a->n);
+    sums = ws.take(a->db ? (int64_t)blocks * a->n * 4 : 0);
+    px = plan<Kind<T>::NP>(a->rows, a->k, a->n, true);
+    pw = plan<Kind<T>::NP>(a->n, a->k, a->rows, true);
+    const int64_t bx = a->dx ? part_bytes<Kind<T>::NP>(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes<Kind<T>::NP>(pw, a->n, a->k) : 0;
+    part = ws.take(bx > bw ? bx : bw);
+    bytes = ws.used;
+  }
+};
+
+template <typename T>
+int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
+  const Bwd<T> f(a);
+  const int np = (int)up8(a->n);
+  const T* z = a->act == CLID_ACT_NONE ? nullptr : (const T*)a->z;
+  Operand dz = {(const uint16_t*)a->dy, a->lddy, 0};
+  if (f.own_dz) dz = {(const uint16_t*)f.dz, np, a->rows * np};
+  if (f.own_dz || a->db) {
+    hipLaunchKernelGGL(k_dz<T>, dim3((np + 255) / 256, f.blocks), dim3(256), 0, s, (const T*)a->dy, a->lddy, z, a->rows, a->n, a->act,
+                       (int)wide8<T>(a->dy, a->lddy), (int)wide8<T>(a->z, a->n), f.own_dz ? (uint16_t*)f.dz : nullptr, np, a->rows * np,
+                       a->db ? (float*)f.sums : nullptr);
+    if (a->db)
+      hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(256), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
+  }
+  const int wide = a->k % 4 == 0;
+  if (a->dx) {
+    Product g = {dz, stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->k, a->n, nullptr, 0, 1, 0, 0};
+    StoreOut<T> o = {(T*)a->dx, nullptr, nullptr, nullptr, a->k, wide && (uintptr_t)a->dx % (4 * sizeof(T)) == 0};
+    const int rc = launch_out<T, StoreOut<T>, false, true, EpiStore, T>(g, f.px, o, (float*)f.part, (const T*)nullptr, s);
+    if (rc != CLID_OK) return rc;
+  }
+  if (a->dw) {
+    Product g = {dz, stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), a->n, a->k, a->rows, nullptr, 0, 1, 0, 0};
+    StoreOut<T> o = {(T*)a->dw, nullptr, nullptr, nullptr, a->k, wide && (uintptr_t)a->dw % (4 * sizeof(T)) == 0};
+    return launch_out<T, StoreOut<T>, true, true, EpiStore, T>(g, f.pw, o, (float*)f.part, (const T*)nullptr, s);
+  }
+  return CLID_OK;
+}
+
+bool args_ok(const clid_linear_args* a) {
+  return a && sizes_ok(a->rows, a->k, a->n) && dtype_ok(a->dtype) && a->act >= 0 && a->act <= CLID_ACT_SILU;
+}
+bool args_ok(const clid_linear_bwd_args* a) {
+  return a && sizes_ok(a->rows, a->k, a->n) && dtype_ok(a->dtype) && a->act >= 0 && a->act <= CLID_ACT_SILU;
+}
+
+}  // namespace
+
+extern "C" int64_t clid_linear_workspace(const clid_linear_args* a) {
+  if (!args_ok(a)) return bad("clid_linear_workspace", "bad argument");
+  BY_DTYPE(a->dtype, return Fwd<T>(a).bytes;);
+}
+extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
+  const char* me = "clid_linear_fwd";
+  if (!args_ok(a)) return bad(me, "bad argument");
+  if (a->rows == 0) return CLID_OK;
+  if (!a->x || !a->w || !a->y || a->ldx < a->k || a->ldw < a->k || (a->residual && a->ldr < a->n)) return bad(me, "bad pointer or row stride");
+  const int64_t need = clid_linear_workspace(a);
+  if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  int rc = CLID_OK;
+  BY_DTYPE(a->dtype, rc = fwd<T>(a, (hipStream_t)stream););
+  if (rc != CLID_OK) return rc;
+  DENSE_CHECK_LAUNCH(me);
+  return CLID_OK;
+}
+
+extern "C" int64_t clid_linear_bwd_workspace(const clid_linear_bwd_args* a) {
+  if (!args_ok(a)) return bad("clid_linear_bwd_workspace", "bad argument");
+  BY_DTYPE(a->dtype, return Bwd<T>(a).bytes;);
+}
+extern "C" int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream) {
+  const char* me = "clid_linear_bwd";
+  if (!args_ok(a)) return bad(me, "bad argument");
+  if (a->rows == 0) return bad(me, "no rows");
+  if (!a->x || !a->w || !a->dy || a->ldx < a->k || a->ldw < a->k || a->lddy < a->n || (!a->z && a->act != CLID_ACT_NONE)) return bad(me, "bad pointer or row stride");
+  const int64_t need = clid_linear_bwd_workspace(a);
+  if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  int rc = CLID_OK;
+  BY_DTYPE(a->dtype, rc = bwd<T>(a, (hipStream_t)stream););
+  if (rc != CLID_OK) return rc;
+  DENSE_CHECK_LAUNCH(me);
+  return CLID_OK;
+}

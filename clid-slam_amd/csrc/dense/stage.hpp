@@ -1,0 +1,293 @@
+// Operands made ready for the tiles (tile.hpp): copies with padded rows, bf16 planes of fp32, dz of a layer, column sums, and the
+// choice of tile.
+#pragma once
+#include <atomic>
+
+#include "epi.hpp"
+
+namespace clid_dense {
+
+template <typename T> struct Kind;  // NP: planes a value takes, F16: the matrix instruction
+template <> struct Kind<float> { static constexpr int NP = 3; static constexpr bool F16 = false; using E = bf16; };
+template <> struct Kind<bf16> { static constexpr int NP = 1; static constexpr bool F16 = false; using E = bf16; };
+template <> struct Kind<f16> { static constexpr int NP = 1; static constexpr bool F16 = true; using E = f16; };
+
+inline int64_t up8(int64_t v) { return (v + 7) & ~int64_t(7); }
+constexpr int64_t kLdMost = int64_t(1) << 22;  // a tile's offsets stay under 2^31 bytes
+
+// 8 neighbouring values of a row, wide where the row allows it
+template <typename T>
+__device__ __forceinline__ void get8(const T* p, float (&v)[8], int count, bool wide) {
+  if (wide && count >= 8) {
+    union { uint4 w[sizeof(T) / 2]; T t[8]; } u;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.w[i] = ((const uint4*)p)[i];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = up(u.t[q]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = q < count ? up(p[q]) : 0.f;
+  }
+}
+// 8 values as the planes of T at to (aligned to 16 bytes)
+template <typename T>
+__device__ __forceinline__ void put8(uint16_t* to, int64_t plane, const float (&v)[8]) {
+  if constexpr (Kind<T>::NP == 1) {
+    union { uint4 w; T t[8]; } u;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) u.t[q] = down<T>(v[q]);
+    *(uint4*)to = u.w;
+  } else {
+    union { uint4 w; uint16_t t[8]; } u[3];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      uint16_t h[3];
+      planes(v[q], h);
+#pragma unroll
+      for (int s = 0; s < 3; ++s) u[s].t[q] = h[s];
+    }
+#pragma unroll
+    for (int s = 0; s < 3; ++s) *(uint4*)(to + s * plane) = u[s].w;
+  }
+}
+template <typename T>
+inline bool wide8(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % (16 / (int64_t)sizeof(T)) == 0; }
+
+// rows of src (in `order`, as many as are live) -> planes with rows of kp values, zeros behind k
+template <typename T>
+__global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t rows, int k, const int32_t* order, const int32_t* live, int wide,
+                                               uint16_t* dst, int kp, int64_t plane) {
+  if (live) rows = *live < rows ? *live : rows;
+  const int per = kp / 8;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per;
+    const int c = (int)(i - r * per) * 8;
+    float v[8];
+    get8(src + (order ? (int64_t)order[r] : r) * ld + c, v, k - c < 8 ? k - c : 8, wide);
+    put8<T>(dst + r * kp + c, plane, v);
+  }
+}
+
+inline dim3 grid_for(int64_t items, int64_t most = 16384) {
+  const int64_t b = (items + 255) / 256;
+  return dim3((unsigned)(b < 1 ? 1 : b < most ? b : most));
+}
+
+// An operand as the tiles read it: the caller's own rows where they are 16-bit, aligned and whole, else a copy in the workspace
+template <typename T>
+inline bool direct(const void* p, int64_t ld, int k) {
+  return Kind<T>::NP == 1 && k % 8 == 0 && ld % 8 == 0 && ld <= kLdMost && (reinterpret_cast<uintptr_t>(p) & 15) == 0;
+}
+template <typename T>
+inline int64_t stage_bytes(const void* p, int64_t ld, int64_t rows, int k, bool always = false) {
+  return direct<T>(p, ld, k) && !always ? 0 : up256(Kind<T>::NP * rows * up8(k) * 2);
+}
+template <typename T>
+inline Operand stage(const void* p, int64_t ld, int64_t rows, int k, char* ws, hipStream_t s, bool always = false, const int32_t* order = nullptr,
+                     const int32_t* live = nullptr) {
+  if (direct<T>(p, ld, k) && !always) return {(const uint16_t*)p, ld, 0};
+  const int64_t kp = up8(k);
+  hipLaunchKernelGGL(k_stage<T>, grid_for(rows * kp / 8), dim3(256), 0, s, (const T*)p, ld, rows, k, order, live, (int)wide8<T>(p, ld), (uint16_t*)ws,
+                     (int)kp, rows * kp);
+  return {(const uint16_t*)ws, kp, rows * kp};
+}
+
+// dz = dy act'(z) -> planes with rows of np values (dst may be NULL: the sums alone), and its column sums over blocks of rows ->
+// part[row block][n].  A block takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows.
+template <typename T>
+__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* z, int64_t rows, int n, int act, int wide, int z_wide, uint16_t* dst, int np,
+                                            int64_t plane, float* part) {
+  __shared__ float sums[8][256 + 8];
+  const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8, count = n - c < 8 ? n - c : 8;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c < np)
+    for (int64_t m = (int64_t)blockIdx.y * 8 + rr; m < rows; m += (int64_t)gridDim.y * 8) {
+      float v[8];
+      get8(dy + m * lddy + c, v, count, wide);
+      if (z) {
+        float y[8];
+        get8(z + m * n + c, y, count, z_wide);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < count ? v[q] * act_slope(y[q], act) : 0.f;
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sum[q] += v[q];
+      if (dst) put8<T>(dst + m * np + c, plane, v);
+    }
+  if (!part) return;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sums[rr][cg * 8 + q] = sum[q];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < n) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s += sums[r][threadIdx.x];
+    part[(int64_t)blockIdx.y * n + col] = s;
+  }
+}
+// column sums of planes, as k_dz's
+template <typename T>
+__global__ void __launch_bounds__(256) k_colsum(const uint16_t* src, int64_t rows, const int32_t* live, int n, int np, int64_t plane, float* part) {
+  __shared__ float sums[8][256 + 8];
+  if (live) rows = *live < rows ? *live : rows;
+  const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8;
+  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  if (c < np)
+    for (int64_t m = (int64_t)blockIdx.y * 8 + rr; m < rows; m += (int64_t)gridDim.y * 8) {
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = Kind<T>::NP - 1; s >= 0; --s) {
+        union { uint4 w; typename Kind<T>::E t[8]; } u;
+        u.w = *(const uint4*)(src + s * plane + m * np + c);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += up(u.t[q]);
+      }
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sum[q] += v[q];
+    }
+#pragma unroll
+  for (int q = 0; q < 8; ++q) sums[rr][cg * 8 + q] = sum[q];
+  __syncthreads();
+  const int col = blockIdx.x * 256 + threadIdx.x;
+  if (col < n) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s += sums[r][threadIdx.x];
+    part[(int64_t)blockIdx.y * n + col] = s;
+  }
+}
+// 64 columns a block, 4 threads a column
+template <typename T>
+__global__ void __launch_bounds__(256) k_colsum_join(const float* part, int blocks, int n, const float* alpha, T* out) {
+  __shared__ float p[4][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+  float s = 0.f;
+  if (c < n)
+    for (int b = g; b < blocks; b += 4) s += part[(int64_t)b * n + c];
+  p[g][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (g == 0 && c < n) out[c] = down<T>((alpha ? *alpha : 1.f) * (p[0][threadIdx.x] + p[1][threadIdx.x] + p[2][threadIdx.x] + p[3][threadIdx.x]));
+}
+inline int row_blocks(int64_t rows, int n) {
+  const int64_t cols = (n + 255) / 256, want = 1024 / cols + 1, most = (rows + 63) / 64;
+  return (int)(most < want ? most : want);
+}
+
+// ---- tiles --------------------------------------------------------------------------------------------------------------
+template <int NP, int SIZE> struct Tile;
+template <> struct Tile<1, 2> { static constexpr int BM = 256, BN = 256, BK = 64, WM = 2, WN = 4; };
+template <> struct Tile<1, 1> { static constexpr int BM = 128, BN = 128, BK = 64, WM = 2, WN = 2; };
+template <> struct Tile<1, 0> { static constexpr int BM = 64, BN = 64, BK = 64, WM = 2, WN = 2; };
+template <> struct Tile<3, 2> { static constexpr int BM = 256, BN = 128, BK = 32, WM = 4, WN = 2; };
+template <> struct Tile<3, 1> { static constexpr int BM = 128, BN = 64, BK = 32, WM = 2, WN = 2; };
+template <> struct Tile<3, 0> { static constexpr int BM = 64, BN = 64, BK = 32, WM = 2, WN = 2; };
+template <int NP>
+inline void tile_shape(int size, int* bm, int* bn, int* bk) {
+  *bm = size == 2 ? Tile<NP, 2>::BM : size == 1 ? Tile<NP, 1>::BM : Tile<NP, 0>::BM;
+  *bn = size == 2 ? Tile<NP, 2>::BN : size == 1 ? Tile<NP, 1>::BN : Tile<NP, 0>::BN;
+  *bk = size == 2 ? Tile<NP, 2>::BK : size == 1 ? Tile<NP, 1>::BK : Tile<NP, 0>::BK;
+}
+
+constexpr int kCus = 256;
+
+// Which tile, and into how many parts k is cut.  The largest tile that still gives every CU one; where even the smallest leaves
+// CUs idle, k is cut while each part keeps 8 steps (a part costs its sums' trip through memory).
+struct Plan {
+  int size, splits;
+};
+template <int NP>
+inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
+  Plan p = {0, 1};
+  int bm, bn, bk;
+  for (int size = 2; size >= 0; --size) {
+    tile_shape<NP>(size, &bm, &bn, &bk);
+    p.size = size;
+    if (((m + bm - 1) / bm) * ((n + bn - 1) / bn) >= kCus) return p;
+  }
+  if (!may_split) return p;
+  // cut the tile in the middle: its operands' traffic is half the smallest one's
+  p.size = m > 64 && n > 64 ? 1 : 0;
+  tile_shape<NP>(p.size, &bm, &bn, &bk);
+  const int64_t tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn), steps = (k + bk - 1) / bk;
+  int64_t s = (2 * kCus + tiles - 1) / tiles;
+  if (s > steps / 8) s = steps / 8;
+  if (s > 64) s = 64;
+  p.splits = s < 1 ? 1 : (int)s;
+  return p;
+}
+
+template <typename T, int SIZE, bool PKS, bool QKS, class Epi>
+inline int launch_one(Product g, const Epi& epi, hipStream_t s) {
+  constexpr int NP = Kind<T>::NP;
+  using C = Tile<NP, SIZE>;
+  g.tiles_m = (int)((g.m + C::BM - 1) / C::BM);
+  g.tiles_n = (int)((g.n + C::BN - 1) / C::BN);
+  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
+  if (blocks * 64 * C::WM * C::WN >= (int64_t(1) << 32)) {
+    clid_set_error("dense product: %lld x %lld results are more than one launch takes", (long long)g.m, (long long)g.n);
+    return CLID_E_SHAPE;
+  }
+  constexpr int kLds = 2 * NP * (C::BM + C::BN) * C::BK * 2 + C::BN * 4;
+  auto k = k_tile<Kind<T>::F16, NP, C::BM, C::BN, C::BK, C::WM, C::WN, PKS, QKS, Epi>;
+  if (kLds > 65536) {  // asked for once a device
+    static std::atomic<uint64_t> asked{0};
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev > 63 || !(asked.load() >> dev & 1)) {
+      const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+      if (e != hipSuccess) {
+        clid_set_error("dense product: %d bytes of LDS refused: %s", kLds, hipGetErrorString(e));
+        return CLID_E_HIP;
+      }
+      if (dev < 64) asked.fetch_or(uint64_t(1) << dev);
+    }
+  }
+  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * C::WM * C::WN), kLds, s, g, epi);
+  return CLID_OK;
+}
+
+template <typename T, class Out, bool PKS, bool QKS, template <typename, int> class Epi, typename TO>
+inline int launch_out(Product g, const Plan& p, const Out& o, float* part, const TO* bias, hipStream_t s) {
+  g.splits = p.splits;
+  if (p.splits > 1) {
+    const int64_t n4 = (g.n + 3) / 4 * 4;
+    int rc;
+    if (p.size == 1) rc = launch_one<T, 1, PKS, QKS>(g, EpiPart<Tile<Kind<T>::NP, 1>::BN>{part, g.m, n4}, s);
+    else rc = launch_one<T, 0, PKS, QKS>(g, EpiPart<Tile<Kind<T>::NP, 0>::BN>{part, g.m, n4}, s);
+    if (rc != CLID_OK) return rc;
+    hipLaunchKernelGGL((k_join<TO, Out>), grid_for(g.m * n4 / 4), dim3(256), 0, s, part, p.splits, g.m, n4, g.live_k ? nullptr : g.live, bias, o);
+    return CLID_OK;
+  }
+  if (p.size == 2) return launch_one<T, 2, PKS, QKS>(g, Epi<TO, Tile<Kind<T>::NP, 2>::BN>{o}, s);
+  if (p.size == 1) return launch_one<T, 1, PKS, QKS>(g, Epi<TO, Tile<Kind<T>::NP, 1>::BN>{o}, s);
+  return launch_one<T, 0, PKS, QKS>(g, Epi<TO, Tile<Kind<T>::NP, 0>::BN>{o}, s);
+}
+template <int NP>
+inline int64_t part_bytes(const Plan& p, int64_t m, int64_t n) { return p.splits > 1 ? up256(p.splits * m * ((n + 3) / 4 * 4) * 4) : 0; }
+
+// the workspace handed out front to back; sizes and pointers come from one walk, so they cannot differ
+struct Ws {
+  char* base;
+  int64_t used = 0;
+  explicit Ws(void* p) : base((char*)p) {}
+  char* take(int64_t bytes) {
+    char* at = base ? base + used : nullptr;
+    used += up256(bytes);
+    return at;
+  }
+};
+
+inline int bad(const char* what, const char* why) {
+  clid_set_error("%s: %s", what, why);
+  return CLID_E_ARG;
+}
+inline bool dtype_ok(int d) { return d == CLID_F32 || d == CLID_BF16 || d == CLID_F16; }
+
+}  // namespace clid_dense
+
+#define BY_DTYPE(dtype, ...)                                       \
+  do {                                                             \
+    if ((dtype) == CLID_F32) { using T = float; __VA_ARGS__ }      \
+    else if ((dtype) == CLID_BF16) { using T = clid_dense::bf16; __VA_ARGS__ } \
+    else { using T = clid_dense::f16; __VA_ARGS__ }                \
+  } while (0)

@@ -1,0 +1,247 @@
+// The matrix-core product under the dense operators: OUT(m, n) = sum_k P(m, k) Q(n, k), fp32 sums, 16-bit operands.
+//
+// Operands.  P and Q lie in memory either with k contiguous (rows of a layer's input, a weight) or with k as the row (KS: the
+// same matrices seen from the gradients' products); both go through LDS as they lie, and the fragments of a KS operand are
+// turned on the way out of LDS (ds_read_b64_tr_b16), so no transposed copy is ever made.
+// fp32 operands come as NP = 3 bf16 planes, hi + mid + lo = v exactly (8 bits each, by truncation): six plane products
+// (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave out less than 2^-22 of |p q| and run at the bf16 rate, 2.5 PFLOP/s / 6 =
+// 417 TFLOP/s against 157 of the fp32 matrix instructions.  Infinities behave: planes() below.
+//
+// Tiles.  One block computes BM x BN with WM x WN waves, each 32 x 32 x 16 instructions on a (BM / WM) x (BN / WN) part.  Per step
+// of BK along k the block copies both tiles from memory straight to LDS (16 bytes a lane, buffer loads whose bounds check turns
+// everything outside the matrix into zeros), one step ahead, into the other half of LDS, while the waves multiply.
+// LDS rows are dealt out in 16-byte chunks whose place is permuted per row so that the lanes that read together hit different
+// banks; the copy writes LDS in lane order, so the permutation is applied to the address each lane loads from.
+// The instruction's row operand is Q, its column operand P: a lane then holds one m and, per instruction, four runs of four
+// neighbouring n -- stores are 8 or 16 bytes wide and a row's softmax statistics need one exchange between two lanes.
+//
+// Blocks.  Block ids go round the 8 XCDs in turn; consecutive tiles of one XCD share rows of Q (8 of them, then the next m), so that an
+// XCD's 32 CUs work on an 8 x 4 patch of tiles out of their own L2.
+#pragma once
+#include "dense.hpp"
+
+namespace clid_dense {
+
+typedef __attribute__((ext_vector_type(8))) __bf16 bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(8))) short s16x8;
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) float f32x4;
+
+struct Operand {
+  const uint16_t* p;  // plane 0
+  int64_t ld;         // elements between rows
+  int64_t plane;      // elements between planes
+};
+
+struct Product {
+  Operand p, q;
+  int64_t m, n, k;      // k (contiguous operands) or the rows' lengths (KS ones) are multiples of 8, by zeros where need be
+  const int32_t* live;  // how many of m (or of k, live_k) there are on the device; NULL: all
+  int live_k;
+  int splits;           // k is cut into so many parts, part s of tile t is block t * splits + s
+  int tiles_m, tiles_n;
+};
+
+template <bool F16>
+__device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
+  if constexpr (F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+constexpr uint32_t kOutside = 0x80000000u;  // an offset that every bounds check here refuses: the load returns zeros
+
+// v as three bf16 planes.  Each is the one before's remainder cut to 8 bits, so they have v's sign and their sum is v.  A plane that
+// comes out as 0 is 2^-126 with v's sign instead, and an infinity's planes are all infinite: then an infinity in the other operand
+// meets no zero that is not a zero of the matrix, and all six products have the sign of the one that they stand for.
+__device__ __forceinline__ void planes(float v, uint16_t (&h)[3]) {
+  const uint32_t b = __float_as_uint(v), sign = b & 0x80000000u;
+  if ((b & 0x7f800000u) == 0x7f800000u || (b & 0x7fffffffu) == 0) {
+    h[0] = h[1] = h[2] = (uint16_t)((b >> 16) | ((b & 0xffffu) ? 1 : 0));  // inf, 0, or a NaN that stays one
+    return;
+  }
+  const float r1 = v - __uint_as_float(b & 0xffff0000u);
+  const uint32_t b1 = __float_as_uint(r1) & 0xffff0000u;
+  const uint32_t b2 = __float_as_uint(r1 - __uint_as_float(b1)) & 0xffff0000u;
+  const uint16_t tiny = (uint16_t)((sign | 0x00800000u) >> 16);
+  h[0] = (b >> 16) & 0x7fff ? (uint16_t)(b >> 16) : tiny;
+  h[1] = b1 & 0x7fffffffu ? (uint16_t)(b1 >> 16) : tiny;
+  h[2] = b2 & 0x7fffffffu ? (uint16_t)(b2 >> 16) : tiny;
+}
+
+// R rows (m or n) x BK of one operand in LDS, NP planes
+template <int R, int BK, int NP, bool KS, int WAVES>
+struct Side {
+  static constexpr int kBytes = R * BK * 2;                  // of a plane
+  static constexpr int kLoads = kBytes / 1024 / WAVES;       // 16-byte loads per lane and plane
+  static constexpr int kChunks = KS ? R / 8 : BK / 8;        // 16-byte chunks of an LDS row
+  static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
+
+  // where chunk c of LDS row `row` lies
+  static __device__ __forceinline__ int place(int row, int c) {
+    if constexpr (KS) {
+      // a fragment read takes 64 bytes of rows k .. k + 3 and k + 8 .. k + 11
+      if constexpr (kChunks >= 32) return c ^ ((((row >> 1) & 4) | (row & 3)) << 2);
+      if constexpr (kChunks == 16) return c ^ ((row & 3) << 2);
+      return c ^ (((row >> 1) & 1) << 2);
+    } else {
+      if constexpr (kChunks == 8) return c ^ (row & 7);
+      return c ^ ((row >> 2) & 3);
+    }
+  }
+
+  uint32_t at[kLoads];  // byte offset of this lane's loads within the tile of plane 0
+
+  // first: the tile's first row (m or n); rows: how many there are
+  __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t rows, int wave, int lane) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
+      if constexpr (KS) {
+        at[i] = first + chunk * 8 < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
+      } else {
+        at[i] = first + row < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
+      }
+    }
+  }
+
+  // copies the tile at k0 .. k0 + BK (those below k) to LDS
+  __device__ __forceinline__ void load(const Operand& o, int64_t first, int64_t rows, int64_t k0, int64_t k, char* lds, int wave, int lane) const {
+#pragma unroll
+    for (int s = 0; s < NP; ++s) {
+      const uint16_t* base = o.p + s * o.plane + (KS ? k0 * o.ld + first : first * o.ld + k0);
+      int64_t bytes;
+      if constexpr (KS) bytes = ((k - k0 - 1) * o.ld + (rows - first)) * 2;
+      else bytes = ((rows - first - 1) * o.ld + ((k - k0 + 7) & ~int64_t(7))) * 2;  // rows are whole chunks
+      const uint32_t bound = bytes > 0x7fffffff ? 0x7fffffffu : (uint32_t)bytes;
+      auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bound, 0x00027000);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        uint32_t off = at[i];
+        if constexpr (!KS) {
+          if (k0 + BK > k) {  // the last step: chunks past k read zeros, not the next row
+            const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
+            if (k0 + chunk * 8 >= k) off = kOutside;
+          }
+        }
+        char* dst = lds + s * kBytes + (i * WAVES + wave) * 1024;
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
+      }
+    }
+  }
+
+  // this lane's 8 values of k (16 kk + 8 (lane / 32) ..) of row 32 t + lane % 32
+  static __device__ __forceinline__ s16x8 fragment(const char* lds, int s, int first, int kk, int lane) {
+    if constexpr (!KS) {
+      const int row = first + (lane & 31), c = 2 * kk + (lane >> 5);
+      return *(const s16x8*)(lds + s * kBytes + (row * kChunks + place(row, c)) * 16);
+    } else {
+      // 16 lanes together read 4 rows (k) of 16 columns; lane i of them gets column i of the four rows
+      const int i = lane & 15, k = 16 * kk + 8 * (lane >> 5) + (i >> 2), col = first + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
+      const char* at0 = lds + s * kBytes + (k * kChunks + place(k, col >> 3)) * 16 + (col & 4) * 2;
+      const char* at1 = lds + s * kBytes + ((k + 4) * kChunks + place(k + 4, col >> 3)) * 16 + (col & 4) * 2;
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at0);
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at1);
+      return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+  }
+};
+
+// (tile row, tile column) of tile t
+__device__ __forceinline__ void place_tile(const Product& g, int64_t block, int64_t blocks, int* tm, int* tn) {
+  constexpr int64_t kXcd = 8, kCols = 8;
+  int64_t t = block;
+  const int64_t whole = blocks / kXcd * kXcd;
+  if (t < whole) t = (t % kXcd) * (blocks / kXcd) + t / kXcd;
+  const int64_t band = kCols * g.tiles_m, b = t / band, in = t % band;
+  const int64_t cols = g.tiles_n - b * kCols < kCols ? g.tiles_n - b * kCols : kCols;
+  *tn = (int)(b * kCols + in % cols);
+  *tm = (int)(in / cols);
+}
+
+template <bool F16, int NP, int BM, int BN, int BK, int WM, int WN, bool PKS, bool QKS, class Epi>
+__global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  using SideP = Side<BM, BK, NP, PKS, WAVES>;
+  using SideQ = Side<BN, BK, NP, QKS, WAVES>;
+  constexpr int kStage = NP * (SideP::kBytes + SideQ::kBytes);
+  extern __shared__ __align__(16) char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int wm = wave / WN, wn = wave % WN;
+  int tm, tn;
+  place_tile(g, blockIdx.x / g.splits, gridDim.x / g.splits, &tm, &tn);
+  const int split = blockIdx.x % g.splits;
+  int64_t rows_m = g.m, rows_k = g.k;
+  if (g.live) {
+    const int64_t live = *g.live;
+    if (g.live_k) rows_k = live < rows_k ? live : rows_k;
+    else rows_m = live < rows_m ? live : rows_m;
+  }
+  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  if (m0 >= rows_m) return;
+  const int64_t steps_all = (rows_k + BK - 1) / BK, per = (steps_all + g.splits - 1) / g.splits;
+  const int64_t from = split * per * BK, to = (split + 1) * per * BK < rows_k ? (split + 1) * per * BK : rows_k;
+  const int64_t steps = to > from ? (to - from + BK - 1) / BK : 0;
+
+  // rows of a KS operand are as long as its matrix, padded to 8
+  const int64_t lim_m = PKS ? (rows_m + 7) / 8 * 8 : rows_m, lim_n = QKS ? (g.n + 7) / 8 * 8 : g.n;
+  SideP sp;
+  SideQ sq;
+  sp.init(g.p, m0, lim_m, wave, lane);
+  sq.init(g.q, n0, lim_n, wave, lane);
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int j = 0; j < TM; ++j)
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
+
+  auto load = [&](int64_t step, char* buf) {
+    sp.load(g.p, m0, lim_m, from + step * BK, to, buf, wave, lane);
+    sq.load(g.q, n0, lim_n, from + step * BK, to, buf + NP * SideP::kBytes, wave, lane);
+  };
+  auto multiply = [&](const char* buf) {
+#pragma unroll
+    for (int kk = 0; kk < BK / 16; ++kk) {
+      s16x8 p[NP][TM], q[NP][TN];
+#pragma unroll
+      for (int s = 0; s < NP; ++s) {
+#pragma unroll
+        for (int j = 0; j < TM; ++j) p[s][j] = SideP::fragment(buf, s, (wm * TM + j) * 32, kk, lane);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) q[s][i] = SideQ::fragment(buf + NP * SideP::kBytes, s, (wn * TN + i) * 32, kk, lane);
+      }
+      constexpr int kPairs = NP == 3 ? 6 : 1;
+      constexpr int kP[6] = {0, 2, 1, 0, 1, 0}, kQ[6] = {2, 0, 1, 1, 0, 0};  // the small products first
+#pragma unroll
+      for (int t = 0; t < kPairs; ++t)
+#pragma unroll
+        for (int j = 0; j < TM; ++j)
+#pragma unroll
+          for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(q[NP == 1 ? 0 : kQ[t]][i], p[NP == 1 ? 0 : kP[t]][j], acc[j][i]);
+    }
+  };
+  if (steps > 0) load(0, lds);
+  epi.prepare(n0, lds + 2 * kStage);
+  for (int64_t s = 0; s < steps; ++s) {
+    __builtin_amdgcn_s_waitcnt(0);  // this wave's copies of step s have landed ...
+    __syncthreads();                // ... and everyone's; nobody still reads the other half
+    if (s + 1 < steps) load(s + 1, lds + ((s + 1) & 1) * kStage);
+    multiply(lds + (s & 1) * kStage);
+  }
+  if (steps == 0) __syncthreads();  // what prepare() left in LDS
+
+  const int half = lane >> 5;
+#pragma unroll
+  for (int j = 0; j < TM; ++j) {
+    const int64_t m = m0 + (wm * TM + j) * 32 + (lane & 31);
+    const int64_t nw = n0 + wn * TN * 32;
+    epi.template row<TN>(acc[j], m, m < rows_m, nw, g.n, half, split, lds + 2 * kStage, (int)(nw - n0));
+  }
+}
+
+}  // namespace clid_dense

@@ -31,7 +31,7 @@ class LinearBwdArgs(C.Structure):
 
 
 class CeArgs(C.Structure):
-    _fields_ = [("x", _vp), ("w", _vp), ("bias", _vp), ("target", _vp), ("stat", _vp), ("total", _vp), ("loss_out", _vp),
+    _fields_ = [("x", _vp), ("w", _vp), ("bias", _vp), ("target", _vp), ("order", _vp), ("stat", _vp), ("total", _vp), ("loss_out", _vp),
                 ("g", _vp), ("dx", _vp), ("dw", _vp), ("db", _vp),
                 ("ldx", _i64), ("ldw", _i64), ("rows", _i64), ("ignore_index", _i64),
                 ("k", _i32), ("n", _i32), ("dtype", _i32), ("reduction", _i32), ("ws", _vp), ("ws_bytes", _i64)]

@@ -47,22 +47,23 @@ class _LinearCrossEntropy(torch.autograd.Function):
         b = None if bias is None else bias.detach().contiguous()
         t = target.detach().reshape(-1).to(torch.int64).contiguous()
         rows, dev = x2.shape[0], x.device
+        order = torch.empty(rows + 1, dtype=torch.int32, device=dev)
         stat = torch.empty((rows, 4), dtype=torch.float32, device=dev)
         total = torch.empty(2, dtype=torch.float32, device=dev)
         loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
         if rows or reduction != 0:
-            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(stat), _lib.ptr(total), _lib.ptr(loss),
+            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(order), _lib.ptr(stat), _lib.ptr(total), _lib.ptr(loss),
                                  None, None, None, None, linear.ld_of(x2), linear.ld_of(w), rows, ignore_index, k, n,
                                  linear.DTYPES[x.dtype], reduction)
             linear.call("clid_ce_fwd", "clid_ce_workspace", args, dev)
         ctx.ignore_index, ctx.reduction, ctx.has_bias = ignore_index, reduction, bias is not None
-        ctx.save_for_backward(x, weight, t, stat, total, *(() if bias is None else (bias,)))
+        ctx.save_for_backward(x, weight, t, order, stat, total, *(() if bias is None else (bias,)))
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, weight, t, stat, total, *rest = ctx.saved_tensors
+        x, weight, t, order, stat, total, *rest = ctx.saved_tensors
         n, k = weight.shape
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
@@ -76,7 +77,7 @@ class _LinearCrossEntropy(torch.autograd.Function):
         else:
             b = rest[0].detach().contiguous() if rest else None
             g = g.detach().reshape(-1).to(torch.float32).contiguous()
-            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(stat), _lib.ptr(total), None, _lib.ptr(g),
+            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(order), _lib.ptr(stat), _lib.ptr(total), None, _lib.ptr(g),
                                  _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), linear.ld_of(x2), linear.ld_of(w), x2.shape[0], ctx.ignore_index,
                                  k, n, linear.DTYPES[x.dtype], ctx.reduction)
             linear.call("clid_ce_bwd", "clid_ce_bwd_workspace", args, x.device)

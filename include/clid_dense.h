@@ -11,7 +11,7 @@
  *   - dtype (CLID_F32 / CLID_BF16 / CLID_F16) is that of x, w, bias, residual, y and of the gradients; sums, softmax statistics,
  *     losses and log-probabilities are fp32;
  *   - `ws` has at least clid_*_workspace() bytes, 256-byte aligned, and holds nothing between calls;
- *   - rows >= 0, k >= 1, n >= 1, each matrix at most 2^40 elements; rows < 2^31, k, n < 2^24.
+ *   - rows >= 0, k >= 1, n >= 1, each matrix at most 2^40 elements; rows < 2^31, k, n < 2^22.
  */
 #ifndef CLID_DENSE_H
 #define CLID_DENSE_H
@@ -64,17 +64,19 @@ int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream);
 /* Softmax cross entropy of z = x w^T + bias against target, never storing z.  A row whose target is ignore_index has loss 0, no
  * gradient, and what its x holds (NaN, infinities) reaches nothing.  A target outside [0, n) that is not ignore_index makes its
  * row's loss NaN.
- *   stat      [rows][4] fp32: largest z, 1 / sum exp(z - largest), p_target - 1, loss of the row
+ *   order     [rows + 1] int32: the rows that count, in their order, and in the last place how many there are
+ *   stat      [rows][4] fp32, by place in `order`: largest z, 1 / sum exp(z - largest), p_target - 1, loss of the row
  *   total     [2] fp32: sum of the losses; number of rows that count
  *   loss_out  [1] (CLID_REDUCE_MEAN: the sum over the counted rows / their number, 0 if there are none; CLID_REDUCE_SUM) or
  *             [rows] (CLID_REDUCE_NONE) fp32
- * Backward: g is dL/dloss_out (fp32, one value or [rows]); stat, total as the forward call left them. */
+ * Backward: g is dL/dloss_out (fp32, one value or [rows]); order, stat, total as the forward call left them. */
 #define CLID_REDUCE_NONE 0
 #define CLID_REDUCE_MEAN 1
 #define CLID_REDUCE_SUM 2
 typedef struct clid_ce_args {
   const void *x, *w, *bias; /* [rows][k], [n][k], [n] or NULL */
   const int64_t* target;    /* [rows] */
+  int32_t* order;
   float *stat, *total, *loss_out;
   const float* g;     /* backward only */
   void *dx, *dw, *db; /* backward only, dense, NULL where not wanted */
