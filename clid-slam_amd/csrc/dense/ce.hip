@@ -260,7 +260,7 @@ struct CeBwd {
     w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
     dz = ws.take(NP * a->rows * ld * 2);
     sum = ws.take(a->dx && piece < a->n ? a->rows * a->k * 4 : 0);
-    const int64_t bx = a->dx ? part_bytes<NP>(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes<NP>(pw, piece, a->k) : 0;
+    const int64_t bx = a->dx ? part_bytes(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes(pw, piece, a->k) : 0;
     part = ws.take(bx > bw ? bx : bw);
     blocks = row_blocks(a->rows, (int)piece);
     sums = ws.take(a->db ? blocks * piece * 4 : 0);
@@ -280,7 +280,6 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
     hipLaunchKernelGGL(k_clear_rows<T>, dim3((unsigned)(a->rows < 2048 ? a->rows : 2048)), dim3(256), 0, s, a->target, a->rows, a->ignore_index, a->k, (T*)a->dx);
   const Operand x = stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, a->order, live);
   const Operand w = stage<T>(a->w, a->ldw, a->n, a->k, f.w, s);
-  const int wide = a->k % 4 == 0, four = 4 * sizeof(T);
   for (int64_t v0 = 0; v0 < a->n; v0 += f.piece) {
     const int64_t nv = a->n - v0 < f.piece ? a->n - v0 : f.piece, ld = up8(nv);
     Operand wv = w;
@@ -294,22 +293,22 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
       const bool last = v0 + nv == a->n;
       Product g = {dz, wv, a->rows, a->k, nv, live, 0, 1, 0, 0};
       const float* before = v0 ? (const float*)f.sum : nullptr;
+      const int sum_wide = wide8<float>(f.sum, a->k);
       if (last)
-        rc = launch_out<T, StoreOut<T>, false, true, EpiStore, T>(g, f.px, {(T*)a->dx, before, scale + 1, a->order, a->k, wide && (uintptr_t)a->dx % four == 0},
-                                                                 (float*)f.part, (const T*)nullptr, s);
+        rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, before, scale + 1, a->order, a->k, wide8<T>(a->dx, a->k), sum_wide}, f.part, s);
       else
-        rc = launch_out<T, StoreOut<float>, false, true, EpiStore, float>(g, f.px, {(float*)f.sum, before, nullptr, nullptr, a->k, wide}, (float*)f.part, (const float*)nullptr, s);
+        rc = launch_out<T, false, true>(g, f.px, StoreOut<float>{nullptr, (float*)f.sum, before, nullptr, nullptr, a->k, sum_wide, sum_wide}, f.part, s);
       if (rc != CLID_OK) return rc;
     }
     if (a->dw) {
       T* to = (T*)a->dw + v0 * a->k;
       Product g = {dz, x, nv, a->k, a->rows, live, 1, 1, 0, 0};
-      rc = launch_out<T, StoreOut<T>, true, true, EpiStore, T>(g, f.pw, {to, nullptr, scale + 1, nullptr, a->k, wide && (uintptr_t)to % four == 0}, (float*)f.part, (const T*)nullptr, s);
+      rc = launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, to, nullptr, scale + 1, nullptr, a->k, wide8<T>(to, a->k), 0}, f.part, s);
       if (rc != CLID_OK) return rc;
     }
     if (a->db) {
       hipLaunchKernelGGL(k_colsum<T>, dim3((unsigned)((ld + 255) / 256), f.blocks), dim3(256), 0, s, (const uint16_t*)f.dz, a->rows, live, (int)nv, (int)ld, a->rows * ld, (float*)f.sums);
-      hipLaunchKernelGGL(k_colsum_join<T>, dim3((unsigned)((nv + 63) / 64)), dim3(256), 0, s, (const float*)f.sums, f.blocks, (int)nv, (const float*)(scale + 1), (T*)a->db + v0);
+      hipLaunchKernelGGL(k_colsum_join<T>, dim3((unsigned)((nv + 63) / 64)), dim3(1024), 0, s, (const float*)f.sums, f.blocks, (int)nv, (const float*)(scale + 1), (T*)a->db + v0);
     }
   }
   return CLID_OK;

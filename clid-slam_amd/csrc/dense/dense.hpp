@@ -33,12 +33,31 @@ template <> __device__ __forceinline__ f16 down<f16>(float v) { return __float2h
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
 // ---- activations: act(z) and its slope, in fp32 ------------------------------------------------------------------------
+// Phi(z) by the Chebyshev fit of erfc(x) = t exp(-x^2 + p(t)), t = 2 / (2 + x), of Press et al., Numerical Recipes, 6.2 (relative
+// error 1.2e-7 for x >= 0): one exp, one reciprocal and nine FMAs without a branch, where the library's erf takes two branches.
+__device__ __forceinline__ float normal_cdf(float z) {
+  const float x = fabsf(z) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(fmaf(0.5f, x, 1.f));
+  float p = 0.17087277f;
+  p = fmaf(p, t, -0.82215223f);
+  p = fmaf(p, t, 1.48851587f);
+  p = fmaf(p, t, -1.13520398f);
+  p = fmaf(p, t, 0.27886807f);
+  p = fmaf(p, t, -0.18628806f);
+  p = fmaf(p, t, 0.09678418f);
+  p = fmaf(p, t, 0.37409196f);
+  p = fmaf(p, t, 1.00002368f);
+  p = fmaf(p, t, -1.26551223f);
+  const float half = 0.5f * t * __builtin_amdgcn_exp2f(fmaf(-x, x, p) * 1.4426950408889634f);
+  return z < 0.f ? half : 1.f - half;
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(z * -1.4426950408889634f)); }
+
 __device__ __forceinline__ float act_value(float z, int act) {
   switch (act) {
     case CLID_ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
     case CLID_ACT_LEAKY_RELU: return z > 0.f ? z : 0.01f * z;
-    case CLID_ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case CLID_ACT_SILU: return z / (1.f + expf(-z));
+    case CLID_ACT_GELU: return z * normal_cdf(z);
+    case CLID_ACT_SILU: return z * sigmoid(z);
     default: return z;
   }
 }
@@ -46,9 +65,9 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   switch (act) {
     case CLID_ACT_RELU: return z > 0.f ? 1.f : 0.f;
     case CLID_ACT_LEAKY_RELU: return z > 0.f ? 1.f : 0.01f;
-    case CLID_ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * expf(-0.5f * z * z) * 0.3989422804014327f;
+    case CLID_ACT_GELU: return fmaf(z * 0.3989422804014327f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f), normal_cdf(z));
     case CLID_ACT_SILU: {
-      const float p = 1.f / (1.f + expf(-z));
+      const float p = sigmoid(z);
       return p * (1.f + z * (1.f - p));
     }
     default: return 1.f;

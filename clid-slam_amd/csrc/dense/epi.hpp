@@ -1,69 +1,101 @@
 // What the tiles' sums become: a layer's output, a gradient, a row's softmax statistics, a piece of dz.
-// Each is called with one lane's 16 TN sums of a row m: element (i, r) is column nw + 32 i + 8 (r / 4) + 4 half + r % 4.
+// Each gets 32 rows of a wave's sums: lane l holds row m_first + l % 32, its element (i, r) column nw + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4.
 #pragma once
 #include "tile.hpp"
 
 namespace clid_dense {
 
-template <typename T> struct Four;  // four neighbouring values of a type as one load or store
-template <> struct Four<float> { using V = float4; };
-template <> struct Four<bf16> { using V = ushort4; };
-template <> struct Four<f16> { using V = ushort4; };
-
+// 8 neighbouring values of a row, wide where the row allows it (rows whose starts and lengths are multiples of 16 bytes)
 template <typename T>
-__device__ __forceinline__ void put4(T* p, const float (&v)[4], int count, bool wide) {
-  if (wide && count >= 4) {
-    union { typename Four<T>::V w; T t[4]; } u;
+__device__ __forceinline__ void get8(const T* p, float (&v)[8], int count, bool wide) {
+  if (wide && count >= 8) {
+    union { uint4 w[sizeof(T) / 2]; T t[8]; } u;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) u.t[q] = down<T>(v[q]);
-    *(typename Four<T>::V*)p = u.w;
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.w[i] = ((const uint4*)p)[i];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = up(u.t[q]);
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < count) p[q] = down<T>(v[q]);
+    for (int q = 0; q < 8; ++q) v[q] = q < count ? up(p[q]) : 0.f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void get4(const T* p, float (&v)[4], int count, bool wide) {
-  if (wide && count >= 4) {
-    union { typename Four<T>::V w; T t[4]; } u;
-    u.w = *(const typename Four<T>::V*)p;
+__device__ __forceinline__ void out8(T* p, const T (&t)[8], int count, bool wide) {
+  if (wide && count >= 8) {
+    union { uint4 w[sizeof(T) / 2]; T t[8]; } u;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = up(u.t[q]);
+    for (int q = 0; q < 8; ++q) u.t[q] = t[q];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4*)p)[i] = u.w[i];
   } else {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = q < count ? up(p[q]) : 0.f;
+    for (int q = 0; q < 8; ++q)
+      if (q < count) p[q] = t[q];
   }
 }
+template <typename T>
+inline bool wide8(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % (16 / (int64_t)sizeof(T)) == 0; }
 
-// z + bias -> act -> + residual -> y, and z for the backward pass; also behind a sum over splits (k_join)
+// z + bias -> act -> + residual -> y, and z for the backward pass
 template <typename T>
 struct LinearOut {
   const T *bias, *res;
   T *y, *z;
   int64_t ldr, n;
-  int act, wide, res_wide;  // 4 neighbouring values of y and z (of res) are one aligned store (load)
-  // (v: four sums at row m, column c)
-  __device__ __forceinline__ void four(float (&v)[4], const float (&b)[4], int64_t m, int64_t c) const {
-    const int count = (int)(n - c < 4 ? n - c : 4);
+  int act, wide, res_wide;
+  // v: sums at row m, columns c ..; b: their bias
+  __device__ __forceinline__ void eight(float (&v)[8], const float (&b)[8], int64_t m, int64_t c, int) const {
+    const int count = (int)(n - c < 8 ? n - c : 8);
     if (count <= 0) return;
-    float r[4] = {0.f, 0.f, 0.f, 0.f};
-    if (res) get4(res + m * ldr + c, r, count, res_wide);
+    float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (res) get8(res + m * ldr + c, r, count, res_wide);
+    T t[8];
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] += b[q];
+    for (int q = 0; q < 8; ++q) v[q] += b[q];
     if (z) {
-      if (wide && count >= 4) {
-        union { typename Four<T>::V w; T t[4]; } u;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) u.t[q] = keep_z<T>(v[q]);
-        *(typename Four<T>::V*)(z + m * n + c) = u.w;
-      } else {
-        for (int q = 0; q < count; ++q) z[m * n + c + q] = keep_z<T>(v[q]);
-      }
+      for (int q = 0; q < 8; ++q) t[q] = keep_z<T>(v[q]);
+      out8(z + m * n + c, t, count, wide);
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = act_value(v[q], act) + r[q];
-    put4(y + m * n + c, v, count, wide);
+    for (int q = 0; q < 8; ++q) t[q] = down<T>(act_value(v[q], act) + r[q]);
+    out8(y + m * n + c, t, count, wide);
+  }
+};
+
+// out[order ? order[m] : m] = alpha (sum + add)
+template <typename T>
+struct StoreOut {
+  const T* bias;  // none
+  T* out;
+  const float *add, *alpha;  // add: [m][n] fp32 of the pieces before
+  const int32_t* order;
+  int64_t n;
+  int wide, add_wide;
+  __device__ __forceinline__ void eight(float (&v)[8], const float (&)[8], int64_t m, int64_t c, int) const {
+    const int count = (int)(n - c < 8 ? n - c : 8);
+    if (count <= 0) return;
+    if (add) {
+      float a[8];
+      get8(add + m * n + c, a, count, add_wide);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[q] += a[q];
+    }
+    const float s = alpha ? *alpha : 1.f;
+    T t[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) t[q] = down<T>(v[q] * s);
+    out8(out + (order ? (int64_t)order[m] : m) * n + c, t, count, wide);
+  }
+};
+
+// part[split][m][n8] = sum over this block's share of k (n8: n up to 8)
+struct PartOut {
+  const float* bias;  // none
+  float* part;
+  int64_t m_all, n8;
+  __device__ __forceinline__ void eight(float (&v)[8], const float (&)[8], int64_t m, int64_t c, int split) const {
+    if (c < n8) out8(part + ((int64_t)split * m_all + m) * n8 + c, v, 8, true);
   }
 };
 
@@ -73,100 +105,74 @@ __device__ __forceinline__ void stage_bias(const T* bias, int64_t n0, int64_t n,
   for (int c = threadIdx.x; c < cols; c += blockDim.x) ((float*)lds)[c] = bias && n0 + c < n ? up(bias[n0 + c]) : 0.f;
 }
 
-template <typename T, int BN>
-struct EpiLinear {
-  LinearOut<T> o;
-  __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(o.bias, n0, o.n, BN, lds); }
-  template <int TN>
-  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m, bool on, int64_t nw, int64_t n, int half, int, const char* lds, int at) const {
-    if (!on) return;
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = 32 * i + 8 * j + 4 * half;
-        const float4 b4 = *(const float4*)(lds + (at + c) * 4);
-        float v[4] = {acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
-        const float b[4] = {b4.x, b4.y, b4.z, b4.w};
-        o.four(v, b, m, nw + c);
-      }
-  }
-};
-
-// out[order ? order[m] : m] = alpha sum + add
-template <typename T>
-struct StoreOut {
-  T* out;
-  const float *add, *alpha;  // add: [m][n] fp32 of the pieces before
-  const int32_t* order;
+// Sums handed on in rows: 32 rows of a wave go through its LDS once, so that 4 TN neighbouring lanes hold 8 columns each of one row and
+// loads and stores are 16 bytes wide; one loop then does whatever there is to do, where the registers' own order would need the
+// code once per register.
+template <class Out, int BN>
+struct EpiRows {
+  static constexpr bool kThroughLds = true;
+  Out o;
   int64_t n;
-  int wide;
-  __device__ __forceinline__ void four(float (&v)[4], const float (&)[4], int64_t m, int64_t c) const {
-    const int count = (int)(n - c < 4 ? n - c : 4);
-    if (count <= 0) return;
-    if (add) {
-      float a[4];
-      get4(add + m * n + c, a, count, n % 4 == 0);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) v[q] += a[q];
-    }
-    const float s = alpha ? *alpha : 1.f;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] *= s;
-    put4(out + (order ? (int64_t)order[m] : m) * n + c, v, count, wide);
-  }
-};
-template <typename T, int BN>
-struct EpiStore {
-  StoreOut<T> o;
-  __device__ __forceinline__ void prepare(int64_t, char*) const {}
+  __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(o.bias, n0, n, BN, lds); }
   template <int TN>
-  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m, bool on, int64_t nw, int64_t, int half, int, const char*, int) const {
-    if (!on) return;
-    const float b[4] = {0.f, 0.f, 0.f, 0.f};
+  __device__ __forceinline__ void rows(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int split, int lane, const char* bias, char* lds) const {
+    constexpr int kRow = 32 * TN + 4, kLanes = 4 * TN, kStep = 64 / kLanes;
+    float* mine = (float*)lds;
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        float v[4] = {acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
-        o.four(v, b, m, nw + 32 * i + 8 * j + 4 * half);
-      }
-  }
-};
-
-// part[split][m][n4] = sum over this block's share of k (n4: n up to 4)
-template <int BN>
-struct EpiPart {
-  float* part;
-  int64_t m, n4;
-  __device__ __forceinline__ void prepare(int64_t, char*) const {}
-  template <int TN>
-  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t mm, bool on, int64_t nw, int64_t, int half, int split, const char*, int) const {
-    if (!on) return;
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t c = nw + 32 * i + 8 * j + 4 * half;
-        if (c < n4) *(float4*)(part + ((int64_t)split * m + mm) * n4 + c) = float4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
-      }
-  }
-};
-
-// the splits' sums joined in their order, four columns a thread, and handed on
-template <typename T, class Out>
-__global__ void __launch_bounds__(256) k_join(const float* part, int splits, int64_t m, int64_t n4, const int32_t* live, const T* bias, Out o) {
-  const int64_t rows = live && *live < m ? *live : m;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * (n4 / 4); i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / (n4 / 4), c = (i - r * (n4 / 4)) * 4;
-    float v[4] = {0.f, 0.f, 0.f, 0.f}, b[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int s = 0; s < splits; ++s) {
-      const float4 p = *(const float4*)(part + ((int64_t)s * m + r) * n4 + c);
-      v[0] += p.x; v[1] += p.y; v[2] += p.z; v[3] += p.w;
+      for (int j = 0; j < 4; ++j)
+        *(float4*)(mine + (lane & 31) * kRow + 32 * i + 8 * j + 4 * (lane >> 5)) = float4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
+    __builtin_amdgcn_wave_barrier();
+    const int c = (lane % kLanes) * 8;
+    float b[8];
+    *(float4*)b = *(const float4*)(bias + (at + c) * 4);
+    *(float4*)(b + 4) = *(const float4*)(bias + (at + c) * 4 + 16);
+#pragma unroll 1
+    for (int r = lane / kLanes; r < 32; r += kStep) {
+      float v[8];
+      *(float4*)v = *(const float4*)(mine + r * kRow + c);
+      *(float4*)(v + 4) = *(const float4*)(mine + r * kRow + c + 4);
+      if (m_first + r < m_end) o.eight(v, b, m_first + r, nw + c, split);
     }
-    if (bias)
-      for (int q = 0; q < 4; ++q) b[q] = c + q < o.n ? up(bias[c + q]) : 0.f;
-    o.four(v, b, r, c);
+    __builtin_amdgcn_wave_barrier();
+  }
+};
+
+// the splits' sums joined in their order and handed on: 8 columns a thread, G threads of a block share them by split
+template <typename T, class Out, int G>
+__global__ void __launch_bounds__(256) k_join(const float* part, int splits, int64_t m, int64_t n8, const int32_t* live, Out o) {
+  __shared__ float sums[G][256 / G][9];
+  const int64_t rows = live && *live < m ? *live : m, per = n8 / 8;
+  const int t = threadIdx.x % (256 / G), g = threadIdx.x / (256 / G), share = (splits + G - 1) / G;
+  const int from = g * share, to = from + share < splits ? from + share : splits;
+  for (int64_t i0 = (int64_t)blockIdx.x * (256 / G); i0 < rows * per; i0 += (int64_t)gridDim.x * (256 / G)) {
+    const int64_t i = i0 + t, r = i / per, c = (i - r * per) * 8;
+    float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (i < rows * per)
+#pragma unroll 4
+      for (int s = from; s < to; ++s) {
+        const float4* p = (const float4*)(part + ((int64_t)s * m + r) * n8 + c);
+        const float4 a = p[0], b = p[1];
+        v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+        v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+      }
+    if constexpr (G > 1) {
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < 8; ++q) sums[g][t][q] = v[q];
+      __syncthreads();
+      if (g) continue;
+      for (int s = 1; s < G; ++s)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] += sums[s][t][q];
+    }
+    if (i >= rows * per) continue;
+    float b[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) b[q] = o.bias && c + q < o.n ? up(o.bias[c + q]) : 0.f;
+    o.eight(v, b, r, c, 0);
   }
 }
 
@@ -181,9 +187,13 @@ struct EpiStat {
   int32_t* part_at;
   float* zt;
   int64_t m_all, n;
+  static constexpr bool kThroughLds = false;
   __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(bias, n0, n, BN, lds); }
   template <int TN>
-  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m, bool on, int64_t nw, int64_t, int half, int, const char* lds, int at) const {
+  __device__ __forceinline__ void rows(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int, int lane, const char* lds, char*) const {
+    const int half = lane >> 5;
+    const int64_t m = m_first + (lane & 31);
+    const bool on = m < m_end;
     if (nw >= n) return;
     int t = -1;
     if constexpr (!LABEL) {
@@ -272,10 +282,13 @@ struct EpiDz {
   const float* g;      // per-row factor, by original row, or NULL
   uint16_t* dz;
   int64_t v0, n, ld, plane;  // columns v0 .. v0 + n, ld: n up to 8 (zeros there)
+  static constexpr bool kThroughLds = false;
   __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(bias, n0, n, BN, lds); }
   template <int TN>
-  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m, bool on, int64_t nw, int64_t, int half, int, const char* lds, int at) const {
-    if (!on) return;
+  __device__ __forceinline__ void rows(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int, int lane, const char* lds, char*) const {
+    const int half = lane >> 5;
+    const int64_t m = m_first + (lane & 31);
+    if (m >= m_end) return;
     const int64_t from = order[m];
     const float4 s = stat[m];
     const int64_t tt = target[from] - v0 - nw;

@@ -16,7 +16,7 @@ struct Fwd {
     x = ws.take(stage_bytes<T>(a->x, a->ldx, a->rows, a->k));
     w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
     p = plan<Kind<T>::NP>(a->rows, a->n, a->k, true);
-    part = ws.take(part_bytes<Kind<T>::NP>(p, a->rows, a->n));
+    part = ws.take(part_bytes(p, a->rows, a->n));
     bytes = ws.used;
   }
 };
@@ -25,10 +25,9 @@ template <typename T>
 int fwd(const clid_linear_args* a, hipStream_t s) {
   const Fwd<T> f(a);
   Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
-  const int64_t four = 4 * sizeof(T);
   LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (T*)a->z_out, a->ldr, a->n, a->act,
-                    a->n % 4 == 0 && (uintptr_t)a->y % four == 0 && (uintptr_t)a->z_out % four == 0, a->ldr % 4 == 0 && (uintptr_t)a->residual % four == 0};
-  return launch_out<T, LinearOut<T>, false, false, EpiLinear, T>(g, f.p, o, (float*)f.part, (const T*)a->bias, s);
+                    wide8<T>(a->y, a->n) && wide8<T>(a->z_out, a->n), wide8<T>(a->residual, a->ldr)};
+  return launch_out<T, false, false>(g, f.p, o, f.part, s);
 }
 
 template <typename T>
@@ -48,7 +47,7 @@ struct Bwd {
     sums = ws.take(a->db ? (int64_t)blocks * a->n * 4 : 0);
     px = plan<Kind<T>::NP>(a->rows, a->k, a->n, true);
     pw = plan<Kind<T>::NP>(a->n, a->k, a->rows, true);
-    const int64_t bx = a->dx ? part_bytes<Kind<T>::NP>(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes<Kind<T>::NP>(pw, a->n, a->k) : 0;
+    const int64_t bx = a->dx ? part_bytes(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes(pw, a->n, a->k) : 0;
     part = ws.take(bx > bw ? bx : bw);
     bytes = ws.used;
   }
@@ -66,19 +65,16 @@ int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
                        (int)wide8<T>(a->dy, a->lddy), (int)wide8<T>(a->z, a->n), f.own_dz ? (uint16_t*)f.dz : nullptr, np, a->rows * np,
                        a->db ? (float*)f.sums : nullptr);
     if (a->db)
-      hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(256), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
+      hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
   }
-  const int wide = a->k % 4 == 0;
   if (a->dx) {
     Product g = {dz, stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->k, a->n, nullptr, 0, 1, 0, 0};
-    StoreOut<T> o = {(T*)a->dx, nullptr, nullptr, nullptr, a->k, wide && (uintptr_t)a->dx % (4 * sizeof(T)) == 0};
-    const int rc = launch_out<T, StoreOut<T>, false, true, EpiStore, T>(g, f.px, o, (float*)f.part, (const T*)nullptr, s);
+    const int rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, nullptr, nullptr, nullptr, a->k, wide8<T>(a->dx, a->k), 0}, f.part, s);
     if (rc != CLID_OK) return rc;
   }
   if (a->dw) {
     Product g = {dz, stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), a->n, a->k, a->rows, nullptr, 0, 1, 0, 0};
-    StoreOut<T> o = {(T*)a->dw, nullptr, nullptr, nullptr, a->k, wide && (uintptr_t)a->dw % (4 * sizeof(T)) == 0};
-    return launch_out<T, StoreOut<T>, true, true, EpiStore, T>(g, f.pw, o, (float*)f.part, (const T*)nullptr, s);
+    return launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, (T*)a->dw, nullptr, nullptr, nullptr, a->k, wide8<T>(a->dw, a->k), 0}, f.part, s);
   }
   return CLID_OK;
 }

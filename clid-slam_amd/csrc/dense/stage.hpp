@@ -15,20 +15,6 @@ template <> struct Kind<f16> { static constexpr int NP = 1; static constexpr boo
 inline int64_t up8(int64_t v) { return (v + 7) & ~int64_t(7); }
 constexpr int64_t kLdMost = int64_t(1) << 22;  // a tile's offsets stay under 2^31 bytes
 
-// 8 neighbouring values of a row, wide where the row allows it
-template <typename T>
-__device__ __forceinline__ void get8(const T* p, float (&v)[8], int count, bool wide) {
-  if (wide && count >= 8) {
-    union { uint4 w[sizeof(T) / 2]; T t[8]; } u;
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.w[i] = ((const uint4*)p)[i];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = up(u.t[q]);
-  } else {
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = q < count ? up(p[q]) : 0.f;
-  }
-}
 // 8 values as the planes of T at to (aligned to 16 bytes)
 template <typename T>
 __device__ __forceinline__ void put8(uint16_t* to, int64_t plane, const float (&v)[8]) {
@@ -50,9 +36,6 @@ __device__ __forceinline__ void put8(uint16_t* to, int64_t plane, const float (&
     for (int s = 0; s < 3; ++s) *(uint4*)(to + s * plane) = u[s].w;
   }
 }
-template <typename T>
-inline bool wide8(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % (16 / (int64_t)sizeof(T)) == 0; }
-
 // rows of src (in `order`, as many as are live) -> planes with rows of kp values, zeros behind k
 template <typename T>
 __global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t rows, int k, const int32_t* order, const int32_t* live, int wide,
@@ -157,17 +140,20 @@ __global__ void __launch_bounds__(256) k_colsum(const uint16_t* src, int64_t row
     part[(int64_t)blockIdx.y * n + col] = s;
   }
 }
-// 64 columns a block, 4 threads a column
+// 64 columns a block, 16 threads a column
 template <typename T>
-__global__ void __launch_bounds__(256) k_colsum_join(const float* part, int blocks, int n, const float* alpha, T* out) {
-  __shared__ float p[4][64];
+__global__ void __launch_bounds__(1024) k_colsum_join(const float* part, int blocks, int n, const float* alpha, T* out) {
+  __shared__ float p[16][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
   float s = 0.f;
   if (c < n)
-    for (int b = g; b < blocks; b += 4) s += part[(int64_t)b * n + c];
+#pragma unroll 4
+    for (int b = g; b < blocks; b += 16) s += part[(int64_t)b * n + c];
   p[g][threadIdx.x & 63] = s;
   __syncthreads();
-  if (g == 0 && c < n) out[c] = down<T>((alpha ? *alpha : 1.f) * (p[0][threadIdx.x] + p[1][threadIdx.x] + p[2][threadIdx.x] + p[3][threadIdx.x]));
+  if (g || c >= n) return;
+  for (int i = 1; i < 16; ++i) s += p[i][threadIdx.x];
+  out[c] = down<T>((alpha ? *alpha : 1.f) * s);
 }
 inline int row_blocks(int64_t rows, int n) {
   const int64_t cols = (n + 255) / 256, want = 1024 / cols + 1, most = (rows + 63) / 64;
@@ -191,30 +177,33 @@ inline void tile_shape(int size, int* bm, int* bn, int* bk) {
 
 constexpr int kCus = 256;
 
-// Which tile, and into how many parts k is cut.  The largest tile that still gives every CU one; where even the smallest leaves
-// CUs idle, k is cut while each part keeps 8 steps (a part costs its sums' trip through memory).
+// Which tile, and into how many parts k is cut: the cheapest by an estimate of the time.  A CU works through its blocks one
+// after the other (rounds of 256 blocks) at a rate that grows with the tile, since a larger tile reads less LDS and memory per
+// product; a part costs its sums' trip through memory and back, and a launch.
 struct Plan {
   int size, splits;
 };
 template <int NP>
 inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
-  Plan p = {0, 1};
-  int bm, bn, bk;
-  for (int size = 2; size >= 0; --size) {
+  const double rate[3] = {1.1e12, 2.6e12, 4.4e12};  // plane products' FLOP/s of a CU with tiles 0, 1, 2
+  Plan best = {0, 1};
+  double least = 1e300;
+  for (int size = 0; size <= 2; ++size) {
+    int bm, bn, bk;
     tile_shape<NP>(size, &bm, &bn, &bk);
-    p.size = size;
-    if (((m + bm - 1) / bm) * ((n + bn - 1) / bn) >= kCus) return p;
+    const int64_t tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn), steps = (k + bk - 1) / bk;
+    for (int s = 1; s <= (may_split ? 64 : 1) && (s == 1 || s * 4 <= steps); s += s < 8 ? 1 : 8) {
+      const double rounds = (double)((tiles * s + kCus - 1) / kCus);
+      const double share = (double)((steps + s - 1) / s) * bk;
+      double t = rounds * (2.0 * bm * bn * share * (NP == 3 ? 6 : 1) / rate[size] + 1.5e-6);
+      if (s > 1) t += 4e-6 + (double)s * m * n * 8 / 4e12;
+      if (t < least) {
+        least = t;
+        best = {size, s};
+      }
+    }
   }
-  if (!may_split) return p;
-  // cut the tile in the middle: its operands' traffic is half the smallest one's
-  p.size = m > 64 && n > 64 ? 1 : 0;
-  tile_shape<NP>(p.size, &bm, &bn, &bk);
-  const int64_t tiles = ((m + bm - 1) / bm) * ((n + bn - 1) / bn), steps = (k + bk - 1) / bk;
-  int64_t s = (2 * kCus + tiles - 1) / tiles;
-  if (s > steps / 8) s = steps / 8;
-  if (s > 64) s = 64;
-  p.splits = s < 1 ? 1 : (int)s;
-  return p;
+  return best;
 }
 
 template <typename T, int SIZE, bool PKS, bool QKS, class Epi>
@@ -246,24 +235,26 @@ inline int launch_one(Product g, const Epi& epi, hipStream_t s) {
   return CLID_OK;
 }
 
-template <typename T, class Out, bool PKS, bool QKS, template <typename, int> class Epi, typename TO>
-inline int launch_out(Product g, const Plan& p, const Out& o, float* part, const TO* bias, hipStream_t s) {
-  g.splits = p.splits;
-  if (p.splits > 1) {
-    const int64_t n4 = (g.n + 3) / 4 * 4;
-    int rc;
-    if (p.size == 1) rc = launch_one<T, 1, PKS, QKS>(g, EpiPart<Tile<Kind<T>::NP, 1>::BN>{part, g.m, n4}, s);
-    else rc = launch_one<T, 0, PKS, QKS>(g, EpiPart<Tile<Kind<T>::NP, 0>::BN>{part, g.m, n4}, s);
-    if (rc != CLID_OK) return rc;
-    hipLaunchKernelGGL((k_join<TO, Out>), grid_for(g.m * n4 / 4), dim3(256), 0, s, part, p.splits, g.m, n4, g.live_k ? nullptr : g.live, bias, o);
-    return CLID_OK;
-  }
-  if (p.size == 2) return launch_one<T, 2, PKS, QKS>(g, Epi<TO, Tile<Kind<T>::NP, 2>::BN>{o}, s);
-  if (p.size == 1) return launch_one<T, 1, PKS, QKS>(g, Epi<TO, Tile<Kind<T>::NP, 1>::BN>{o}, s);
-  return launch_one<T, 0, PKS, QKS>(g, Epi<TO, Tile<Kind<T>::NP, 0>::BN>{o}, s);
+template <typename T, bool PKS, bool QKS, class Out>
+inline int launch_rows(const Product& g, int size, const Out& o, hipStream_t s) {
+  constexpr int NP = Kind<T>::NP;
+  if (size == 2) return launch_one<T, 2, PKS, QKS>(g, EpiRows<Out, Tile<NP, 2>::BN>{o, g.n}, s);
+  if (size == 1) return launch_one<T, 1, PKS, QKS>(g, EpiRows<Out, Tile<NP, 1>::BN>{o, g.n}, s);
+  return launch_one<T, 0, PKS, QKS>(g, EpiRows<Out, Tile<NP, 0>::BN>{o, g.n}, s);
 }
-template <int NP>
-inline int64_t part_bytes(const Plan& p, int64_t m, int64_t n) { return p.splits > 1 ? up256(p.splits * m * ((n + 3) / 4 * 4) * 4) : 0; }
+template <typename T, bool PKS, bool QKS, class Out>
+inline int launch_out(Product g, const Plan& p, const Out& o, char* part, hipStream_t s) {
+  g.splits = p.splits;
+  if (p.splits == 1) return launch_rows<T, PKS, QKS>(g, p.size, o, s);
+  const int64_t n8 = up8(g.n);
+  const int rc = launch_rows<T, PKS, QKS>(g, p.size, PartOut{nullptr, (float*)part, g.m, n8}, s);
+  if (rc != CLID_OK) return rc;
+  const int32_t* live = g.live_k ? nullptr : g.live;
+  if (p.splits > 8) hipLaunchKernelGGL((k_join<T, Out, 8>), grid_for(g.m * n8), dim3(256), 0, s, (const float*)part, p.splits, g.m, n8, live, o);
+  else hipLaunchKernelGGL((k_join<T, Out, 1>), grid_for(g.m * n8 / 8), dim3(256), 0, s, (const float*)part, p.splits, g.m, n8, live, o);
+  return CLID_OK;
+}
+inline int64_t part_bytes(const Plan& p, int64_t m, int64_t n) { return p.splits > 1 ? up256(p.splits * m * up8(n) * 4) : 0; }
 
 // the workspace handed out front to back; sizes and pointers come from one walk, so they cannot differ
 struct Ws {

@@ -150,6 +150,9 @@ struct Side {
   }
 };
 
+// LDS of one wave for 32 rows of its sums, a row 4 floats longer than its columns: neighbouring rows start 4 banks apart
+template <int TN> constexpr int kRowsLds = 32 * (32 * TN + 4) * 4;
+
 // (tile row, tile column) of tile t
 __device__ __forceinline__ void place_tile(const Product& g, int64_t block, int64_t blocks, int* tm, int* tn) {
   constexpr int64_t kXcd = 8, kCols = 8;
@@ -233,14 +236,12 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
     if (s + 1 < steps) load(s + 1, lds + ((s + 1) & 1) * kStage);
     multiply(lds + (s & 1) * kStage);
   }
-  if (steps == 0) __syncthreads();  // what prepare() left in LDS
+  if (Epi::kThroughLds || steps == 0) __syncthreads();  // LDS is the epilogue's; what prepare() left there is seen
 
-  const int half = lane >> 5;
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
-    const int64_t m = m0 + (wm * TM + j) * 32 + (lane & 31);
-    const int64_t nw = n0 + wn * TN * 32;
-    epi.template row<TN>(acc[j], m, m < rows_m, nw, g.n, half, split, lds + 2 * kStage, (int)(nw - n0));
+    const int64_t m_first = m0 + (wm * TM + j) * 32;
+    epi.template rows<TN>(acc[j], m_first, rows_m, n0 + wn * TN * 32, wn * TN * 32, split, lane, lds + 2 * kStage, lds + wave * kRowsLds<TN>);
   }
 }
 
