@@ -347,6 +347,7 @@ int label(const clid_label_args* a, hipStream_t s) {
 
 extern "C" int64_t clid_ce_workspace(const clid_ce_args* a) {
   if (!ce_ok(a)) return bad("clid_ce_workspace", "bad argument");
+  if (is_narrow(a->k, a->n) && a->rows) return narrow_ce_bytes(a);
   BY_DTYPE(a->dtype, return CeFwd<T>(a).bytes;);
 }
 extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
@@ -358,13 +359,15 @@ extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
   const int64_t need = clid_ce_workspace(a);
   if (a->rows && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
   int rc = CLID_OK;
-  BY_DTYPE(a->dtype, rc = ce_fwd<T>(a, (hipStream_t)stream););
+  if (is_narrow(a->k, a->n) && a->rows) rc = narrow_ce(a, (hipStream_t)stream);
+  else BY_DTYPE(a->dtype, rc = ce_fwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);
   return CLID_OK;
 }
 extern "C" int64_t clid_ce_bwd_workspace(const clid_ce_args* a) {
   if (!ce_ok(a)) return bad("clid_ce_bwd_workspace", "bad argument");
+  if (is_narrow(a->k, a->n)) return narrow_ce_bwd_bytes(a);
   BY_DTYPE(a->dtype, return CeBwd<T>(a).bytes;);
 }
 extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
@@ -375,7 +378,8 @@ extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
   const int64_t need = clid_ce_bwd_workspace(a);
   if (!a->ws || a->ws_bytes < need) return bad(me, "workspace too small");
   int rc = CLID_OK;
-  BY_DTYPE(a->dtype, rc = ce_bwd<T>(a, (hipStream_t)stream););
+  if (is_narrow(a->k, a->n)) rc = narrow_ce_bwd(a, (hipStream_t)stream);
+  else BY_DTYPE(a->dtype, rc = ce_bwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);
   return CLID_OK;
@@ -383,6 +387,7 @@ extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
 
 extern "C" int64_t clid_label_workspace(const clid_label_args* a) {
   if (!label_ok(a)) return bad("clid_label_workspace", "bad argument");
+  if (is_narrow(a->k, a->n)) return 0;
   BY_DTYPE(a->dtype, return Label<T>(a).bytes;);
 }
 extern "C" int clid_label_fwd(const clid_label_args* a, void* stream) {
@@ -391,9 +396,10 @@ extern "C" int clid_label_fwd(const clid_label_args* a, void* stream) {
   if (a->rows == 0) return CLID_OK;
   if (!a->x || !a->w || !a->label || !a->log_prob || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
   const int64_t need = clid_label_workspace(a);
-  if (!a->ws || a->ws_bytes < need) return bad(me, "workspace too small");
+  if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
   int rc = CLID_OK;
-  BY_DTYPE(a->dtype, rc = label<T>(a, (hipStream_t)stream););
+  if (is_narrow(a->k, a->n)) rc = narrow_label(a, (hipStream_t)stream);
+  else BY_DTYPE(a->dtype, rc = label<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);
   return CLID_OK;

@@ -90,6 +90,7 @@ bool args_ok(const clid_linear_bwd_args* a) {
 
 extern "C" int64_t clid_linear_workspace(const clid_linear_args* a) {
   if (!args_ok(a)) return bad("clid_linear_workspace", "bad argument");
+  if (is_narrow(a->k, a->n)) return 0;
   BY_DTYPE(a->dtype, return Fwd<T>(a).bytes;);
 }
 extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
@@ -100,7 +101,8 @@ extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
   const int64_t need = clid_linear_workspace(a);
   if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
   int rc = CLID_OK;
-  BY_DTYPE(a->dtype, rc = fwd<T>(a, (hipStream_t)stream););
+  if (is_narrow(a->k, a->n)) rc = narrow_linear(a, (hipStream_t)stream);
+  else BY_DTYPE(a->dtype, rc = fwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);
   return CLID_OK;
@@ -108,6 +110,7 @@ extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
 
 extern "C" int64_t clid_linear_bwd_workspace(const clid_linear_bwd_args* a) {
   if (!args_ok(a)) return bad("clid_linear_bwd_workspace", "bad argument");
+  if (is_narrow(a->k, a->n)) return narrow_linear_bwd_bytes(a);
   BY_DTYPE(a->dtype, return Bwd<T>(a).bytes;);
 }
 extern "C" int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream) {
@@ -118,7 +121,8 @@ extern "C" int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream) {
   const int64_t need = clid_linear_bwd_workspace(a);
   if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
   int rc = CLID_OK;
-  BY_DTYPE(a->dtype, rc = bwd<T>(a, (hipStream_t)stream););
+  if (is_narrow(a->k, a->n)) rc = narrow_linear_bwd(a, (hipStream_t)stream);
+  else BY_DTYPE(a->dtype, rc = bwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);
   return CLID_OK;

@@ -1,0 +1,600 @@
+// The dense operators at a point decoder's own widths, n <= 64 and k <= 64: memory bound, so x is read once and everything else happens in
+// registers.
+//
+// A wave takes 32 rows at a time; the weight lies in LDS.  z = x w^T on the fp32 matrix instruction (32 x 32 x 2) with the rows of w as its
+// row operand: a lane then holds one row m of x and of z, element (i, r) being column 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4.  A row's
+// softmax is 16 or 32 registers and one exchange between two lanes, with no partial results in memory.  The same registers are the
+// column operand of dx = dz w as they are (the contraction over n takes its columns in that order, and so does the row operand, read from
+// w in LDS).  dw = dz^T x contracts over m: dz goes through LDS once, x is there already; the sums over a wave's rows stay in
+// accumulators, a block's four waves add theirs in LDS, k_narrow_join adds the blocks' in their order.  Nothing is rounded before the
+// results, whatever the type.  The cross entropy's backward pass makes z again rather than keeping anything of it.
+//
+// x comes by 16-byte copies straight to LDS, the next 32 rows' while these are worked on; chunks are permuted within their row so that the
+// lanes' reads fall on different banks.  Rows that are not whole aligned chunks (11 features) come through registers.
+#include "stage.hpp"
+
+namespace clid_dense {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+
+enum class Do { Linear, LinearBwd, Ce, CeBwd, Label };
+
+struct Narrow {
+  const void *x, *w, *bias;
+  int64_t ldx, ldw, rows;
+  int k, n, x_wide;
+  // Linear, LinearBwd
+  const void *res, *dy, *z_in;
+  void *y, *z_out;
+  int64_t ldr, lddy;
+  int act, n_vec, k_vec;  // rows of n (of k) values are whole runs of 4, aligned: y, z, dy, res (dx)
+  // LinearBwd, CeBwd
+  void* dx;
+  float* part;  // [blocks][n k + n]: sums for dw and db
+  int want_w, want_b;
+  // Ce, CeBwd
+  const int64_t* target;
+  int64_t ignore;
+  int reduction;
+  float *loss_none, *total;
+  const float* g;
+  double* sums;  // [blocks][2]: losses, how many
+  // Label
+  int64_t* label;
+  float* log_prob;
+};
+
+__device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
+
+template <typename T>
+__device__ __forceinline__ void get4(const T* p, float (&v)[4], int count, bool vec) {
+  if (vec && count >= 4) {
+    typedef __attribute__((ext_vector_type(4 * sizeof(T) / 4))) uint32_t V;
+    union { V w; T t[4]; } u;
+    u.w = *(const V*)p;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = up(u.t[q]);
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) v[q] = q < count ? up(p[q]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void put4(T* p, const T (&t)[4], int count, bool vec) {
+  if (vec && count >= 4) {
+    typedef __attribute__((ext_vector_type(4 * sizeof(T) / 4))) uint32_t V;
+    union { V w; T t[4]; } u;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) u.t[q] = t[q];
+    *(V*)p = u.w;
+  } else {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < count) p[q] = t[q];
+  }
+}
+
+// TN: 32 columns of z each; KQ: runs of 8 along k
+template <typename T, int TN, int KQ, Do DO>
+struct NarrowShape {
+  static constexpr bool kBwd = DO == Do::LinearBwd || DO == Do::CeBwd;
+  static constexpr int kChunkElems = 16 / sizeof(T);
+  static constexpr int kChunks = 8 * KQ / kChunkElems;             // of an x row in LDS: 2, 4, 8 or 16
+  static constexpr int kXBuf = 32 * kChunks * 16;                  // 32 rows
+  static constexpr int kXLoads = kXBuf / 1024;
+  static constexpr int kMostWaves = kBwd ? 4 : 8;
+  static constexpr int kWRow = 8 * KQ + 4;                         // floats
+  static constexpr int kWBytes = 32 * TN * kWRow * 4;
+  static constexpr int kZRow = 32 * TN + 4;
+  static constexpr int kZBytes = kBwd ? 32 * kZRow * 4 : 0;
+  static constexpr int kWave = 2 * kXBuf + kZBytes;
+  static constexpr int kTK = (8 * KQ + 31) / 32;
+  static constexpr int kHead = kWBytes + 32 * TN * 4;
+  static constexpr int kSumRow = 32 * kTK + 1, kSums = 32 * TN * kSumRow + 32 * TN;  // a wave's sums for dw and db, floats
+  static constexpr int lds(int waves) { return max_of(kHead + waves * kWave, kBwd ? waves * kSums * 4 : waves * 16); }
+  static constexpr int max_of(int a, int b) { return a > b ? a : b; }
+  // 16 chunks span the banks once: the rows between them are told apart by the chunk's place
+  static __device__ __forceinline__ int place(int row, int c) { return c ^ ((row / (16 / kChunks)) & (kChunks - 1)); }
+};
+
+template <typename T, int TN, int KQ, Do DO>
+__global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ? 4 : 8)) k_narrow(Narrow a) {
+  using S = NarrowShape<T, TN, KQ, DO>;
+  constexpr int TK = S::kTK;
+  extern __shared__ __align__(16) char lds[];
+  float* w = (float*)lds;
+  float* bias = (float*)(lds + S::kWBytes);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+  const int waves = blockDim.x >> 6;
+  char* xbuf = lds + S::kHead + wave * S::kWave;
+  float* zbuf = (float*)(xbuf + 2 * S::kXBuf);
+  const T* x = (const T*)a.x;
+
+  // copies' offsets, the same for every 32 rows
+  uint32_t at[S::kXLoads];
+#pragma unroll
+  for (int i = 0; i < S::kXLoads; ++i) {
+    const int c = i * 64 + lane, row = c / S::kChunks, chunk = S::place(row, c % S::kChunks);
+    at[i] = chunk * S::kChunkElems < a.k ? uint32_t(row) * uint32_t(a.ldx * sizeof(T)) + chunk * 16 : kOutside;
+  }
+  auto fetch = [&](int64_t m0, char* buf) {
+    const int64_t rows = a.rows - m0 < 32 ? a.rows - m0 : 32;
+    if (a.x_wide) {
+      const uint32_t bound = (uint32_t)(((rows - 1) * a.ldx + a.k) * (int64_t)sizeof(T));
+#pragma unroll
+      for (int i = 0; i < S::kXLoads; ++i) copy16(x + m0 * a.ldx, bound, at[i], buf + i * 1024);
+    } else {
+      constexpr int kEach = 8 * KQ / 2;  // two lanes a row
+      const T* from = x + (m0 + col) * a.ldx;
+      T v[kEach];
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) v[e] = col < rows && half * kEach + e < a.k ? from[half * kEach + e] : down<T>(0.f);
+#pragma unroll
+      for (int e = 0; e < kEach; ++e) {
+        const int k = half * kEach + e;
+        ((T*)(buf + (col * S::kChunks + S::place(col, k / S::kChunkElems)) * 16))[k % S::kChunkElems] = v[e];
+      }
+    }
+  };
+
+  const int64_t strips = (a.rows + 31) / 32, step = (int64_t)gridDim.x * waves;
+  int64_t strip = (int64_t)blockIdx.x * waves + wave;
+  if (a.x_wide && strip < strips) fetch(strip * 32, xbuf);
+  for (int e = threadIdx.x; e < 32 * TN * 8 * KQ; e += blockDim.x) {
+    const int n = e / (8 * KQ), k = e % (8 * KQ);
+    w[n * S::kWRow + k] = n < a.n && k < a.k ? up(((const T*)a.w)[n * a.ldw + k]) : 0.f;
+  }
+  for (int n = threadIdx.x; n < 32 * TN; n += blockDim.x) bias[n] = a.bias && n < a.n ? up(((const T*)a.bias)[n]) : 0.f;
+  __syncthreads();
+
+  f32x16 sum_w[S::kBwd ? TN : 1][S::kBwd ? TK : 1];
+  float sum_b[S::kBwd ? TN : 1][16];
+  if constexpr (S::kBwd) {
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        sum_b[i][r] = 0.f;
+#pragma unroll
+        for (int t = 0; t < TK; ++t) sum_w[i][t][r] = 0.f;
+      }
+  }
+  double loss_sum = 0.0;
+  int counted = 0;
+
+  for (int turn = 0; strip < strips; strip += step, turn ^= 1) {
+    char* xs = xbuf + turn * S::kXBuf;
+    const int64_t m0 = strip * 32, m = m0 + col;
+    const bool on = m < a.rows;
+    if (!a.x_wide) fetch(m0, xs);
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // these rows' copies; no read of them moves above it
+    if (a.x_wide && strip + step < strips) fetch((strip + step) * 32, xbuf + (turn ^ 1) * S::kXBuf);
+
+    auto x4 = [&](int q, float (&v)[4]) {  // x[m][8 q + 4 half ..]
+      const int k = 8 * q + 4 * half;
+      const T* p = (const T*)(xs + (col * S::kChunks + S::place(col, k / S::kChunkElems)) * 16) + k % S::kChunkElems;
+      get4(p, v, 4, true);
+    };
+    f32x16 z[TN];
+    if constexpr (DO != Do::LinearBwd) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 b4 = *(const float4*)(bias + 32 * i + 8 * j + 4 * half);
+          z[i][4 * j] = b4.x; z[i][4 * j + 1] = b4.y; z[i][4 * j + 2] = b4.z; z[i][4 * j + 3] = b4.w;
+        }
+#pragma unroll
+      for (int q = 0; q < KQ; ++q) {
+        float xv[4];
+        x4(q, xv);
+#pragma unroll
+        for (int i = 0; i < TN; ++i) {
+          const float4 w4 = *(const float4*)(w + (32 * i + col) * S::kWRow + 8 * q + 4 * half);
+          z[i] = mfma_f32(w4.x, xv[0], z[i]);
+          z[i] = mfma_f32(w4.y, xv[1], z[i]);
+          z[i] = mfma_f32(w4.z, xv[2], z[i]);
+          z[i] = mfma_f32(w4.w, xv[3], z[i]);
+        }
+      }
+    }
+
+    if constexpr (DO == Do::Linear) {
+      if (on)
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int n = 32 * i + 8 * j + 4 * half, count = a.n - n;
+            if (count <= 0) continue;
+            float r[4] = {0.f, 0.f, 0.f, 0.f};
+            if (a.res) get4((const T*)a.res + m * a.ldr + n, r, count, a.n_vec);
+            T t[4];
+            if (a.z_out) {
+#pragma unroll
+              for (int q = 0; q < 4; ++q) t[q] = keep_z<T>(z[i][4 * j + q]);
+              put4((T*)a.z_out + m * a.n + n, t, count, a.n_vec);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) t[q] = down<T>(act_value(z[i][4 * j + q], a.act) + r[q]);
+            put4((T*)a.y + m * a.n + n, t, count, a.n_vec);
+          }
+    }
+
+    // a row's statistics: the largest z, its column, sum over the others of exp(z - largest), the target's z
+    float top = neg_inf(), rest = 0.f, zt = 0.f;
+    int best = 0x7fffffff;
+    bool counts = false;
+    int64_t target = -1;
+    if constexpr (DO == Do::Ce || DO == Do::CeBwd) {
+      if (on) target = a.target[m];
+      counts = on && target != a.ignore;
+    }
+    if constexpr (DO == Do::Ce || DO == Do::CeBwd || DO == Do::Label) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int n = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+          if (n >= a.n) z[i][r] = neg_inf();
+          if (n == target) zt = z[i][r];
+          top = fmaxf(top, z[i][r]);
+        }
+      top = fmaxf(top, __shfl_xor(top, 32, 64));
+      const float safe = top == neg_inf() ? 0.f : top;
+      int same = 0;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool is = z[i][r] == top;
+          rest += is ? 0.f : __builtin_amdgcn_exp2f((z[i][r] - safe) * 1.4426950408889634f);
+          same += is;
+        }
+      rest += __shfl_xor(rest, 32, 64);
+      same += __shfl_xor(same, 32, 64);
+      zt += __shfl_xor(zt, 32, 64);  // the other half's is 0
+      rest = top == neg_inf() ? (rest == rest ? 0.f : rest) : rest + (float)(same - 1);
+      if (top == __builtin_inff()) rest = __builtin_nanf("");
+    }
+    float loss = 0.f;
+    if constexpr (DO == Do::Ce || DO == Do::CeBwd) {
+      loss = target >= 0 && target < a.n ? (top - zt) + log1pf(rest) : __builtin_nanf("");
+      if (!counts) loss = 0.f;
+    }
+    if constexpr (DO == Do::Ce) {
+      if (half == 0 && on) {
+        if (a.loss_none) a.loss_none[m] = loss;
+        loss_sum += loss;
+        counted += counts;
+      }
+    }
+    if constexpr (DO == Do::Label) {
+      bool nan = false;
+#pragma unroll
+      for (int i = TN - 1; i >= 0; --i)
+#pragma unroll
+        for (int r = 15; r >= 0; --r)
+          if (z[i][r] == top) best = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+      if (rest != rest) {
+        int first = 0x7fffffff;
+#pragma unroll
+        for (int i = TN - 1; i >= 0; --i)
+#pragma unroll
+          for (int r = 15; r >= 0; --r)
+            if (z[i][r] != z[i][r]) first = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+        const int other = __shfl_xor(first, 32, 64);
+        first = other < first ? other : first;
+        nan = first != 0x7fffffff;
+        if (nan) best = first;
+      }
+      const int other = __shfl_xor(best, 32, 64);
+      best = other < best ? other : best;
+      if (half == 0 && on) {
+        a.label[m] = best;
+        a.log_prob[m] = nan || top == neg_inf() ? __builtin_nanf("") : -log1pf(rest);
+      }
+    }
+
+    if constexpr (S::kBwd) {
+      // z becomes dz
+      if constexpr (DO == Do::LinearBwd) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int n = 32 * i + 8 * j + 4 * half, count = on ? a.n - n : 0;
+            float v[4] = {0.f, 0.f, 0.f, 0.f}, y[4];
+            if (count > 0) {
+              get4((const T*)a.dy + m * a.lddy + n, v, count, a.n_vec);
+              if (a.z_in) {
+                get4((const T*)a.z_in + m * a.n + n, y, count, a.n_vec);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) v[q] = q < count ? v[q] * act_slope(y[q], a.act) : 0.f;
+              }
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) z[i][4 * j + q] = v[q];
+          }
+      } else {
+        float f = 0.f;
+        if (counts) f = a.reduction == CLID_REDUCE_NONE ? a.g[m] : a.reduction == CLID_REDUCE_MEAN ? a.g[0] / fmaxf(a.total[1], 1.f) : a.g[0];
+        const float inv = loss != loss ? loss : f / (1.f + rest), hit = expm1f(-loss) * f;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int n = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+            const float p = __builtin_amdgcn_exp2f((z[i][r] - top) * 1.4426950408889634f) * inv;
+            z[i][r] = counts && n < a.n ? (n == target ? hit : p) : 0.f;
+          }
+      }
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sum_b[i][r] += z[i][r];
+      if (a.want_w) {
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *(float4*)(zbuf + col * S::kZRow + 32 * i + 8 * j + 4 * half) = float4{z[i][4 * j], z[i][4 * j + 1], z[i][4 * j + 2], z[i][4 * j + 3]};
+      }
+      __builtin_amdgcn_wave_barrier();
+      if (a.dx) {
+        f32x16 d[TK];
+#pragma unroll
+        for (int t = 0; t < TK; ++t)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) d[t][r] = 0.f;
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int n = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+#pragma unroll
+            for (int t = 0; t < TK; ++t) {
+              const int k = 32 * t + col;  // a row of w is 8 KQ values: where that is 16, lanes 16 .. 31 have none
+              d[t] = mfma_f32(8 * KQ >= 32 || k < 8 * KQ ? w[n * S::kWRow + k] : 0.f, z[i][r], d[t]);
+            }
+          }
+        if (on)
+#pragma unroll
+          for (int t = 0; t < TK; ++t)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int k = 32 * t + 8 * j + 4 * half, count = a.k - k;
+              if (count <= 0) continue;
+              const bool zero = DO == Do::CeBwd && !counts;
+              T v[4];
+#pragma unroll
+              for (int q = 0; q < 4; ++q) v[q] = down<T>(zero ? 0.f : d[t][4 * j + q]);
+              put4((T*)a.dx + m * a.k + k, v, count, a.k_vec);
+            }
+      }
+      if (a.want_w) {
+        // rows that do not count are zeros whatever they hold
+        const uint32_t live = DO == Do::CeBwd ? (uint32_t)__ballot(counts) : 0xffffffffu;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+          const int mm = 2 * s + half;
+          float xv[TK];
+#pragma unroll
+          for (int t = 0; t < TK; ++t) {
+            const int k = 32 * t + col;
+            xv[t] = 0.f;
+            if ((8 * KQ >= 32 || k < 8 * KQ) && (live >> mm & 1)) xv[t] = up(((const T*)(xs + (mm * S::kChunks + S::place(mm, k / S::kChunkElems)) * 16))[k % S::kChunkElems]);
+          }
+#pragma unroll
+          for (int i = 0; i < TN; ++i) {
+            const float zv = zbuf[mm * S::kZRow + 32 * i + col];
+#pragma unroll
+            for (int t = 0; t < TK; ++t) sum_w[i][t] = mfma_f32(zv, xv[t], sum_w[i][t]);
+          }
+        }
+      }
+      __builtin_amdgcn_wave_barrier();
+    }
+  }
+
+  if constexpr (DO == Do::Ce) {
+    for (int d = 16; d; d >>= 1) {
+      loss_sum += __shfl_xor(loss_sum, d, 64);
+      counted += __shfl_xor(counted, d, 64);
+    }
+    __syncthreads();
+    double* s = (double*)lds;
+    if (lane == 0) {
+      s[2 * wave] = loss_sum;
+      s[2 * wave + 1] = counted;
+    }
+    __syncthreads();
+    if (threadIdx.x < 2) {
+      double t = 0.0;
+      for (int i = 0; i < waves; ++i) t += s[2 * i + threadIdx.x];
+      a.sums[blockIdx.x * 2 + threadIdx.x] = t;
+    }
+  }
+  if constexpr (S::kBwd) {
+    // the waves' sums: [wave][n][k] and [wave][n], then one partial result a block
+    __syncthreads();
+    constexpr int kRow = S::kSumRow, kMine = S::kSums;
+    float* mine = (float*)lds + wave * kMine;
+#pragma unroll
+    for (int i = 0; i < TN; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int n = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
+        float b = sum_b[i][r];
+        for (int d = 16; d; d >>= 1) b += __shfl_xor(b, d, 64);  // over the 32 rows
+        if (col == 0) mine[32 * TN * kRow + n] = b;
+#pragma unroll
+        for (int t = 0; t < TK; ++t) mine[n * kRow + 32 * t + col] = sum_w[i][t][r];
+      }
+    __syncthreads();
+    const float* all = (const float*)lds;
+    const int nk = a.n * a.k;
+    float* out = a.part + (int64_t)blockIdx.x * (nk + a.n);
+    for (int e = threadIdx.x; e < nk + a.n; e += blockDim.x) {
+      const int from = e < nk ? e / a.k * kRow + e % a.k : 32 * TN * kRow + (e - nk);
+      float t = 0.f;
+      for (int i = 0; i < waves; ++i) t += all[i * kMine + from];
+      out[e] = t;
+    }
+  }
+}
+
+// the blocks' sums -> dw, db: 64 of them a block, 16 threads each
+template <typename T>
+__global__ void __launch_bounds__(1024) k_narrow_join(const float* part, int blocks, int nk, int n, T* dw, T* db) {
+  __shared__ float p[16][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6, all = nk + n;
+  float s = 0.f;
+  if (c < all)
+#pragma unroll 8
+    for (int b = g; b < blocks; b += 16) s += part[(int64_t)b * all + c];
+  p[g][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (g || c >= all) return;
+  for (int i = 1; i < 16; ++i) s += p[i][threadIdx.x];
+  if (c < nk) {
+    if (dw) dw[c] = down<T>(s);
+  } else if (db) {
+    db[c - nk] = down<T>(s);
+  }
+}
+__global__ void __launch_bounds__(256) k_narrow_total(const double* sums, int blocks, int reduction, float* total, float* loss_out) {
+  __shared__ double p[4][2];
+  double s = 0.0, c = 0.0;
+  for (int b = threadIdx.x; b < blocks; b += 256) {
+    s += sums[2 * b];
+    c += sums[2 * b + 1];
+  }
+  for (int d = 32; d; d >>= 1) {
+    s += __shfl_xor(s, d, 64);
+    c += __shfl_xor(c, d, 64);
+  }
+  if ((threadIdx.x & 63) == 0) {
+    p[threadIdx.x >> 6][0] = s;
+    p[threadIdx.x >> 6][1] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  s = p[0][0] + p[1][0] + p[2][0] + p[3][0];
+  c = p[0][1] + p[1][1] + p[2][1] + p[3][1];
+  total[0] = (float)s;
+  total[1] = (float)c;
+  if (reduction == CLID_REDUCE_MEAN) loss_out[0] = c > 0.0 ? (float)(s / c) : 0.f;
+  if (reduction == CLID_REDUCE_SUM) loss_out[0] = (float)s;
+}
+
+// 32 rows a wave and turn: waves fill the CUs before blocks grow, and a block keeps its copy of w for all its turns
+struct NarrowGrid {
+  int waves, blocks;
+};
+static NarrowGrid narrow_grid(int64_t rows, bool bwd) {
+  const int64_t strips = (rows + 31) / 32;
+  int waves = 1;
+  while (waves < (bwd ? 4 : 8) && strips > (int64_t)kCus * waves) waves *= 2;
+  const int64_t b = (strips + waves - 1) / waves, most = bwd ? kCus : 2 * kCus;
+  return {waves, (int)(b < most ? b : most)};
+}
+
+template <typename T, int TN, int KQ, Do DO>
+int narrow_launch(const Narrow& a, const NarrowGrid& g, hipStream_t s) {
+  using S = NarrowShape<T, TN, KQ, DO>;
+  static_assert(S::lds(S::kMostWaves) <= 160 * 1024, "a block fits a CU");
+  auto k = k_narrow<T, TN, KQ, DO>;
+  const int lds = S::lds(g.waves), rc = allow_lds((const void*)k, S::lds(S::kMostWaves));
+  if (rc != CLID_OK) return rc;
+  hipLaunchKernelGGL(k, dim3(g.blocks), dim3(64 * g.waves), lds, s, a);
+  return CLID_OK;
+}
+template <typename T, Do DO>
+int narrow_by_shape(const Narrow& a, const NarrowGrid& g, hipStream_t s) {
+  if (a.n <= 32) {
+    if (a.k <= 16) return narrow_launch<T, 1, 2, DO>(a, g, s);
+    if (a.k <= 32) return narrow_launch<T, 1, 4, DO>(a, g, s);
+    return narrow_launch<T, 1, 8, DO>(a, g, s);
+  }
+  if (a.k <= 16) return narrow_launch<T, 2, 2, DO>(a, g, s);
+  if (a.k <= 32) return narrow_launch<T, 2, 4, DO>(a, g, s);
+  return narrow_launch<T, 2, 8, DO>(a, g, s);
+}
+
+template <typename T>
+static Narrow narrow_args(const void* x, int64_t ldx, const void* w, int64_t ldw, const void* bias, int64_t rows, int k, int n) {
+  Narrow a = {};
+  a.x = x; a.w = w; a.bias = bias;
+  a.ldx = ldx; a.ldw = ldw; a.rows = rows;
+  a.k = k; a.n = n;
+  a.x_wide = wide8<T>(x, ldx) && k % (16 / (int)sizeof(T)) == 0 && ldx < (int64_t(1) << 24);
+  return a;
+}
+// whether rows of `values` starting at p are whole aligned runs of 4
+template <typename T>
+static bool runs4(const void* p, int64_t ld, int values) { return !p || ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0 && values % 4 == 0); }
+
+int narrow_linear(const clid_linear_args* c, hipStream_t s) {
+  BY_DTYPE(c->dtype, {
+    Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
+    a.res = c->residual; a.ldr = c->ldr; a.y = c->y; a.z_out = c->z_out; a.act = c->act;
+    a.n_vec = runs4<T>(c->y, c->n, c->n) && runs4<T>(c->z_out, c->n, c->n) && runs4<T>(c->residual, c->ldr, c->n);
+    return narrow_by_shape<T, Do::Linear>(a, narrow_grid(c->rows, false), s);
+  });
+}
+int64_t narrow_linear_bwd_bytes(const clid_linear_bwd_args* c) { return up256((int64_t)narrow_grid(c->rows, true).blocks * (c->n * c->k + c->n) * 4); }
+int narrow_linear_bwd(const clid_linear_bwd_args* c, hipStream_t s) {
+  const NarrowGrid grid = narrow_grid(c->rows, true);
+  const int blocks = grid.blocks, all = c->n * c->k + c->n;
+  BY_DTYPE(c->dtype, {
+    Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, nullptr, c->rows, c->k, c->n);
+    a.dy = c->dy; a.lddy = c->lddy; a.z_in = c->act == CLID_ACT_NONE ? nullptr : c->z; a.act = c->act; a.dx = c->dx;
+    a.n_vec = runs4<T>(c->dy, c->lddy, c->n) && runs4<T>(a.z_in, c->n, c->n);
+    a.k_vec = runs4<T>(c->dx, c->k, c->k);
+    a.part = (float*)c->ws; a.want_w = c->dw != nullptr; a.want_b = c->db != nullptr;
+    const int rc = narrow_by_shape<T, Do::LinearBwd>(a, grid, s);
+    if (rc != CLID_OK) return rc;
+    if (c->dw || c->db) hipLaunchKernelGGL(k_narrow_join<T>, dim3((all + 63) / 64), dim3(1024), 0, s, a.part, blocks, c->n * c->k, c->n, (T*)c->dw, (T*)c->db);
+    return CLID_OK;
+  });
+}
+int64_t narrow_ce_bytes(const clid_ce_args* c) { return up256((int64_t)narrow_grid(c->rows, false).blocks * 16); }
+int narrow_ce(const clid_ce_args* c, hipStream_t s) {
+  const NarrowGrid grid = narrow_grid(c->rows, false);
+  const int blocks = grid.blocks;
+  BY_DTYPE(c->dtype, {
+    Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
+    a.target = c->target; a.ignore = c->ignore_index; a.reduction = c->reduction;
+    a.loss_none = c->reduction == CLID_REDUCE_NONE ? c->loss_out : nullptr;
+    a.sums = (double*)c->ws;
+    const int rc = narrow_by_shape<T, Do::Ce>(a, grid, s);
+    if (rc != CLID_OK) return rc;
+    hipLaunchKernelGGL(k_narrow_total, dim3(1), dim3(256), 0, s, a.sums, blocks, c->reduction, c->total, c->loss_out);
+    return CLID_OK;
+  });
+}
+int64_t narrow_ce_bwd_bytes(const clid_ce_args* c) { return up256((int64_t)narrow_grid(c->rows, true).blocks * (c->n * c->k + c->n) * 4); }
+int narrow_ce_bwd(const clid_ce_args* c, hipStream_t s) {
+  const NarrowGrid grid = narrow_grid(c->rows, true);
+  const int blocks = grid.blocks, all = c->n * c->k + c->n;
+  BY_DTYPE(c->dtype, {
+    Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
+    a.target = c->target; a.ignore = c->ignore_index; a.reduction = c->reduction; a.g = c->g; a.total = c->total;
+    a.dx = c->dx; a.k_vec = runs4<T>(c->dx, c->k, c->k);
+    a.part = (float*)c->ws; a.want_w = c->dw != nullptr; a.want_b = c->db != nullptr;
+    const int rc = narrow_by_shape<T, Do::CeBwd>(a, grid, s);
+    if (rc != CLID_OK) return rc;
+    if (c->dw || c->db) hipLaunchKernelGGL(k_narrow_join<T>, dim3((all + 63) / 64), dim3(1024), 0, s, a.part, blocks, c->n * c->k, c->n, (T*)c->dw, (T*)c->db);
+    return CLID_OK;
+  });
+}
+int narrow_label(const clid_label_args* c, hipStream_t s) {
+  BY_DTYPE(c->dtype, {
+    Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
+    a.label = c->label; a.log_prob = c->log_prob;
+    return narrow_by_shape<T, Do::Label>(a, narrow_grid(c->rows, false), s);
+  });
+}
+
+}  // namespace clid_dense

@@ -160,6 +160,36 @@ inline int row_blocks(int64_t rows, int n) {
   return (int)(most < want ? most : want);
 }
 
+// more than 64 KB of LDS is asked for, once a kernel and device (the flag costs nothing to set again: no lock)
+inline int allow_lds(const void* kernel, int bytes) {
+  if (bytes <= 65536) return CLID_OK;
+  constexpr int kSlots = 1024;
+  static std::atomic<uintptr_t> seen[kSlots];
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess) dev = 0;
+  const uintptr_t key = (uintptr_t)kernel * 64 + (uintptr_t)(dev & 63) + 1;
+  std::atomic<uintptr_t>& slot = seen[(key >> 6 ^ key >> 16 ^ key) % kSlots];
+  if (slot.load() == key) return CLID_OK;
+  const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != hipSuccess) {
+    clid_set_error("dense kernel: %d bytes of LDS refused: %s", bytes, hipGetErrorString(e));
+    return CLID_E_HIP;
+  }
+  slot.store(key);
+  return CLID_OK;
+}
+
+// n, k <= 64 (narrow.hip)
+inline bool is_narrow(int32_t k, int32_t n) { return k <= 64 && n <= 64; }
+int narrow_linear(const clid_linear_args* a, hipStream_t s);
+int64_t narrow_linear_bwd_bytes(const clid_linear_bwd_args* a);
+int narrow_linear_bwd(const clid_linear_bwd_args* a, hipStream_t s);
+int64_t narrow_ce_bytes(const clid_ce_args* a);
+int narrow_ce(const clid_ce_args* a, hipStream_t s);
+int64_t narrow_ce_bwd_bytes(const clid_ce_args* a);
+int narrow_ce_bwd(const clid_ce_args* a, hipStream_t s);
+int narrow_label(const clid_label_args* a, hipStream_t s);
+
 // ---- tiles --------------------------------------------------------------------------------------------------------------
 template <int NP, int SIZE> struct Tile;
 template <> struct Tile<1, 2> { static constexpr int BM = 256, BN = 256, BK = 64, WM = 2, WN = 4; };
@@ -219,18 +249,8 @@ inline int launch_one(Product g, const Epi& epi, hipStream_t s) {
   }
   constexpr int kLds = 2 * NP * (C::BM + C::BN) * C::BK * 2 + C::BN * 4;
   auto k = k_tile<Kind<T>::F16, NP, C::BM, C::BN, C::BK, C::WM, C::WN, PKS, QKS, Epi>;
-  if (kLds > 65536) {  // asked for once a device
-    static std::atomic<uint64_t> asked{0};
-    int dev = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev > 63 || !(asked.load() >> dev & 1)) {
-      const hipError_t e = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
-      if (e != hipSuccess) {
-        clid_set_error("dense product: %d bytes of LDS refused: %s", kLds, hipGetErrorString(e));
-        return CLID_E_HIP;
-      }
-      if (dev < 64) asked.fetch_or(uint64_t(1) << dev);
-    }
-  }
+  const int rc = allow_lds((const void*)k, kLds);
+  if (rc != CLID_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * C::WM * C::WN), kLds, s, g, epi);
   return CLID_OK;
 }

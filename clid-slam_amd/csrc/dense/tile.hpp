@@ -54,6 +54,12 @@ __device__ __forceinline__ f32x16 mfma(s16x8 a, s16x8 b, f32x16 c) {
 
 constexpr uint32_t kOutside = 0x80000000u;  // an offset that every bounds check here refuses: the load returns zeros
 
+// 16 bytes a lane from base + offset (zeros where they end behind `bound`) to lds + 16 lane
+__device__ __forceinline__ void copy16(const void* base, uint32_t bound, uint32_t offset, char* lds) {
+  auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bound, 0x00027000);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
+}
+
 // v as three bf16 planes.  Each is the one before's remainder cut to 8 bits, so they have v's sign and their sum is v.  A plane that
 // comes out as 0 is 2^-126 with v's sign instead, and an infinity's planes are all infinite: then an infinity in the other operand
 // meets no zero that is not a zero of the matrix, and all six products have the sign of the one that they stand for.
@@ -117,7 +123,6 @@ struct Side {
       if constexpr (KS) bytes = ((k - k0 - 1) * o.ld + (rows - first)) * 2;
       else bytes = ((rows - first - 1) * o.ld + ((k - k0 + 7) & ~int64_t(7))) * 2;  // rows are whole chunks
       const uint32_t bound = bytes > 0x7fffffff ? 0x7fffffffu : (uint32_t)bytes;
-      auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)base, 0, bound, 0x00027000);
 #pragma unroll
       for (int i = 0; i < kLoads; ++i) {
         uint32_t off = at[i];
@@ -127,8 +132,7 @@ struct Side {
             if (k0 + chunk * 8 >= k) off = kOutside;
           }
         }
-        char* dst = lds + s * kBytes + (i * WAVES + wave) * 1024;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)dst, 16, off, 0, 0, 0);
+        copy16(base, bound, off, lds + s * kBytes + (i * WAVES + wave) * 1024);
       }
     }
   }

@@ -66,6 +66,7 @@ int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream);
  * row's loss NaN.
  *   order     [rows + 1] int32: the rows that count, in their order, and in the last place how many there are
  *   stat      [rows][4] fp32, by place in `order`: largest z, 1 / sum exp(z - largest), p_target - 1, loss of the row
+ *             (both left as they were where n, k <= 64: the backward pass makes z and its statistics again)
  *   total     [2] fp32: sum of the losses; number of rows that count
  *   loss_out  [1] (CLID_REDUCE_MEAN: the sum over the counted rows / their number, 0 if there are none; CLID_REDUCE_SUM) or
  *             [rows] (CLID_REDUCE_NONE) fp32
