@@ -193,6 +193,23 @@ bool ce_ok(const clid_ce_args* a) {
   return a && sizes_ok(a->rows, a->k, a->n) && dtype_ok(a->dtype) && a->reduction >= 0 && a->reduction <= CLID_REDUCE_SUM;
 }
 
+// clid_ce_args.saved: the sum of the losses and how many rows count (fp32); the rows that count in their order, and in the place after the
+// last how many there are; by place in that order: largest z, 1 / sum exp(z - largest), p_target - 1, loss
+struct Saved {
+  float* total;
+  int32_t* order;
+  float4* stat;
+  int64_t bytes;
+  explicit Saved(const clid_ce_args* a) {
+    Ws ws(a->saved);
+    total = (float*)ws.take(8);
+    const bool lists = !is_narrow(a->k, a->n);
+    order = (int32_t*)ws.take(lists ? (a->rows + 1) * 4 : 0);
+    stat = (float4*)ws.take(lists ? a->rows * 16 : 0);
+    bytes = ws.used;
+  }
+};
+
 template <typename T>
 struct CeFwd {
   Plan p;
@@ -217,19 +234,20 @@ struct CeFwd {
 template <typename T>
 int ce_fwd(const clid_ce_args* a, hipStream_t s) {
   const CeFwd<T> f(a);
+  const Saved v(a);
   float* none = a->reduction == CLID_REDUCE_NONE ? a->loss_out : nullptr;
   if (a->rows) {
     const int blocks = (int)((a->rows + kRowsPer - 1) / kRowsPer);
     if (blocks > 1) hipLaunchKernelGGL(k_count, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (int*)f.counts);
-    hipLaunchKernelGGL(k_order, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (const int*)f.counts, a->order, none);
-    const int32_t* live = a->order + a->rows;
-    Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, a->order, live), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), live, 0, 1, 0, 0};
-    const int rc = launch_stat<T, false>(g, f.p.size, (const T*)a->bias, a->target, a->order, (float2*)f.part, nullptr, (float*)f.zt, s);
+    hipLaunchKernelGGL(k_order, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (const int*)f.counts, v.order, none);
+    const int32_t* live = v.order + a->rows;
+    Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, v.order, live), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), live, 0, 1, 0, 0};
+    const int rc = launch_stat<T, false>(g, f.p.size, (const T*)a->bias, a->target, v.order, (float2*)f.part, nullptr, (float*)f.zt, s);
     if (rc != CLID_OK) return rc;
-    hipLaunchKernelGGL(k_loss_rows, dim3(f.joins), dim3(1024), 0, s, (const float2*)f.part, f.strips, (const float*)f.zt, a->target, a->order, a->rows, a->n,
-                       (float4*)a->stat, none, (double*)f.sums);
+    hipLaunchKernelGGL(k_loss_rows, dim3(f.joins), dim3(1024), 0, s, (const float2*)f.part, f.strips, (const float*)f.zt, a->target, v.order, a->rows, a->n,
+                       v.stat, none, (double*)f.sums);
   }
-  hipLaunchKernelGGL(k_loss_total, dim3(1), dim3(1024), 0, s, (const double*)f.sums, f.joins, a->rows ? a->order + a->rows : nullptr, a->reduction, a->total, a->loss_out);
+  hipLaunchKernelGGL(k_loss_total, dim3(1), dim3(1024), 0, s, (const double*)f.sums, f.joins, a->rows ? v.order + a->rows : nullptr, a->reduction, v.total, a->loss_out);
   return CLID_OK;
 }
 
@@ -273,12 +291,13 @@ template <typename T>
 int ce_bwd(const clid_ce_args* a, hipStream_t s) {
   constexpr int NP = Kind<T>::NP;
   const CeBwd<T> f(a);
-  const int32_t* live = a->order + a->rows;
+  const Saved v(a);
+  const int32_t* live = v.order + a->rows;
   float* scale = (float*)f.scale;
-  hipLaunchKernelGGL(k_scale, dim3(1), dim3(1024), 0, s, a->g, a->total, a->rows, a->reduction, (int)Kind<T>::F16, scale);
+  hipLaunchKernelGGL(k_scale, dim3(1), dim3(1024), 0, s, a->g, v.total, a->rows, a->reduction, (int)Kind<T>::F16, scale);
   if (a->dx)
     hipLaunchKernelGGL(k_clear_rows<T>, dim3((unsigned)(a->rows < 2048 ? a->rows : 2048)), dim3(256), 0, s, a->target, a->rows, a->ignore_index, a->k, (T*)a->dx);
-  const Operand x = stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, a->order, live);
+  const Operand x = stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, v.order, live);
   const Operand w = stage<T>(a->w, a->ldw, a->n, a->k, f.w, s);
   for (int64_t v0 = 0; v0 < a->n; v0 += f.piece) {
     const int64_t nv = a->n - v0 < f.piece ? a->n - v0 : f.piece, ld = up8(nv);
@@ -286,7 +305,7 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
     wv.p += v0 * w.ld;
     const Operand dz = {(const uint16_t*)f.dz, ld, a->rows * ld};
     Product gz = {x, wv, a->rows, nv, up8(a->k), live, 0, 1, 0, 0};
-    int rc = launch_dz<T>(gz, f.pz.size, {a->bias ? (const T*)a->bias + v0 : nullptr, a->target, a->order, (const float4*)a->stat, scale,
+    int rc = launch_dz<T>(gz, f.pz.size, {a->bias ? (const T*)a->bias + v0 : nullptr, a->target, v.order, v.stat, scale,
                                           a->reduction == CLID_REDUCE_NONE ? a->g : nullptr, (uint16_t*)f.dz, v0, nv, ld, a->rows * ld}, s);
     if (rc != CLID_OK) return rc;
     if (a->dx) {
@@ -295,7 +314,7 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
       const float* before = v0 ? (const float*)f.sum : nullptr;
       const int sum_wide = wide8<float>(f.sum, a->k);
       if (last)
-        rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, before, scale + 1, a->order, a->k, wide8<T>(a->dx, a->k), sum_wide}, f.part, s);
+        rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, before, scale + 1, v.order, a->k, wide8<T>(a->dx, a->k), sum_wide}, f.part, s);
       else
         rc = launch_out<T, false, true>(g, f.px, StoreOut<float>{nullptr, (float*)f.sum, before, nullptr, nullptr, a->k, sum_wide, sum_wide}, f.part, s);
       if (rc != CLID_OK) return rc;
@@ -345,6 +364,10 @@ int label(const clid_label_args* a, hipStream_t s) {
 
 }  // namespace
 
+extern "C" int64_t clid_ce_saved(const clid_ce_args* a) {
+  if (!ce_ok(a)) return bad("clid_ce_saved", "bad argument");
+  return Saved(a).bytes;
+}
 extern "C" int64_t clid_ce_workspace(const clid_ce_args* a) {
   if (!ce_ok(a)) return bad("clid_ce_workspace", "bad argument");
   if (is_narrow(a->k, a->n) && a->rows) return narrow_ce_bytes(a);
@@ -353,7 +376,7 @@ extern "C" int64_t clid_ce_workspace(const clid_ce_args* a) {
 extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
   const char* me = "clid_ce_fwd";
   if (!ce_ok(a)) return bad(me, "bad argument");
-  if (!a->total || (a->rows && (!a->x || !a->w || !a->target || !a->stat || !a->order || a->ldx < a->k || a->ldw < a->k)) ||
+  if (!a->saved || (a->rows && (!a->x || !a->w || !a->target || a->ldx < a->k || a->ldw < a->k)) ||
       (!a->loss_out && !(a->reduction == CLID_REDUCE_NONE && a->rows == 0)))
     return bad(me, "bad pointer or row stride");
   const int64_t need = clid_ce_workspace(a);
@@ -374,7 +397,7 @@ extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
   const char* me = "clid_ce_bwd";
   if (!ce_ok(a)) return bad(me, "bad argument");
   if (a->rows == 0) return bad(me, "no rows");
-  if (!a->x || !a->w || !a->target || !a->stat || !a->total || !a->order || !a->g || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
+  if (!a->x || !a->w || !a->target || !a->saved || !a->g || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
   const int64_t need = clid_ce_bwd_workspace(a);
   if (!a->ws || a->ws_bytes < need) return bad(me, "workspace too small");
   int rc = CLID_OK;

@@ -570,7 +570,7 @@ int narrow_ce(const clid_ce_args* c, hipStream_t s) {
     a.sums = (double*)c->ws;
     const int rc = narrow_by_shape<T, Do::Ce>(a, grid, s);
     if (rc != CLID_OK) return rc;
-    hipLaunchKernelGGL(k_narrow_total, dim3(1), dim3(256), 0, s, a.sums, blocks, c->reduction, c->total, c->loss_out);
+    hipLaunchKernelGGL(k_narrow_total, dim3(1), dim3(256), 0, s, a.sums, blocks, c->reduction, (float*)c->saved, c->loss_out);
     return CLID_OK;
   });
 }
@@ -580,7 +580,7 @@ int narrow_ce_bwd(const clid_ce_args* c, hipStream_t s) {
   const int blocks = grid.blocks, all = c->n * c->k + c->n;
   BY_DTYPE(c->dtype, {
     Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
-    a.target = c->target; a.ignore = c->ignore_index; a.reduction = c->reduction; a.g = c->g; a.total = c->total;
+    a.target = c->target; a.ignore = c->ignore_index; a.reduction = c->reduction; a.g = c->g; a.total = (float*)c->saved;
     a.dx = c->dx; a.k_vec = runs4<T>(c->dx, c->k, c->k);
     a.part = (float*)c->ws; a.want_w = c->dw != nullptr; a.want_b = c->db != nullptr;
     const int rc = narrow_by_shape<T, Do::CeBwd>(a, grid, s);

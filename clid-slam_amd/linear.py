@@ -31,7 +31,7 @@ class LinearBwdArgs(C.Structure):
 
 
 class CeArgs(C.Structure):
-    _fields_ = [("x", _vp), ("w", _vp), ("bias", _vp), ("target", _vp), ("order", _vp), ("stat", _vp), ("total", _vp), ("loss_out", _vp),
+    _fields_ = [("x", _vp), ("w", _vp), ("bias", _vp), ("target", _vp), ("saved", _vp), ("loss_out", _vp),
                 ("g", _vp), ("dx", _vp), ("dw", _vp), ("db", _vp),
                 ("ldx", _i64), ("ldw", _i64), ("rows", _i64), ("ignore_index", _i64),
                 ("k", _i32), ("n", _i32), ("dtype", _i32), ("reduction", _i32), ("ws", _vp), ("ws_bytes", _i64)]
@@ -48,6 +48,7 @@ _SIGS = {
     "clid_linear_fwd": (C.c_int, [C.POINTER(LinearArgs), _vp]),
     "clid_linear_bwd_workspace": (_i64, [C.POINTER(LinearBwdArgs)]),
     "clid_linear_bwd": (C.c_int, [C.POINTER(LinearBwdArgs), _vp]),
+    "clid_ce_saved": (_i64, [C.POINTER(CeArgs)]),
     "clid_ce_workspace": (_i64, [C.POINTER(CeArgs)]),
     "clid_ce_fwd": (C.c_int, [C.POINTER(CeArgs), _vp]),
     "clid_ce_bwd_workspace": (_i64, [C.POINTER(CeArgs)]),
@@ -71,31 +72,36 @@ def load():
     return _bound
 
 
+# (The small shapes are over in 10 us on the GPU, so what Python does around a call is kept to what is needed: no tensor is made only to read its
+# pointer, and one buffer holds what a call leaves for its backward pass.)
 def call(entry: str, workspace: str, args, device) -> None:
     """One entry point on torch's current stream of `device`, with its workspace from torch's allocator: a buffer of this call
     alone, which the allocator gives back in stream order (and keeps for a graph that is being captured)."""
     if device.index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return call(entry, workspace, args, device)
-    lib = load()
-    need = getattr(lib, workspace)(C.byref(args))
-    if need < 0:
-        _lib.check(int(need), workspace)
-    ws = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-    args.ws, args.ws_bytes = _lib.ptr(ws), need
-    _lib.check(getattr(lib, entry)(C.byref(args), _lib.stream()), entry)
+    lib, ref = _bound or load(), C.byref(args)
+    need = getattr(lib, workspace)(ref)
+    if need:
+        if need < 0:
+            _lib.check(int(need), workspace)
+        ws = torch.empty(need, dtype=torch.uint8, device=device)
+        args.ws, args.ws_bytes = ws.data_ptr(), need
+    rc = getattr(lib, entry)(ref, _lib.stream())
+    if rc:
+        _lib.check(rc, entry)
 
 
-def rows_of(t: torch.Tensor, width: int) -> torch.Tensor:
-    """`t` as [rows, width] with contiguous columns: a view wherever its strides allow, else a copy."""
-    t = t.detach().reshape(-1, width)
-    if t.shape[0] > 1 and t.stride(0) < width or width > 1 and t.stride(1) != 1:
+def rows_of(t: torch.Tensor, width: int):
+    """(`t` as rows of `width` contiguous columns, elements between rows): t itself or a view wherever its strides allow, else a
+    copy.  Called without gradients (inside autograd functions, under no_grad)."""
+    if t.dim() != 2:
+        t = t.reshape(-1, width)
+    rows, (ld, step) = t.shape[0], t.stride()
+    if width > 1 and step != 1 or rows > 1 and ld < width:
         t = t.contiguous()
-    return t
-
-
-def ld_of(t: torch.Tensor) -> int:
-    return max(t.stride(0), t.shape[1]) if t.shape[0] > 1 else t.shape[1]
+        ld = width
+    return t, (ld if rows > 1 else width)
 
 
 def check_operands(what: str, x, weight, bias=None, residual=None) -> None:
@@ -105,18 +111,23 @@ def check_operands(what: str, x, weight, bias=None, residual=None) -> None:
             raise RuntimeError(f"{what}: {name} must be a tensor")
     if not x.is_cuda:
         raise RuntimeError(f"{what}: x must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
-    if x.dtype not in DTYPES:
-        raise RuntimeError(f"{what}: x must be float32, bfloat16 or float16, got {x.dtype}")
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise RuntimeError(f"{what}: x {tuple(x.shape)} and weight {tuple(weight.shape)} must be [..., k] and [n, k] with n, k >= 1")
-    n = weight.shape[0]
-    for name, t, shape in (("weight", weight, weight.shape), ("bias", bias, (n,)), ("residual", residual, (*x.shape[:-1], n))):
-        if t is None:
-            continue
-        if t.shape != shape:
-            raise RuntimeError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-        if t.dtype != x.dtype or t.device != x.device:
-            raise RuntimeError(f"{what}: {name} must be {x.dtype} on {x.device} like x, got {t.dtype} on {t.device}")
+    dtype, shape, wshape = x.dtype, x.shape, weight.shape
+    if dtype not in DTYPES:
+        raise RuntimeError(f"{what}: x must be float32, bfloat16 or float16, got {dtype}")
+    if len(wshape) != 2 or len(shape) < 1 or shape[-1] != wshape[1] or 0 in wshape:
+        raise RuntimeError(f"{what}: x {tuple(shape)} and weight {tuple(wshape)} must be [..., k] and [n, k] with n, k >= 1")
+    _like(what, "weight", weight, wshape, dtype, x.device)
+    if bias is not None:
+        _like(what, "bias", bias, wshape[:1], dtype, x.device)
+    if residual is not None:
+        _like(what, "residual", residual, (*shape[:-1], wshape[0]), dtype, x.device)
+
+
+def _like(what, name, t, shape, dtype, device):
+    if t.shape != shape:
+        raise RuntimeError(f"{what}: {name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.dtype != dtype or t.device != device:
+        raise RuntimeError(f"{what}: {name} must be {dtype} on {device} like x, got {t.dtype} on {t.device}")
 
 
 def wants_grad(*tensors) -> bool:
@@ -125,15 +136,16 @@ def wants_grad(*tensors) -> bool:
 
 def _forward(x, weight, bias, act, residual, keep_z):
     n, k = weight.shape
-    x2, w = rows_of(x, k), rows_of(weight, k)
-    b = None if bias is None else bias.detach().contiguous()
-    r = None if residual is None else rows_of(residual, n)
+    (x2, ldx), (w, ldw) = rows_of(x, k), rows_of(weight, k)
+    r, ldr = (None, n) if residual is None else rows_of(residual, n)
+    b = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    z = torch.empty((x2.shape[0], n), dtype=x.dtype, device=x.device) if keep_z else None
-    if x2.shape[0]:
-        args = LinearArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(r), _lib.ptr(y), _lib.ptr(z), ld_of(x2), ld_of(w),
-                          ld_of(r) if r is not None else n, x2.shape[0], k, n, DTYPES[x.dtype], act)
-        call("clid_linear_fwd", "clid_linear_workspace", args, x.device)
+    z = torch.empty_like(y) if keep_z else None
+    rows = x2.shape[0]
+    if rows:
+        call("clid_linear_fwd", "clid_linear_workspace",
+             LinearArgs(x2.data_ptr(), w.data_ptr(), _lib.ptr(b), _lib.ptr(r), y.data_ptr(), _lib.ptr(z), ldx, ldw, ldr, rows, k, n,
+                        DTYPES[x.dtype], act), x.device)
     return y, z
 
 
@@ -153,19 +165,21 @@ class _LinearAct(torch.autograd.Function):
     def backward(ctx, dy):
         x, weight, z = ctx.saved_tensors
         n, k = weight.shape
-        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_w else None
-        db = torch.empty(n, dtype=x.dtype, device=x.device) if need_b else None
-        x2, w, dy2 = rows_of(x, k), rows_of(weight, k), rows_of(dy, n)
-        if x2.shape[0] == 0:
+        need_x, need_w, need_b, need_r, _ = ctx.needs_input_grad
+        dtype, device = x.dtype, x.device
+        dx = torch.empty(x.shape, dtype=dtype, device=device) if need_x else None
+        dw = torch.empty((n, k), dtype=dtype, device=device) if need_w else None
+        db = torch.empty(n, dtype=dtype, device=device) if need_b else None
+        (x2, ldx), (w, ldw), (dy2, lddy) = rows_of(x, k), rows_of(weight, k), rows_of(dy, n)
+        rows = x2.shape[0]
+        if rows == 0:
             for t in (dw, db):
                 if t is not None:
                     t.zero_()
         elif need_x or need_w or need_b:
-            args = LinearBwdArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(dy2), _lib.ptr(z), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db),
-                                 ld_of(x2), ld_of(w), ld_of(dy2), x2.shape[0], k, n, DTYPES[x.dtype], ctx.act)
-            call("clid_linear_bwd", "clid_linear_bwd_workspace", args, x.device)
+            call("clid_linear_bwd", "clid_linear_bwd_workspace",
+                 LinearBwdArgs(x2.data_ptr(), w.data_ptr(), dy2.data_ptr(), _lib.ptr(z), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), ldx, ldw,
+                               lddy, rows, k, n, DTYPES[dtype], ctx.act), device)
         return dx, dw, db, (dy if need_r else None), None
 
 
@@ -176,12 +190,14 @@ def linear_act(x, weight, bias=None, activation: str = "none", residual=None):
     float16) on one GPU; rows may be a view of a wider buffer.  `activation`: none, relu, leaky_relu (slope 0.01), gelu (erf),
     silu.  Sums are fp32; y is rounded once, after the residual.  Runs on torch's current stream, captures into a graph,
     differentiates once."""
-    if activation not in ACTIVATIONS:
+    act = ACTIVATIONS.get(activation)
+    if act is None:
         raise NotImplementedError(f"linear_act: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     check_operands("linear_act", x, weight, bias, residual)
     if wants_grad(x, weight, bias, residual):
-        return _LinearAct.apply(x, weight, bias, residual, ACTIVATIONS[activation])
-    return _forward(x, weight, bias, ACTIVATIONS[activation], residual, False)[0]
+        return _LinearAct.apply(x, weight, bias, residual, act)
+    with torch.no_grad():
+        return _forward(x, weight, bias, act, residual, False)[0]
 
 
 @torch.no_grad()
@@ -191,12 +207,13 @@ def linear_label(x, weight, bias=None):
     differentiable (the class head's training loss is `loss.linear_cross_entropy`)."""
     check_operands("linear_label", x, weight, bias)
     n, k = weight.shape
-    x2, w = rows_of(x, k), rows_of(weight, k)
-    b = None if bias is None else bias.detach().contiguous()
+    (x2, ldx), (w, ldw) = rows_of(x, k), rows_of(weight, k)
+    b = None if bias is None else bias.contiguous()
     label = torch.empty(x.shape[:-1], dtype=torch.int64, device=x.device)
     log_prob = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    if x2.shape[0]:
-        args = LabelArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(label), _lib.ptr(log_prob), ld_of(x2), ld_of(w),
-                         x2.shape[0], k, n, DTYPES[x.dtype], 0)
-        call("clid_label_fwd", "clid_label_workspace", args, x.device)
+    rows = x2.shape[0]
+    if rows:
+        call("clid_label_fwd", "clid_label_workspace",
+             LabelArgs(x2.data_ptr(), w.data_ptr(), _lib.ptr(b), label.data_ptr(), log_prob.data_ptr(), ldx, ldw, rows, k, n, DTYPES[x.dtype], 0),
+             x.device)
     return label, log_prob

@@ -43,44 +43,44 @@ class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, target, ignore_index, reduction):
         n, k = weight.shape
-        x2, w = linear.rows_of(x, k), linear.rows_of(weight, k)
-        b = None if bias is None else bias.detach().contiguous()
-        t = target.detach().reshape(-1).to(torch.int64).contiguous()
+        (x2, ldx), (w, ldw) = linear.rows_of(x, k), linear.rows_of(weight, k)
+        b = None if bias is None else bias.contiguous()
+        t = target.to(torch.int64).contiguous()
         rows, dev = x2.shape[0], x.device
-        order = torch.empty(rows + 1, dtype=torch.int32, device=dev)
-        stat = torch.empty((rows, 4), dtype=torch.float32, device=dev)
-        total = torch.empty(2, dtype=torch.float32, device=dev)
         loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
-        if rows or reduction != 0:
-            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(order), _lib.ptr(stat), _lib.ptr(total), _lib.ptr(loss),
-                                 None, None, None, None, linear.ld_of(x2), linear.ld_of(w), rows, ignore_index, k, n,
-                                 linear.DTYPES[x.dtype], reduction)
+        args = linear.CeArgs(x2.data_ptr(), w.data_ptr(), _lib.ptr(b), t.data_ptr(), None, loss.data_ptr(), None, None, None, None, ldx, ldw,
+                             rows, ignore_index, k, n, linear.DTYPES[x.dtype], reduction)
+        saved = torch.empty(linear.load().clid_ce_saved(args), dtype=torch.uint8, device=dev)
+        args.saved = saved.data_ptr()
+        if rows or reduction:
             linear.call("clid_ce_fwd", "clid_ce_workspace", args, dev)
-        ctx.ignore_index, ctx.reduction, ctx.has_bias = ignore_index, reduction, bias is not None
-        ctx.save_for_backward(x, weight, t, order, stat, total, *(() if bias is None else (bias,)))
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        ctx.save_for_backward(x, weight, t, saved, bias)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, weight, t, order, stat, total, *rest = ctx.saved_tensors
+        x, weight, t, saved, bias = ctx.saved_tensors
         n, k = weight.shape
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = torch.empty((n, k), dtype=x.dtype, device=x.device) if need_w else None
-        db = torch.empty(n, dtype=x.dtype, device=x.device) if need_b else None
-        x2, w = linear.rows_of(x, k), linear.rows_of(weight, k)
-        if x2.shape[0] == 0:
+        dtype, dev = x.dtype, x.device
+        dx = torch.empty(x.shape, dtype=dtype, device=dev) if need_x else None
+        dw = torch.empty((n, k), dtype=dtype, device=dev) if need_w else None
+        db = torch.empty(n, dtype=dtype, device=dev) if need_b else None
+        (x2, ldx), (w, ldw) = linear.rows_of(x, k), linear.rows_of(weight, k)
+        rows = x2.shape[0]
+        if rows == 0:
             for v in (dw, db):
                 if v is not None:
                     v.zero_()
         else:
-            b = rest[0].detach().contiguous() if rest else None
-            g = g.detach().reshape(-1).to(torch.float32).contiguous()
-            args = linear.CeArgs(_lib.ptr(x2), _lib.ptr(w), _lib.ptr(b), _lib.ptr(t), _lib.ptr(order), _lib.ptr(stat), _lib.ptr(total), None, _lib.ptr(g),
-                                 _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), linear.ld_of(x2), linear.ld_of(w), x2.shape[0], ctx.ignore_index,
-                                 k, n, linear.DTYPES[x.dtype], ctx.reduction)
-            linear.call("clid_ce_bwd", "clid_ce_bwd_workspace", args, x.device)
+            b = None if bias is None else bias.contiguous()
+            g = g.to(torch.float32).contiguous()
+            linear.call("clid_ce_bwd", "clid_ce_bwd_workspace",
+                        linear.CeArgs(x2.data_ptr(), w.data_ptr(), _lib.ptr(b), t.data_ptr(), saved.data_ptr(), None, g.data_ptr(), _lib.ptr(dx),
+                                      _lib.ptr(dw), _lib.ptr(db), ldx, ldw, rows, ctx.ignore_index, k, n, linear.DTYPES[dtype],
+                                      ctx.reduction), dev)
         return dx, dw, db, None, None, None
 
 

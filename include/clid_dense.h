@@ -64,21 +64,19 @@ int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream);
 /* Softmax cross entropy of z = x w^T + bias against target, never storing z.  A row whose target is ignore_index has loss 0, no
  * gradient, and what its x holds (NaN, infinities) reaches nothing.  A target outside [0, n) that is not ignore_index makes its
  * row's loss NaN.
- *   order     [rows + 1] int32: the rows that count, in their order, and in the last place how many there are
- *   stat      [rows][4] fp32, by place in `order`: largest z, 1 / sum exp(z - largest), p_target - 1, loss of the row
- *             (both left as they were where n, k <= 64: the backward pass makes z and its statistics again)
- *   total     [2] fp32: sum of the losses; number of rows that count
+ *   saved     clid_ce_saved() bytes, 256-byte aligned: what the backward pass needs of the forward one (which rows count, their
+ *             statistics; never z)
  *   loss_out  [1] (CLID_REDUCE_MEAN: the sum over the counted rows / their number, 0 if there are none; CLID_REDUCE_SUM) or
  *             [rows] (CLID_REDUCE_NONE) fp32
- * Backward: g is dL/dloss_out (fp32, one value or [rows]); order, stat, total as the forward call left them. */
+ * Backward: g is dL/dloss_out (fp32, one value or [rows]); saved as the forward call left it. */
 #define CLID_REDUCE_NONE 0
 #define CLID_REDUCE_MEAN 1
 #define CLID_REDUCE_SUM 2
 typedef struct clid_ce_args {
   const void *x, *w, *bias; /* [rows][k], [n][k], [n] or NULL */
   const int64_t* target;    /* [rows] */
-  int32_t* order;
-  float *stat, *total, *loss_out;
+  void* saved;
+  float* loss_out;
   const float* g;     /* backward only */
   void *dx, *dw, *db; /* backward only, dense, NULL where not wanted */
   int64_t ldx, ldw;
@@ -87,6 +85,7 @@ typedef struct clid_ce_args {
   void* ws;
   int64_t ws_bytes;
 } clid_ce_args;
+int64_t clid_ce_saved(const clid_ce_args* a);
 int64_t clid_ce_workspace(const clid_ce_args* a);
 int clid_ce_fwd(const clid_ce_args* a, void* stream);
 int64_t clid_ce_bwd_workspace(const clid_ce_args* a);
