@@ -411,6 +411,7 @@ extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
 extern "C" int64_t clid_label_workspace(const clid_label_args* a) {
   if (!label_ok(a)) return bad("clid_label_workspace", "bad argument");
   if (is_narrow(a->k, a->n)) return 0;
+  if (is_few(a->rows)) return few_label_bytes(a);
   BY_DTYPE(a->dtype, return Label<T>(a).bytes;);
 }
 extern "C" int clid_label_fwd(const clid_label_args* a, void* stream) {
@@ -422,6 +423,7 @@ extern "C" int clid_label_fwd(const clid_label_args* a, void* stream) {
   if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_label(a, (hipStream_t)stream);
+  else if (is_few(a->rows)) rc = few_label(a, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = label<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);

@@ -43,6 +43,11 @@ struct LinearOut {
   T *y, *z;
   int64_t ldr, n;
   int act, wide, res_wide;
+  __device__ __forceinline__ void one(float v, int64_t m, int64_t c) const {
+    v += bias ? up(bias[c]) : 0.f;
+    if (z) z[m * n + c] = keep_z<T>(v);
+    y[m * n + c] = down<T>(act_value(v, act) + (res ? up(res[m * ldr + c]) : 0.f));
+  }
   // v: sums at row m, columns c ..; b: their bias
   __device__ __forceinline__ void eight(float (&v)[8], const float (&b)[8], int64_t m, int64_t c, int) const {
     const int count = (int)(n - c < 8 ? n - c : 8);

@@ -90,7 +90,7 @@ bool args_ok(const clid_linear_bwd_args* a) {
 
 extern "C" int64_t clid_linear_workspace(const clid_linear_args* a) {
   if (!args_ok(a)) return bad("clid_linear_workspace", "bad argument");
-  if (is_narrow(a->k, a->n)) return 0;
+  if (is_narrow(a->k, a->n) || is_few(a->rows)) return 0;
   BY_DTYPE(a->dtype, return Fwd<T>(a).bytes;);
 }
 extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
@@ -102,6 +102,7 @@ extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
   if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_linear(a, (hipStream_t)stream);
+  else if (is_few(a->rows)) rc = few_linear(a, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = fwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);

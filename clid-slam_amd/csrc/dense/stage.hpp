@@ -190,6 +190,12 @@ int64_t narrow_ce_bwd_bytes(const clid_ce_args* a);
 int narrow_ce_bwd(const clid_ce_args* a, hipStream_t s);
 int narrow_label(const clid_label_args* a, hipStream_t s);
 
+// at most 32 rows (few.hip)
+inline bool is_few(int64_t rows) { return rows <= 32; }
+int few_linear(const clid_linear_args* a, hipStream_t s);
+int64_t few_label_bytes(const clid_label_args* a);
+int few_label(const clid_label_args* a, hipStream_t s);
+
 // ---- tiles --------------------------------------------------------------------------------------------------------------
 template <int NP, int SIZE> struct Tile;
 template <> struct Tile<1, 2> { static constexpr int BM = 256, BN = 256, BK = 64, WM = 2, WN = 4; };
