@@ -312,17 +312,16 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
       const bool last = v0 + nv == a->n;
       Product g = {dz, wv, a->rows, a->k, nv, live, 0, 1, 0, 0};
       const float* before = v0 ? (const float*)f.sum : nullptr;
-      const int sum_wide = wide8<float>(f.sum, a->k);
       if (last)
-        rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, before, scale + 1, v.order, a->k, wide8<T>(a->dx, a->k), sum_wide}, f.part, s);
+        rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, before, scale + 1, v.order, a->k}, f.part, s);
       else
-        rc = launch_out<T, false, true>(g, f.px, StoreOut<float>{nullptr, (float*)f.sum, before, nullptr, nullptr, a->k, sum_wide, sum_wide}, f.part, s);
+        rc = launch_out<T, false, true>(g, f.px, StoreOut<float>{nullptr, (float*)f.sum, before, nullptr, nullptr, a->k}, f.part, s);
       if (rc != CLID_OK) return rc;
     }
     if (a->dw) {
       T* to = (T*)a->dw + v0 * a->k;
       Product g = {dz, x, nv, a->k, a->rows, live, 1, 1, 0, 0};
-      rc = launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, to, nullptr, scale + 1, nullptr, a->k, wide8<T>(to, a->k), 0}, f.part, s);
+      rc = launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, to, nullptr, scale + 1, nullptr, a->k}, f.part, s);
       if (rc != CLID_OK) return rc;
     }
     if (a->db) {

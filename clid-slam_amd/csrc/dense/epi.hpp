@@ -5,36 +5,29 @@
 
 namespace clid_dense {
 
-// 8 neighbouring values of a row, wide where the row allows it (rows whose starts and lengths are multiples of 16 bytes)
+// 8 neighbouring values of a row, by 16 bytes (which need not be aligned) where there are 8
 template <typename T>
-__device__ __forceinline__ void get8(const T* p, float (&v)[8], int count, bool wide) {
-  if (wide && count >= 8) {
-    union { uint4 w[sizeof(T) / 2]; T t[8]; } u;
+__device__ __forceinline__ void get8(const T* p, float (&v)[8], int count) {
+  T t[8];
+  if (count >= 8) {
+    __builtin_memcpy(t, p, sizeof(t));
 #pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.w[i] = ((const uint4*)p)[i];
-#pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = up(u.t[q]);
+    for (int q = 0; q < 8; ++q) v[q] = up(t[q]);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = q < count ? up(p[q]) : 0.f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void out8(T* p, const T (&t)[8], int count, bool wide) {
-  if (wide && count >= 8) {
-    union { uint4 w[sizeof(T) / 2]; T t[8]; } u;
-#pragma unroll
-    for (int q = 0; q < 8; ++q) u.t[q] = t[q];
-#pragma unroll
-    for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((uint4*)p)[i] = u.w[i];
+__device__ __forceinline__ void out8(T* p, const T (&t)[8], int count) {
+  if (count >= 8) {
+    __builtin_memcpy(p, t, sizeof(t));
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
       if (q < count) p[q] = t[q];
   }
 }
-template <typename T>
-inline bool wide8(const void* p, int64_t ld) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && ld % (16 / (int64_t)sizeof(T)) == 0; }
 
 // z + bias -> act -> + residual -> y, and z for the backward pass
 template <typename T>
@@ -42,7 +35,7 @@ struct LinearOut {
   const T *bias, *res;
   T *y, *z;
   int64_t ldr, n;
-  int act, wide, res_wide;
+  int act;
   __device__ __forceinline__ void one(float v, int64_t m, int64_t c) const {
     v += bias ? up(bias[c]) : 0.f;
     if (z) z[m * n + c] = keep_z<T>(v);
@@ -53,18 +46,18 @@ struct LinearOut {
     const int count = (int)(n - c < 8 ? n - c : 8);
     if (count <= 0) return;
     float r[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (res) get8(res + m * ldr + c, r, count, res_wide);
+    if (res) get8(res + m * ldr + c, r, count);
     T t[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] += b[q];
     if (z) {
 #pragma unroll
       for (int q = 0; q < 8; ++q) t[q] = keep_z<T>(v[q]);
-      out8(z + m * n + c, t, count, wide);
+      out8(z + m * n + c, t, count);
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) t[q] = down<T>(act_value(v[q], act) + r[q]);
-    out8(y + m * n + c, t, count, wide);
+    out8(y + m * n + c, t, count);
   }
 };
 
@@ -76,13 +69,12 @@ struct StoreOut {
   const float *add, *alpha;  // add: [m][n] fp32 of the pieces before
   const int32_t* order;
   int64_t n;
-  int wide, add_wide;
   __device__ __forceinline__ void eight(float (&v)[8], const float (&)[8], int64_t m, int64_t c, int) const {
     const int count = (int)(n - c < 8 ? n - c : 8);
     if (count <= 0) return;
     if (add) {
       float a[8];
-      get8(add + m * n + c, a, count, add_wide);
+      get8(add + m * n + c, a, count);
 #pragma unroll
       for (int q = 0; q < 8; ++q) v[q] += a[q];
     }
@@ -90,7 +82,7 @@ struct StoreOut {
     T t[8];
 #pragma unroll
     for (int q = 0; q < 8; ++q) t[q] = down<T>(v[q] * s);
-    out8(out + (order ? (int64_t)order[m] : m) * n + c, t, count, wide);
+    out8(out + (order ? (int64_t)order[m] : m) * n + c, t, count);
   }
 };
 
@@ -100,7 +92,7 @@ struct PartOut {
   float* part;
   int64_t m_all, n8;
   __device__ __forceinline__ void eight(float (&v)[8], const float (&)[8], int64_t m, int64_t c, int split) const {
-    if (c < n8) out8(part + ((int64_t)split * m_all + m) * n8 + c, v, 8, true);
+    if (c < n8) out8(part + ((int64_t)split * m_all + m) * n8 + c, v, 8);
   }
 };
 

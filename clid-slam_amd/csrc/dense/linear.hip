@@ -25,8 +25,7 @@ template <typename T>
 int fwd(const clid_linear_args* a, hipStream_t s) {
   const Fwd<T> f(a);
   Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
-  LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (T*)a->z_out, a->ldr, a->n, a->act,
-                    wide8<T>(a->y, a->n) && wide8<T>(a->z_out, a->n), wide8<T>(a->residual, a->ldr)};
+  LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (T*)a->z_out, a->ldr, a->n, a->act};
   return launch_out<T, false, false>(g, f.p, o, f.part, s);
 }
 
@@ -62,19 +61,19 @@ int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
   if (f.own_dz) dz = {(const uint16_t*)f.dz, np, a->rows * np};
   if (f.own_dz || a->db) {
     hipLaunchKernelGGL(k_dz<T>, dim3((np + 255) / 256, f.blocks), dim3(256), 0, s, (const T*)a->dy, a->lddy, z, a->rows, a->n, a->act,
-                       (int)wide8<T>(a->dy, a->lddy), (int)wide8<T>(a->z, a->n), f.own_dz ? (uint16_t*)f.dz : nullptr, np, a->rows * np,
+                       f.own_dz ? (uint16_t*)f.dz : nullptr, np, a->rows * np,
                        a->db ? (float*)f.sums : nullptr);
     if (a->db)
       hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
   }
   if (a->dx) {
     Product g = {dz, stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->k, a->n, nullptr, 0, 1, 0, 0};
-    const int rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, nullptr, nullptr, nullptr, a->k, wide8<T>(a->dx, a->k), 0}, f.part, s);
+    const int rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, nullptr, nullptr, nullptr, a->k}, f.part, s);
     if (rc != CLID_OK) return rc;
   }
   if (a->dw) {
     Product g = {dz, stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), a->n, a->k, a->rows, nullptr, 0, 1, 0, 0};
-    return launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, (T*)a->dw, nullptr, nullptr, nullptr, a->k, wide8<T>(a->dw, a->k), 0}, f.part, s);
+    return launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, (T*)a->dw, nullptr, nullptr, nullptr, a->k}, f.part, s);
   }
   return CLID_OK;
 }

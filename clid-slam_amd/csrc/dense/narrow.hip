@@ -27,7 +27,7 @@ struct Narrow {
   const void *res, *dy, *z_in;
   void *y, *z_out;
   int64_t ldr, lddy;
-  int act, n_vec, k_vec;  // rows of n (of k) values are whole runs of 4, aligned: y, z, dy, res (dx)
+  int act;
   // LinearBwd, CeBwd
   void* dx;
   float* part;  // [blocks][n k + n]: sums for dw and db
@@ -46,27 +46,23 @@ struct Narrow {
 
 __device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 
+// 4 neighbouring values of a row, in one load or store (which need not be aligned) where there are 4
 template <typename T>
-__device__ __forceinline__ void get4(const T* p, float (&v)[4], int count, bool vec) {
-  if (vec && count >= 4) {
-    typedef __attribute__((ext_vector_type(4 * sizeof(T) / 4))) uint32_t V;
-    union { V w; T t[4]; } u;
-    u.w = *(const V*)p;
+__device__ __forceinline__ void get4(const T* p, float (&v)[4], int count) {
+  T t[4];
+  if (count >= 4) {
+    __builtin_memcpy(t, p, sizeof(t));
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = up(u.t[q]);
+    for (int q = 0; q < 4; ++q) v[q] = up(t[q]);
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q) v[q] = q < count ? up(p[q]) : 0.f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void put4(T* p, const T (&t)[4], int count, bool vec) {
-  if (vec && count >= 4) {
-    typedef __attribute__((ext_vector_type(4 * sizeof(T) / 4))) uint32_t V;
-    union { V w; T t[4]; } u;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) u.t[q] = t[q];
-    *(V*)p = u.w;
+__device__ __forceinline__ void put4(T* p, const T (&t)[4], int count) {
+  if (count >= 4) {
+    __builtin_memcpy(p, t, sizeof(t));
   } else {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
@@ -173,7 +169,7 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     auto x4 = [&](int q, float (&v)[4]) {  // x[m][8 q + 4 half ..]
       const int k = 8 * q + 4 * half;
       const T* p = (const T*)(xs + (col * S::kChunks + S::place(col, k / S::kChunkElems)) * 16) + k % S::kChunkElems;
-      get4(p, v, 4, true);
+      get4((const T*)__builtin_assume_aligned(p, 4 * sizeof(T)), v, 4);
     };
     f32x16 z[TN];
     if constexpr (DO != Do::LinearBwd) {
@@ -208,16 +204,16 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
             const int n = 32 * i + 8 * j + 4 * half, count = a.n - n;
             if (count <= 0) continue;
             float r[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.res) get4((const T*)a.res + m * a.ldr + n, r, count, a.n_vec);
+            if (a.res) get4((const T*)a.res + m * a.ldr + n, r, count);
             T t[4];
             if (a.z_out) {
 #pragma unroll
               for (int q = 0; q < 4; ++q) t[q] = keep_z<T>(z[i][4 * j + q]);
-              put4((T*)a.z_out + m * a.n + n, t, count, a.n_vec);
+              put4((T*)a.z_out + m * a.n + n, t, count);
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) t[q] = down<T>(act_value(z[i][4 * j + q], a.act) + r[q]);
-            put4((T*)a.y + m * a.n + n, t, count, a.n_vec);
+            put4((T*)a.y + m * a.n + n, t, count);
           }
     }
 
@@ -306,9 +302,9 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
             const int n = 32 * i + 8 * j + 4 * half, count = on ? a.n - n : 0;
             float v[4] = {0.f, 0.f, 0.f, 0.f}, y[4];
             if (count > 0) {
-              get4((const T*)a.dy + m * a.lddy + n, v, count, a.n_vec);
+              get4((const T*)a.dy + m * a.lddy + n, v, count);
               if (a.z_in) {
-                get4((const T*)a.z_in + m * a.n + n, y, count, a.n_vec);
+                get4((const T*)a.z_in + m * a.n + n, y, count);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) v[q] = q < count ? v[q] * act_slope(y[q], a.act) : 0.f;
               }
@@ -369,7 +365,7 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
               T v[4];
 #pragma unroll
               for (int q = 0; q < 4; ++q) v[q] = down<T>(zero ? 0.f : d[t][4 * j + q]);
-              put4((T*)a.dx + m * a.k + k, v, count, a.k_vec);
+              put4((T*)a.dx + m * a.k + k, v, count);
             }
       }
       if (a.want_w) {
@@ -528,18 +524,13 @@ static Narrow narrow_args(const void* x, int64_t ldx, const void* w, int64_t ldw
   a.x = x; a.w = w; a.bias = bias;
   a.ldx = ldx; a.ldw = ldw; a.rows = rows;
   a.k = k; a.n = n;
-  a.x_wide = wide8<T>(x, ldx) && k % (16 / (int)sizeof(T)) == 0 && ldx < (int64_t(1) << 24);
+  a.x_wide = (uintptr_t)x % 16 == 0 && ldx % (16 / (int)sizeof(T)) == 0 && k % (16 / (int)sizeof(T)) == 0 && ldx < (int64_t(1) << 24);
   return a;
 }
-// whether rows of `values` starting at p are whole aligned runs of 4
-template <typename T>
-static bool runs4(const void* p, int64_t ld, int values) { return !p || ((uintptr_t)p % (4 * sizeof(T)) == 0 && ld % 4 == 0 && values % 4 == 0); }
-
 int narrow_linear(const clid_linear_args* c, hipStream_t s) {
   BY_DTYPE(c->dtype, {
     Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
     a.res = c->residual; a.ldr = c->ldr; a.y = c->y; a.z_out = c->z_out; a.act = c->act;
-    a.n_vec = runs4<T>(c->y, c->n, c->n) && runs4<T>(c->z_out, c->n, c->n) && runs4<T>(c->residual, c->ldr, c->n);
     return narrow_by_shape<T, Do::Linear>(a, narrow_grid(c->rows, false), s);
   });
 }
@@ -550,8 +541,6 @@ int narrow_linear_bwd(const clid_linear_bwd_args* c, hipStream_t s) {
   BY_DTYPE(c->dtype, {
     Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, nullptr, c->rows, c->k, c->n);
     a.dy = c->dy; a.lddy = c->lddy; a.z_in = c->act == CLID_ACT_NONE ? nullptr : c->z; a.act = c->act; a.dx = c->dx;
-    a.n_vec = runs4<T>(c->dy, c->lddy, c->n) && runs4<T>(a.z_in, c->n, c->n);
-    a.k_vec = runs4<T>(c->dx, c->k, c->k);
     a.part = (float*)c->ws; a.want_w = c->dw != nullptr; a.want_b = c->db != nullptr;
     const int rc = narrow_by_shape<T, Do::LinearBwd>(a, grid, s);
     if (rc != CLID_OK) return rc;
@@ -581,7 +570,7 @@ int narrow_ce_bwd(const clid_ce_args* c, hipStream_t s) {
   BY_DTYPE(c->dtype, {
     Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, c->bias, c->rows, c->k, c->n);
     a.target = c->target; a.ignore = c->ignore_index; a.reduction = c->reduction; a.g = c->g; a.total = (float*)c->saved;
-    a.dx = c->dx; a.k_vec = runs4<T>(c->dx, c->k, c->k);
+    a.dx = c->dx;
     a.part = (float*)c->ws; a.want_w = c->dw != nullptr; a.want_b = c->db != nullptr;
     const int rc = narrow_by_shape<T, Do::CeBwd>(a, grid, s);
     if (rc != CLID_OK) return rc;

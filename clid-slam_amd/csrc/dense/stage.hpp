@@ -38,7 +38,7 @@ __device__ __forceinline__ void put8(uint16_t* to, int64_t plane, const float (&
 }
 // rows of src (in `order`, as many as are live) -> planes with rows of kp values, zeros behind k
 template <typename T>
-__global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t rows, int k, const int32_t* order, const int32_t* live, int wide,
+__global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t rows, int k, const int32_t* order, const int32_t* live,
                                                uint16_t* dst, int kp, int64_t plane) {
   if (live) rows = *live < rows ? *live : rows;
   const int per = kp / 8;
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
     float v[8];
-    get8(src + (order ? (int64_t)order[r] : r) * ld + c, v, k - c < 8 ? k - c : 8, wide);
+    get8(src + (order ? (int64_t)order[r] : r) * ld + c, v, k - c < 8 ? k - c : 8);
     put8<T>(dst + r * kp + c, plane, v);
   }
 }
@@ -70,15 +70,14 @@ inline Operand stage(const void* p, int64_t ld, int64_t rows, int k, char* ws, h
                      const int32_t* live = nullptr) {
   if (direct<T>(p, ld, k) && !always) return {(const uint16_t*)p, ld, 0};
   const int64_t kp = up8(k);
-  hipLaunchKernelGGL(k_stage<T>, grid_for(rows * kp / 8), dim3(256), 0, s, (const T*)p, ld, rows, k, order, live, (int)wide8<T>(p, ld), (uint16_t*)ws,
-                     (int)kp, rows * kp);
+  hipLaunchKernelGGL(k_stage<T>, grid_for(rows * kp / 8), dim3(256), 0, s, (const T*)p, ld, rows, k, order, live, (uint16_t*)ws, (int)kp, rows * kp);
   return {(const uint16_t*)ws, kp, rows * kp};
 }
 
 // dz = dy act'(z) -> planes with rows of np values (dst may be NULL: the sums alone), and its column sums over blocks of rows ->
 // part[row block][n].  A block takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows.
 template <typename T>
-__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* z, int64_t rows, int n, int act, int wide, int z_wide, uint16_t* dst, int np,
+__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* z, int64_t rows, int n, int act, uint16_t* dst, int np,
                                             int64_t plane, float* part) {
   __shared__ float sums[8][256 + 8];
   const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8, count = n - c < 8 ? n - c : 8;
@@ -86,10 +85,10 @@ __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* 
   if (c < np)
     for (int64_t m = (int64_t)blockIdx.y * 8 + rr; m < rows; m += (int64_t)gridDim.y * 8) {
       float v[8];
-      get8(dy + m * lddy + c, v, count, wide);
+      get8(dy + m * lddy + c, v, count);
       if (z) {
         float y[8];
-        get8(z + m * n + c, y, count, z_wide);
+        get8(z + m * n + c, y, count);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = q < count ? v[q] * act_slope(y[q], act) : 0.f;
       }
@@ -198,12 +197,12 @@ int few_label(const clid_label_args* a, hipStream_t s);
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------
 template <int NP, int SIZE> struct Tile;
-template <> struct Tile<1, 2> { static constexpr int BM = 256, BN = 256, BK = 64, WM = 2, WN = 4; };
-template <> struct Tile<1, 1> { static constexpr int BM = 128, BN = 128, BK = 64, WM = 2, WN = 2; };
-template <> struct Tile<1, 0> { static constexpr int BM = 64, BN = 64, BK = 64, WM = 2, WN = 2; };
-template <> struct Tile<3, 2> { static constexpr int BM = 256, BN = 128, BK = 32, WM = 4, WN = 2; };
-template <> struct Tile<3, 1> { static constexpr int BM = 128, BN = 64, BK = 32, WM = 2, WN = 2; };
-template <> struct Tile<3, 0> { static constexpr int BM = 64, BN = 64, BK = 32, WM = 2, WN = 2; };
+template <> struct Tile<1, 2> { static constexpr int BM = 256, BN = 256, BK = 64, WM = 2, WN = 4, STAGES = 2; };
+template <> struct Tile<1, 1> { static constexpr int BM = 128, BN = 128, BK = 64, WM = 2, WN = 2, STAGES = 4; };
+template <> struct Tile<1, 0> { static constexpr int BM = 64, BN = 64, BK = 64, WM = 2, WN = 2, STAGES = 4; };
+template <> struct Tile<3, 2> { static constexpr int BM = 256, BN = 128, BK = 32, WM = 4, WN = 2, STAGES = 2; };
+template <> struct Tile<3, 1> { static constexpr int BM = 128, BN = 64, BK = 32, WM = 2, WN = 2, STAGES = 3; };
+template <> struct Tile<3, 0> { static constexpr int BM = 64, BN = 64, BK = 32, WM = 2, WN = 2, STAGES = 3; };
 template <int NP>
 inline void tile_shape(int size, int* bm, int* bn, int* bk) {
   *bm = size == 2 ? Tile<NP, 2>::BM : size == 1 ? Tile<NP, 1>::BM : Tile<NP, 0>::BM;
@@ -253,8 +252,8 @@ inline int launch_one(Product g, const Epi& epi, hipStream_t s) {
     clid_set_error("dense product: %lld x %lld results are more than one launch takes", (long long)g.m, (long long)g.n);
     return CLID_E_SHAPE;
   }
-  constexpr int kLds = 2 * NP * (C::BM + C::BN) * C::BK * 2 + C::BN * 4;
-  auto k = k_tile<Kind<T>::F16, NP, C::BM, C::BN, C::BK, C::WM, C::WN, PKS, QKS, Epi>;
+  constexpr int kLds = C::STAGES * NP * (C::BM + C::BN) * C::BK * 2 + C::BN * 4;
+  auto k = k_tile<Kind<T>::F16, NP, C::BM, C::BN, C::BK, C::WM, C::WN, C::STAGES, PKS, QKS, Epi>;
   const int rc = allow_lds((const void*)k, kLds);
   if (rc != CLID_OK) return rc;
   hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * C::WM * C::WN), kLds, s, g, epi);

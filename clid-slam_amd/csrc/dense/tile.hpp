@@ -94,8 +94,8 @@ struct Side {
       if constexpr (kChunks == 16) return c ^ ((row & 3) << 2);
       return c ^ (((row >> 1) & 1) << 2);
     } else {
-      if constexpr (kChunks == 8) return c ^ (row & 7);
-      return c ^ ((row >> 2) & 3);
+      // 16 lanes read together, one chunk of 16 rows: 256 bytes, every bank once
+      return c ^ ((row / (16 / kChunks)) & (kChunks - 1));
     }
   }
 
@@ -169,7 +169,7 @@ __device__ __forceinline__ void place_tile(const Product& g, int64_t block, int6
   *tm = (int)(in / cols);
 }
 
-template <bool F16, int NP, int BM, int BN, int BK, int WM, int WN, bool PKS, bool QKS, class Epi>
+template <bool F16, int NP, int BM, int BN, int BK, int WM, int WN, int STAGES, bool PKS, bool QKS, class Epi>
 __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   using SideP = Side<BM, BK, NP, PKS, WAVES>;
@@ -207,45 +207,61 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
 
-  auto load = [&](int64_t step, char* buf) {
+  constexpr int kLoads = NP * (SideP::kLoads + SideQ::kLoads);  // of a lane and step
+  auto load = [&](int64_t step) {
+    char* buf = lds + step % STAGES * kStage;
     sp.load(g.p, m0, lim_m, from + step * BK, to, buf, wave, lane);
     sq.load(g.q, n0, lim_n, from + step * BK, to, buf + NP * SideP::kBytes, wave, lane);
   };
-  auto multiply = [&](const char* buf) {
+  struct Frags {
+    s16x8 p[NP][TM], q[NP][TN];
+  };
+  auto read = [&](const char* buf, int kk, Frags& f) {
 #pragma unroll
-    for (int kk = 0; kk < BK / 16; ++kk) {
-      s16x8 p[NP][TM], q[NP][TN];
+    for (int s = 0; s < NP; ++s) {
 #pragma unroll
-      for (int s = 0; s < NP; ++s) {
+      for (int j = 0; j < TM; ++j) f.p[s][j] = SideP::fragment(buf, s, (wm * TM + j) * 32, kk, lane);
 #pragma unroll
-        for (int j = 0; j < TM; ++j) p[s][j] = SideP::fragment(buf, s, (wm * TM + j) * 32, kk, lane);
-#pragma unroll
-        for (int i = 0; i < TN; ++i) q[s][i] = SideQ::fragment(buf + NP * SideP::kBytes, s, (wn * TN + i) * 32, kk, lane);
-      }
-      constexpr int kPairs = NP == 3 ? 6 : 1;
-      constexpr int kP[6] = {0, 2, 1, 0, 1, 0}, kQ[6] = {2, 0, 1, 1, 0, 0};  // the small products first
-#pragma unroll
-      for (int t = 0; t < kPairs; ++t)
-#pragma unroll
-        for (int j = 0; j < TM; ++j)
-#pragma unroll
-          for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(q[NP == 1 ? 0 : kQ[t]][i], p[NP == 1 ? 0 : kP[t]][j], acc[j][i]);
+      for (int i = 0; i < TN; ++i) f.q[s][i] = SideQ::fragment(buf + NP * SideP::kBytes, s, (wn * TN + i) * 32, kk, lane);
     }
   };
-  if (steps > 0) load(0, lds);
-  epi.prepare(n0, lds + 2 * kStage);
+  auto multiply = [&](const Frags& f) {
+    constexpr int kPairs = NP == 3 ? 6 : 1;
+    constexpr int kP[6] = {0, 2, 1, 0, 1, 0}, kQ[6] = {2, 0, 1, 1, 0, 0};  // the small products first
+#pragma unroll
+    for (int t = 0; t < kPairs; ++t)
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+#pragma unroll
+        for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(f.q[NP == 1 ? 0 : kQ[t]][i], f.p[NP == 1 ? 0 : kP[t]][j], acc[j][i]);
+  };
+  for (int s = 0; s < STAGES - 1; ++s)
+    if (s < steps) load(s);
+  epi.prepare(n0, lds + STAGES * kStage);
   for (int64_t s = 0; s < steps; ++s) {
-    __builtin_amdgcn_s_waitcnt(0);  // this wave's copies of step s have landed ...
-    __syncthreads();                // ... and everyone's; nobody still reads the other half
-    if (s + 1 < steps) load(s + 1, lds + ((s + 1) & 1) * kStage);
-    multiply(lds + (s & 1) * kStage);
+    // this wave's copies of step s have landed (those of the STAGES - 2 steps behind it may be under way) ...
+    if (s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // ... and everyone's; nobody still reads what the next copy overwrites
+    asm volatile("" ::: "memory");
+    const char* buf = lds + s % STAGES * kStage;
+    constexpr int KK = BK / 16;
+    Frags f[2];  // the next fragments are read while these are multiplied
+    read(buf, 0, f[0]);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if (kk + 1 < KK) read(buf, kk + 1, f[(kk + 1) & 1]);
+      if (kk == 0 && s + STAGES - 1 < steps) load(s + STAGES - 1);  // behind the reads that the first products wait for
+      multiply(f[kk & 1]);
+      __builtin_amdgcn_sched_barrier(0);  // without it the compiler moves reads back to their use (dw 8192 x 4096 x 4096: 236 us, 228 with it)
+    }
   }
   if (Epi::kThroughLds || steps == 0) __syncthreads();  // LDS is the epilogue's; what prepare() left there is seen
 
 #pragma unroll
   for (int j = 0; j < TM; ++j) {
     const int64_t m_first = m0 + (wm * TM + j) * 32;
-    epi.template rows<TN>(acc[j], m_first, rows_m, n0 + wn * TN * 32, wn * TN * 32, split, lane, lds + 2 * kStage, lds + wave * kRowsLds<TN>);
+    epi.template rows<TN>(acc[j], m_first, rows_m, n0 + wn * TN * 32, wn * TN * 32, split, lane, lds + STAGES * kStage, lds + wave * kRowsLds<TN>);
   }
 }
 
