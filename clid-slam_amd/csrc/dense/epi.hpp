@@ -1,18 +1,20 @@
 // What the tiles' sums become: a layer's output, a gradient, a row's softmax statistics, a piece of dz.
-// Each gets 32 rows of a wave's sums: lane l holds row m_first + l % 32, its element (i, r) column nw + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4.
+// Each gets a wave's sums: of 32 rows, lane l holds row m_first + l % 32, its element (i, r) column nw + 32 i + 8 (r / 4) + 4 (l / 32) + r % 4.
 #pragma once
 #include "tile.hpp"
 
 namespace clid_dense {
 
-// 8 neighbouring values of a row, by 16 bytes (which need not be aligned) where there are 8
+// 8 neighbouring values of a row, by 16 bytes (which need no more alignment than the values) where there are 8
+typedef uint32_t words4 __attribute__((ext_vector_type(4), aligned(2)));
 template <typename T>
 __device__ __forceinline__ void get8(const T* p, float (&v)[8], int count) {
-  T t[8];
   if (count >= 8) {
-    __builtin_memcpy(t, p, sizeof(t));
+    union { words4 w[sizeof(T) / 2]; T t[8]; } u;
 #pragma unroll
-    for (int q = 0; q < 8; ++q) v[q] = up(t[q]);
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) u.w[i] = ((const words4*)p)[i];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[q] = up(u.t[q]);
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] = q < count ? up(p[q]) : 0.f;
@@ -21,7 +23,11 @@ __device__ __forceinline__ void get8(const T* p, float (&v)[8], int count) {
 template <typename T>
 __device__ __forceinline__ void out8(T* p, const T (&t)[8], int count) {
   if (count >= 8) {
-    __builtin_memcpy(p, t, sizeof(t));
+    union { words4 w[sizeof(T) / 2]; T t[8]; } u;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) u.t[q] = t[q];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) ((words4*)p)[i] = u.w[i];
   } else {
 #pragma unroll
     for (int q = 0; q < 8; ++q)
@@ -102,38 +108,46 @@ __device__ __forceinline__ void stage_bias(const T* bias, int64_t n0, int64_t n,
   for (int c = threadIdx.x; c < cols; c += blockDim.x) ((float*)lds)[c] = bias && n0 + c < n ? up(bias[n0 + c]) : 0.f;
 }
 
-// Sums handed on in rows: 32 rows of a wave go through its LDS once, so that 4 TN neighbouring lanes hold 8 columns each of one row and
-// loads and stores are 16 bytes wide; one loop then does whatever there is to do, where the registers' own order would need the
-// code once per register.
+// Sums handed on in rows: 64 rows of a wave at a time go through its LDS, so that 4 TN neighbouring lanes hold 8 columns each of one row and
+// loads and stores are 16 bytes wide; one loop then does whatever there is to do, where the registers' own order would need the code
+// once per register (cold instructions cost a one-tile launch more than its products).
 template <class Out, int BN>
 struct EpiRows {
   static constexpr bool kThroughLds = true;
   Out o;
   int64_t n;
   __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(o.bias, n0, n, BN, lds); }
-  template <int TN>
-  __device__ __forceinline__ void rows(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int split, int lane, const char* bias, char* lds) const {
-    constexpr int kRow = 32 * TN + 4, kLanes = 4 * TN, kStep = 64 / kLanes;
+  template <int TM, int TN>
+  __device__ __forceinline__ void rows(f32x16 (&acc)[TM][TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int split, int lane, const char* bias, char* lds) const {
+    constexpr int kRow = 32 * TN + 4, kLanes = 4 * TN, kStep = 64 / kLanes, kAtOnce = TM > 1 ? 2 : 1;
+    static_assert(TM % kAtOnce == 0, "whole turns");
     float* mine = (float*)lds;
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int i = 0; i < TN; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        *(float4*)(mine + (lane & 31) * kRow + 32 * i + 8 * j + 4 * (lane >> 5)) = float4{acc[i][4 * j], acc[i][4 * j + 1], acc[i][4 * j + 2], acc[i][4 * j + 3]};
-    __builtin_amdgcn_wave_barrier();
     const int c = (lane % kLanes) * 8;
     float b[8];
     *(float4*)b = *(const float4*)(bias + (at + c) * 4);
     *(float4*)(b + 4) = *(const float4*)(bias + (at + c) * 4 + 16);
 #pragma unroll 1
-    for (int r = lane / kLanes; r < 32; r += kStep) {
-      float v[8];
-      *(float4*)v = *(const float4*)(mine + r * kRow + c);
-      *(float4*)(v + 4) = *(const float4*)(mine + r * kRow + c + 4);
-      if (m_first + r < m_end) o.eight(v, b, m_first + r, nw + c, split);
+    for (int turn = 0; turn < TM / kAtOnce; ++turn) {
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < TM; ++j)
+        if (j / kAtOnce == turn)
+#pragma unroll
+          for (int i = 0; i < TN; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              *(float4*)(mine + (j % kAtOnce * 32 + (lane & 31)) * kRow + 32 * i + 8 * q + 4 * (lane >> 5)) =
+                  float4{acc[j][i][4 * q], acc[j][i][4 * q + 1], acc[j][i][4 * q + 2], acc[j][i][4 * q + 3]};
+      __builtin_amdgcn_wave_barrier();
+      const int64_t m0 = m_first + turn * 32 * kAtOnce;
+#pragma unroll 1
+      for (int r = lane / kLanes; r < 32 * kAtOnce; r += kStep) {
+        float v[8];
+        *(float4*)v = *(const float4*)(mine + r * kRow + c);
+        *(float4*)(v + 4) = *(const float4*)(mine + r * kRow + c + 4);
+        if (m0 + r < m_end) o.eight(v, b, m0 + r, nw + c, split);
+      }
     }
-    __builtin_amdgcn_wave_barrier();
   }
 };
 
@@ -186,8 +200,13 @@ struct EpiStat {
   int64_t m_all, n;
   static constexpr bool kThroughLds = false;
   __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(bias, n0, n, BN, lds); }
+  template <int TM, int TN>
+  __device__ __forceinline__ void rows(f32x16 (&acc)[TM][TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int, int lane, const char* lds, char*) const {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) row<TN>(acc[j], m_first + 32 * j, m_end, nw, at, lane, lds);
+  }
   template <int TN>
-  __device__ __forceinline__ void rows(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int, int lane, const char* lds, char*) const {
+  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int lane, const char* lds) const {
     const int half = lane >> 5;
     const int64_t m = m_first + (lane & 31);
     const bool on = m < m_end;
@@ -281,8 +300,13 @@ struct EpiDz {
   int64_t v0, n, ld, plane;  // columns v0 .. v0 + n, ld: n up to 8 (zeros there)
   static constexpr bool kThroughLds = false;
   __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(bias, n0, n, BN, lds); }
+  template <int TM, int TN>
+  __device__ __forceinline__ void rows(f32x16 (&acc)[TM][TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int, int lane, const char* lds, char*) const {
+#pragma unroll
+    for (int j = 0; j < TM; ++j) row<TN>(acc[j], m_first + 32 * j, m_end, nw, at, lane, lds);
+  }
   template <int TN>
-  __device__ __forceinline__ void rows(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int, int lane, const char* lds, char*) const {
+  __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int lane, const char* lds) const {
     const int half = lane >> 5;
     const int64_t m = m_first + (lane & 31);
     if (m >= m_end) return;

@@ -201,7 +201,7 @@ template <> struct Tile<1, 2> { static constexpr int BM = 256, BN = 256, BK = 64
 template <> struct Tile<1, 1> { static constexpr int BM = 128, BN = 128, BK = 64, WM = 2, WN = 2, STAGES = 4; };
 template <> struct Tile<1, 0> { static constexpr int BM = 64, BN = 64, BK = 64, WM = 2, WN = 2, STAGES = 4; };
 template <> struct Tile<3, 2> { static constexpr int BM = 256, BN = 128, BK = 32, WM = 4, WN = 2, STAGES = 2; };
-template <> struct Tile<3, 1> { static constexpr int BM = 128, BN = 64, BK = 32, WM = 2, WN = 2, STAGES = 3; };
+template <> struct Tile<3, 1> { static constexpr int BM = 128, BN = 128, BK = 32, WM = 4, WN = 2, STAGES = 3; };
 template <> struct Tile<3, 0> { static constexpr int BM = 64, BN = 64, BK = 32, WM = 2, WN = 2, STAGES = 3; };
 template <int NP>
 inline void tile_shape(int size, int* bm, int* bn, int* bk) {
@@ -252,7 +252,8 @@ inline int launch_one(Product g, const Epi& epi, hipStream_t s) {
     clid_set_error("dense product: %lld x %lld results are more than one launch takes", (long long)g.m, (long long)g.n);
     return CLID_E_SHAPE;
   }
-  constexpr int kLds = C::STAGES * NP * (C::BM + C::BN) * C::BK * 2 + C::BN * 4;
+  constexpr int kLds = tile_lds<NP, C::BM, C::BN, C::BK, C::WM, C::WN, C::STAGES>() + C::BN * 4;
+  static_assert(kLds <= 160 * 1024, "a block fits a CU");
   auto k = k_tile<Kind<T>::F16, NP, C::BM, C::BN, C::BK, C::WM, C::WN, C::STAGES, PKS, QKS, Epi>;
   const int rc = allow_lds((const void*)k, kLds);
   if (rc != CLID_OK) return rc;

@@ -114,26 +114,17 @@ struct Side {
     }
   }
 
-  // copies the tile at k0 .. k0 + BK (those below k) to LDS
-  __device__ __forceinline__ void load(const Operand& o, int64_t first, int64_t rows, int64_t k0, int64_t k, char* lds, int wave, int lane) const {
+  // copies the tile at k0 .. k0 + BK of plane s to LDS, all of it below k: nothing to check but at[]
+  __device__ __forceinline__ void load(const uint16_t* base, int s, char* lds, int wave) const {
 #pragma unroll
-    for (int s = 0; s < NP; ++s) {
-      const uint16_t* base = o.p + s * o.plane + (KS ? k0 * o.ld + first : first * o.ld + k0);
-      int64_t bytes;
-      if constexpr (KS) bytes = ((k - k0 - 1) * o.ld + (rows - first)) * 2;
-      else bytes = ((rows - first - 1) * o.ld + ((k - k0 + 7) & ~int64_t(7))) * 2;  // rows are whole chunks
-      const uint32_t bound = bytes > 0x7fffffff ? 0x7fffffffu : (uint32_t)bytes;
+    for (int i = 0; i < kLoads; ++i) copy16(base, 0x7fffffffu, at[i], lds + s * kBytes + (i * WAVES + wave) * 1024);
+  }
+  // the last step of a share that is no multiple of BK: rows (or chunks) from k on are zeros
+  __device__ __forceinline__ void load_last(const uint16_t* base, int s, char* lds, int wave, int lane, int left, int64_t ld) const {
 #pragma unroll
-      for (int i = 0; i < kLoads; ++i) {
-        uint32_t off = at[i];
-        if constexpr (!KS) {
-          if (k0 + BK > k) {  // the last step: chunks past k read zeros, not the next row
-            const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
-            if (k0 + chunk * 8 >= k) off = kOutside;
-          }
-        }
-        copy16(base, bound, off, lds + s * kBytes + (i * WAVES + wave) * 1024);
-      }
+    for (int i = 0; i < kLoads; ++i) {
+      const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
+      copy16(base, 0x7fffffffu, (KS ? row : chunk * 8) < left ? at[i] : kOutside, lds + s * kBytes + (i * WAVES + wave) * 1024);
     }
   }
 
@@ -154,8 +145,16 @@ struct Side {
   }
 };
 
-// LDS of one wave for 32 rows of its sums, a row 4 floats longer than its columns: neighbouring rows start 4 banks apart
-template <int TN> constexpr int kRowsLds = 32 * (32 * TN + 4) * 4;
+// LDS of one wave for its sums on their way out, 64 rows at a time, a row 4 floats longer than its columns: neighbouring rows start 4
+// banks apart
+template <int TM, int TN> constexpr int kRowsLds = (TM > 1 ? 64 : 32) * (32 * TN + 4) * 4;
+
+// LDS in front of the bias: the stages, later the waves' rows
+template <int NP, int BM, int BN, int BK, int WM, int WN, int STAGES>
+constexpr int tile_lds() {
+  const int stages = STAGES * NP * (BM + BN) * BK * 2, rows = WM * WN * kRowsLds<BM / WM / 32, BN / WN / 32>;
+  return stages > rows ? stages : rows;
+}
 
 // (tile row, tile column) of tile t
 __device__ __forceinline__ void place_tile(const Product& g, int64_t block, int64_t blocks, int* tm, int* tn) {
@@ -175,6 +174,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   using SideP = Side<BM, BK, NP, PKS, WAVES>;
   using SideQ = Side<BN, BK, NP, QKS, WAVES>;
   constexpr int kStage = NP * (SideP::kBytes + SideQ::kBytes);
+  constexpr int kBias = tile_lds<NP, BM, BN, BK, WM, WN, STAGES>();
   extern __shared__ __align__(16) char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN, wn = wave % WN;
@@ -189,9 +189,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   }
   const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
   if (m0 >= rows_m) return;
-  const int64_t steps_all = (rows_k + BK - 1) / BK, per = (steps_all + g.splits - 1) / g.splits;
-  const int64_t from = split * per * BK, to = (split + 1) * per * BK < rows_k ? (split + 1) * per * BK : rows_k;
-  const int64_t steps = to > from ? (to - from + BK - 1) / BK : 0;
+  const int steps_all = (int)((rows_k + BK - 1) / BK), per = (steps_all + g.splits - 1) / g.splits;
+  const int first = split * per, steps = first + per < steps_all ? per : steps_all > first ? steps_all - first : 0;
+  const int last = (int)(rows_k - (int64_t)(first + steps - 1) * BK < BK ? rows_k - (int64_t)(first + steps - 1) * BK : BK);  // values of the last step
 
   // rows of a KS operand are as long as its matrix, padded to 8
   const int64_t lim_m = PKS ? (rows_m + 7) / 8 * 8 : rows_m, lim_n = QKS ? (g.n + 7) / 8 * 8 : g.n;
@@ -208,10 +208,28 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
 
   constexpr int kLoads = NP * (SideP::kLoads + SideQ::kLoads);  // of a lane and step
-  auto load = [&](int64_t step) {
-    char* buf = lds + step % STAGES * kStage;
-    sp.load(g.p, m0, lim_m, from + step * BK, to, buf, wave, lane);
-    sq.load(g.q, n0, lim_n, from + step * BK, to, buf + NP * SideP::kBytes, wave, lane);
+  const int64_t p_step = (PKS ? BK * g.p.ld : BK), q_step = (QKS ? BK * g.q.ld : BK);
+  const uint16_t* p_at = g.p.p + (PKS ? m0 : m0 * g.p.ld) + first * p_step;
+  const uint16_t* q_at = g.q.p + (QKS ? n0 : n0 * g.q.ld) + first * q_step;
+  int loaded = 0;
+  auto load = [&]() {  // the next step's
+    char* buf = lds + loaded % STAGES * kStage;
+    if (loaded + 1 < steps || last == BK) {
+#pragma unroll
+      for (int s = 0; s < NP; ++s) {
+        sp.load(p_at + s * g.p.plane, s, buf, wave);
+        sq.load(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, wave);
+      }
+    } else {
+#pragma unroll
+      for (int s = 0; s < NP; ++s) {
+        sp.load_last(p_at + s * g.p.plane, s, buf, wave, lane, last, g.p.ld);
+        sq.load_last(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, wave, lane, last, g.q.ld);
+      }
+    }
+    ++loaded;
+    p_at += p_step;
+    q_at += q_step;
   };
   struct Frags {
     s16x8 p[NP][TM], q[NP][TN];
@@ -236,9 +254,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
         for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(f.q[NP == 1 ? 0 : kQ[t]][i], f.p[NP == 1 ? 0 : kP[t]][j], acc[j][i]);
   };
   for (int s = 0; s < STAGES - 1; ++s)
-    if (s < steps) load(s);
-  epi.prepare(n0, lds + STAGES * kStage);
-  for (int64_t s = 0; s < steps; ++s) {
+    if (s < steps) load();
+  epi.prepare(n0, lds + kBias);
+  for (int s = 0; s < steps; ++s) {
     // this wave's copies of step s have landed (those of the STAGES - 2 steps behind it may be under way) ...
     if (s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
     else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
@@ -251,18 +269,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       if (kk + 1 < KK) read(buf, kk + 1, f[(kk + 1) & 1]);
-      if (kk == 0 && s + STAGES - 1 < steps) load(s + STAGES - 1);  // behind the reads that the first products wait for
+      if (kk == 0 && s + STAGES - 1 < steps) load();  // behind the reads that the first products wait for
       multiply(f[kk & 1]);
       __builtin_amdgcn_sched_barrier(0);  // without it the compiler moves reads back to their use (dw 8192 x 4096 x 4096: 236 us, 228 with it)
     }
   }
   if (Epi::kThroughLds || steps == 0) __syncthreads();  // LDS is the epilogue's; what prepare() left there is seen
 
-#pragma unroll
-  for (int j = 0; j < TM; ++j) {
-    const int64_t m_first = m0 + (wm * TM + j) * 32;
-    epi.template rows<TN>(acc[j], m_first, rows_m, n0 + wn * TN * 32, wn * TN * 32, split, lane, lds + STAGES * kStage, lds + wave * kRowsLds<TN>);
-  }
+  epi.template rows<TM, TN>(acc, m0 + wm * TM * 32, rows_m, n0 + wn * TN * 32, wn * TN * 32, split, lane, lds + kBias, lds + wave * kRowsLds<TM, TN>);
 }
 
 }  // namespace clid_dense
