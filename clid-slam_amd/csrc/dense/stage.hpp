@@ -214,13 +214,15 @@ constexpr int kCus = 256;
 
 // Which tile, and into how many parts k is cut: the cheapest by an estimate of the time.  A CU works through its blocks one
 // after the other (rounds of 256 blocks) at a rate that grows with the tile, since a larger tile reads less LDS and memory per
-// product; a part costs its sums' trip through memory and back, and a launch.
+// product; a part costs its sums' trip through memory and back, and a launch.  The rates are those of 8192 x 2048 x 8192 bf16 (tiles 64,
+// 128, 256: 487, 416, 270 us) and 2048 x 1024 x 8192 fp32 (280, 219, 198 us); a cut costs 13 us at 2048 x 1024 x 1024 bf16 in two parts
+// (13.3 -> 26.6 us) and gains at 128 x 8192 x 1024 in eight (42.7 -> 16.7 us).
 struct Plan {
   int size, splits;
 };
 template <int NP>
 inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
-  const double rate[3] = {1.1e12, 2.6e12, 4.4e12};  // plane products' FLOP/s of a CU with tiles 0, 1, 2
+  constexpr double rate[3] = {NP == 3 ? 2.9e12 : 2.2e12, NP == 3 ? 3.7e12 : 2.6e12, NP == 3 ? 4.1e12 : 4.0e12};  // plane products' FLOP/s of a CU
   Plan best = {0, 1};
   double least = 1e300;
   for (int size = 0; size <= 2; ++size) {
@@ -230,8 +232,8 @@ inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
     for (int s = 1; s <= (may_split ? 64 : 1) && (s == 1 || s * 4 <= steps); s += s < 8 ? 1 : 8) {
       const double rounds = (double)((tiles * s + kCus - 1) / kCus);
       const double share = (double)((steps + s - 1) / s) * bk;
-      double t = rounds * (2.0 * bm * bn * share * (NP == 3 ? 6 : 1) / rate[size] + 1.5e-6);
-      if (s > 1) t += 4e-6 + (double)s * m * n * 8 / 4e12;
+      double t = rounds * (2.0 * bm * bn * share * (NP == 3 ? 6 : 1) / rate[size] + 1e-6);
+      if (s > 1) t += 6e-6 + (double)s * m * n * 8 / 3e12;
       if (t < least) {
         least = t;
         best = {size, s};
