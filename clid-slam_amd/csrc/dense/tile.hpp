@@ -18,6 +18,8 @@
 // Blocks.  Block ids go round the 8 XCDs in turn; consecutive tiles of one XCD share rows of Q (8 of them, then the next m), so that an
 // XCD's 32 CUs work on an 8 x 4 patch of tiles out of their own L2.
 #pragma once
+#include <type_traits>
+
 #include "dense.hpp"
 
 namespace clid_dense {
@@ -78,13 +80,21 @@ __device__ __forceinline__ void planes(float v, uint16_t (&h)[3]) {
   h[2] = b2 & 0x7fffffffu ? (uint16_t)(b2 >> 16) : tiny;
 }
 
+// 4 rows of 16 columns turned: lane i of 16 gives the address of 4 columns of row i / 4 and gets column i of the four rows.  (__restrict__
+// puts alias information on the read; without any the compiler waits for every copy to LDS under way before it, also for the next
+// step's, which is what arrive() is for.)
+__device__ __forceinline__ s16x4 turned(const char* __restrict__ at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
+}
+
 // R rows (m or n) x BK of one operand in LDS, NP planes
 template <int R, int BK, int NP, bool KS, int WAVES>
 struct Side {
   static constexpr int kBytes = R * BK * 2;                  // of a plane
-  static constexpr int kLoads = kBytes / 1024 / WAVES;       // 16-byte loads per lane and plane
+  static constexpr int kLoads = (kBytes / 1024 + WAVES - 1) / WAVES;  // 16-byte loads per lane and plane: all waves issue as many ...
+  static constexpr bool kWhole = kBytes % (1024 * WAVES) == 0;        // ... some of them, where this is false, of nothing into LDS that nobody reads
   static constexpr int kChunks = KS ? R / 8 : BK / 8;        // 16-byte chunks of an LDS row
-  static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
+  static_assert(kBytes % 1024 == 0, "whole loads of a wave");
 
   // where chunk c of LDS row `row` lies
   static __device__ __forceinline__ int place(int row, int c) {
@@ -106,7 +116,9 @@ struct Side {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
-      if constexpr (KS) {
+      if (!kWhole && c * 16 >= kBytes) {
+        at[i] = kOutside;
+      } else if constexpr (KS) {
         at[i] = first + chunk * 8 < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
       } else {
         at[i] = first + row < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
@@ -115,17 +127,21 @@ struct Side {
   }
 
   // copies the tile at k0 .. k0 + BK of plane s to LDS, all of it below k: nothing to check but at[]
-  __device__ __forceinline__ void load(const uint16_t* base, int s, char* lds, int wave) const {
+  __device__ __forceinline__ void load(const uint16_t* base, int s, char* lds, char* nowhere, int wave) const {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) copy16(base, 0x7fffffffu, at[i], lds + s * kBytes + (i * WAVES + wave) * 1024);
+    for (int i = 0; i < kLoads; ++i) copy16(base, 0x7fffffffu, at[i], place_of(i, s, lds, nowhere, wave));
   }
   // the last step of a share that is no multiple of BK: rows (or chunks) from k on are zeros
-  __device__ __forceinline__ void load_last(const uint16_t* base, int s, char* lds, int wave, int lane, int left, int64_t ld) const {
+  __device__ __forceinline__ void load_last(const uint16_t* base, int s, char* lds, char* nowhere, int wave, int lane, int left) const {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
-      copy16(base, 0x7fffffffu, (KS ? row : chunk * 8) < left ? at[i] : kOutside, lds + s * kBytes + (i * WAVES + wave) * 1024);
+      copy16(base, 0x7fffffffu, (KS ? row : chunk * 8) < left ? at[i] : kOutside, place_of(i, s, lds, nowhere, wave));
     }
+  }
+  static __device__ __forceinline__ char* place_of(int i, int s, char* lds, char* nowhere, int wave) {
+    const int at = (i * WAVES + wave) * 1024;
+    return kWhole || at < kBytes ? lds + s * kBytes + at : nowhere;
   }
 
   // this lane's 8 values of k (16 kk + 8 (lane / 32) ..) of row 32 t + lane % 32
@@ -138,8 +154,8 @@ struct Side {
       const int i = lane & 15, k = 16 * kk + 8 * (lane >> 5) + (i >> 2), col = first + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
       const char* at0 = lds + s * kBytes + (k * kChunks + place(k, col >> 3)) * 16 + (col & 4) * 2;
       const char* at1 = lds + s * kBytes + ((k + 4) * kChunks + place(k + 4, col >> 3)) * 16 + (col & 4) * 2;
-      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at0);
-      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at1);
+      const s16x4 a = turned(at0);
+      const s16x4 b = turned(at1);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -152,7 +168,8 @@ template <int TM, int TN> constexpr int kRowsLds = (TM > 1 ? 64 : 32) * (32 * TN
 // LDS in front of the bias: the stages, later the waves' rows
 template <int NP, int BM, int BN, int BK, int WM, int WN, int STAGES>
 constexpr int tile_lds() {
-  const int stages = STAGES * NP * (BM + BN) * BK * 2, rows = WM * WN * kRowsLds<BM / WM / 32, BN / WN / 32>;
+  const bool whole = BM * BK * 2 % (1024 * WM * WN) == 0 && BN * BK * 2 % (1024 * WM * WN) == 0;
+  const int stages = STAGES * NP * (BM + BN) * BK * 2 + (whole ? 0 : 1024), rows = WM * WN * kRowsLds<BM / WM / 32, BN / WN / 32>;
   return stages > rows ? stages : rows;
 }
 
@@ -174,7 +191,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   using SideP = Side<BM, BK, NP, PKS, WAVES>;
   using SideQ = Side<BN, BK, NP, QKS, WAVES>;
   constexpr int kStage = NP * (SideP::kBytes + SideQ::kBytes);
-  constexpr int kBias = tile_lds<NP, BM, BN, BK, WM, WN, STAGES>();
+  constexpr int kNowhere = STAGES * kStage, kBias = tile_lds<NP, BM, BN, BK, WM, WN, STAGES>();
   extern __shared__ __align__(16) char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN, wn = wave % WN;
@@ -217,14 +234,14 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
     if (loaded + 1 < steps || last == BK) {
 #pragma unroll
       for (int s = 0; s < NP; ++s) {
-        sp.load(p_at + s * g.p.plane, s, buf, wave);
-        sq.load(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, wave);
+        sp.load(p_at + s * g.p.plane, s, buf, lds + kNowhere, wave);
+        sq.load(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, lds + kNowhere, wave);
       }
     } else {
 #pragma unroll
       for (int s = 0; s < NP; ++s) {
-        sp.load_last(p_at + s * g.p.plane, s, buf, wave, lane, last, g.p.ld);
-        sq.load_last(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, wave, lane, last, g.q.ld);
+        sp.load_last(p_at + s * g.p.plane, s, buf, lds + kNowhere, wave, lane, last);
+        sq.load_last(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, lds + kNowhere, wave, lane, last);
       }
     }
     ++loaded;
@@ -253,25 +270,56 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
 #pragma unroll
         for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(f.q[NP == 1 ? 0 : kQ[t]][i], f.p[NP == 1 ? 0 : kP[t]][j], acc[j][i]);
   };
+  // Step s + 1 is there for this wave when nothing but the loads of the steps behind it is under way, and for every wave behind the barrier,
+  // where also nobody reads step s any more: its part of LDS is the next load's.
+  auto arrive = [&](bool more) {
+    if (more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  // The fragments of a product are read while the one before is multiplied, also across the barrier: the matrix pipes have the last
+  // product of step s to do while the first fragments of step s + 1 come.
+  constexpr int KK = BK / 16;
+  constexpr bool kAcross = STAGES >= 3;  // (two stages: the copy is too late for that)
+  Frags f[2];
+  auto step = [&](int s, auto parity) {
+    constexpr int kFirst = decltype(parity)::value;
+    const char* buf = lds + s % STAGES * kStage;
+    if constexpr (!kAcross) {
+      arrive(false);
+      read(buf, 0, f[kFirst]);
+    }
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      Frags &now = f[(kFirst + kk) & 1], &next = f[(kFirst + kk + 1) & 1];
+      if (KK == 1 && s + STAGES - 1 < steps) load();
+      if (kk + 1 < KK) {
+        read(buf, kk + 1, next);
+      } else if (kAcross && s + 1 < steps) {
+        arrive(s + STAGES - 1 < steps);
+        read(lds + (s + 1) % STAGES * kStage, 0, next);
+      }
+      if (KK > 1 && kk == 0 && s + STAGES - 1 < steps) load();
+      multiply(now);
+      __builtin_amdgcn_sched_barrier(0);  // without it the compiler moves reads back to their use
+    }
+  };
   for (int s = 0; s < STAGES - 1; ++s)
     if (s < steps) load();
   epi.prepare(n0, lds + kBias);
-  for (int s = 0; s < steps; ++s) {
-    // this wave's copies of step s have landed (those of the STAGES - 2 steps behind it may be under way) ...
-    if (s + STAGES - 2 < steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((STAGES - 2) * kLoads) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // ... and everyone's; nobody still reads what the next copy overwrites
-    asm volatile("" ::: "memory");
-    const char* buf = lds + s % STAGES * kStage;
-    constexpr int KK = BK / 16;
-    Frags f[2];  // the next fragments are read while these are multiplied
-    read(buf, 0, f[0]);
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      if (kk + 1 < KK) read(buf, kk + 1, f[(kk + 1) & 1]);
-      if (kk == 0 && s + STAGES - 1 < steps) load();  // behind the reads that the first products wait for
-      multiply(f[kk & 1]);
-      __builtin_amdgcn_sched_barrier(0);  // without it the compiler moves reads back to their use (dw 8192 x 4096 x 4096: 236 us, 228 with it)
+  if (steps > 0) {
+    if constexpr (kAcross) {
+      arrive(steps >= STAGES - 1);
+      read(lds, 0, f[0]);
+    }
+    if constexpr (KK % 2 == 0) {
+      for (int s = 0; s < steps; ++s) step(s, std::integral_constant<int, 0>());
+    } else {
+      for (int s = 0; s < steps; s += 2) {
+        step(s, std::integral_constant<int, 0>());
+        if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
+      }
     }
   }
   if (Epi::kThroughLds || steps == 0) __syncthreads();  // LDS is the epilogue's; what prepare() left there is seen
