@@ -9,7 +9,7 @@ using namespace clid_dense;
 namespace {
 
 constexpr int kRowsPer = 8192;  // rows a block of k_count / k_order looks at, 8 a thread
-constexpr int kJoinRows = 64;   // rows a block of k_loss_rows joins
+constexpr int kJoinRows = 16;   // rows a block of k_loss_rows joins
 
 __device__ __forceinline__ int block_scan(int v, int* total) {  // exclusive, 1024 threads
   __shared__ int wsum[16];
@@ -60,12 +60,12 @@ __global__ void __launch_bounds__(1024) k_order(const int64_t* target, int64_t r
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) order[rows] = before + total;
 }
 
-// a row's strips joined: 64 rows a block, 16 threads a row; the block's sum of losses
-__global__ void __launch_bounds__(1024) k_loss_rows(const float2* part, int strips, const float* zt, const int64_t* target, const int32_t* order,
-                                                    int64_t rows, int n, float4* stat, float* loss_none, double* sums) {
-  __shared__ float pm[16][kJoinRows], pr[16][kJoinRows];
+// a row's strips joined: 16 rows a block, 32 threads a row; the block's sum of losses
+__global__ void __launch_bounds__(512) k_loss_rows(const float2* part, int strips, const float* zt, const int64_t* target, const int32_t* order,
+                                                   int64_t rows, int n, float4* stat, float* loss_none, double* sums) {
+  __shared__ float pm[32][kJoinRows], pr[32][kJoinRows];
   const int64_t live = order[rows];
-  const int row = threadIdx.x & 63, g = threadIdx.x >> 6;
+  const int row = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
   const int64_t j = (int64_t)blockIdx.x * kJoinRows + row;
   if ((int64_t)blockIdx.x * kJoinRows >= live) {
     if (threadIdx.x == 0) sums[blockIdx.x] = 0.0;
@@ -73,7 +73,8 @@ __global__ void __launch_bounds__(1024) k_loss_rows(const float2* part, int stri
   }
   Stat s = {neg_inf(), 0.f, 0};
   if (j < live)
-    for (int i = g; i < strips; i += 16) {
+#pragma unroll 4
+    for (int i = g; i < strips; i += 32) {
       const float2 p = part[(int64_t)i * rows + j];
       s = join(s, {p.x, p.y, 0});
     }
@@ -83,14 +84,14 @@ __global__ void __launch_bounds__(1024) k_loss_rows(const float2* part, int stri
   if (g) return;
   double sum = 0.0;
   if (j < live) {
-    for (int i = 1; i < 16; ++i) s = join(s, {pm[i][row], pr[i][row], 0});
+    for (int i = 1; i < 32; ++i) s = join(s, {pm[i][row], pr[i][row], 0});
     const int64_t m = order[j], t = target[m];
     const float loss = t >= 0 && t < n ? (s.m - zt[j]) + log1pf(s.r) : __builtin_nanf("");
     stat[j] = {s.m, 1.f / (1.f + s.r), expm1f(-loss), loss};
     if (loss_none) loss_none[m] = loss;
     sum = loss;
   }
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
+  for (int d = kJoinRows / 2; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
   if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
 __global__ void __launch_bounds__(1024) k_loss_total(const double* sums, int blocks, const int32_t* live, int reduction, float* total, float* loss_out) {
@@ -244,7 +245,7 @@ int ce_fwd(const clid_ce_args* a, hipStream_t s) {
     Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, v.order, live), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), live, 0, 1, 0, 0};
     const int rc = launch_stat<T, false>(g, f.p.size, (const T*)a->bias, a->target, v.order, (float2*)f.part, nullptr, (float*)f.zt, s);
     if (rc != CLID_OK) return rc;
-    hipLaunchKernelGGL(k_loss_rows, dim3(f.joins), dim3(1024), 0, s, (const float2*)f.part, f.strips, (const float*)f.zt, a->target, v.order, a->rows, a->n,
+    hipLaunchKernelGGL(k_loss_rows, dim3(f.joins), dim3(512), 0, s, (const float2*)f.part, f.strips, (const float*)f.zt, a->target, v.order, a->rows, a->n,
                        v.stat, none, (double*)f.sums);
   }
   hipLaunchKernelGGL(k_loss_total, dim3(1), dim3(1024), 0, s, (const double*)f.sums, f.joins, a->rows ? v.order + a->rows : nullptr, a->reduction, v.total, a->loss_out);

@@ -207,52 +207,69 @@ struct EpiStat {
   }
   template <int TN>
   __device__ __forceinline__ void row(f32x16 (&acc)[TN], int64_t m_first, int64_t m_end, int64_t nw, int at, int lane, const char* lds) const {
+    if (nw >= n) return;
     const int half = lane >> 5;
     const int64_t m = m_first + (lane & 31);
     const bool on = m < m_end;
-    if (nw >= n) return;
-    int t = -1;
+    if (bias) {
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float4 b = *(const float4*)(lds + (at + 32 * i + 8 * j + 4 * half) * 4);
+          acc[i][4 * j] += b.x; acc[i][4 * j + 1] += b.y; acc[i][4 * j + 2] += b.z; acc[i][4 * j + 3] += b.w;
+        }
+    }
+    if (nw + 32 * TN > n) {  // columns that are not there
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (nw + 32 * i + 8 * (r >> 2) + 4 * half + (r & 3) >= n) acc[i][r] = neg_inf();
+    }
     if constexpr (!LABEL) {
-      if (on) {
-        const int64_t tt = target[order[m]];
-        t = tt >= nw && tt < nw + 32 * TN ? (int)(tt - nw) : -1;
+      const int64_t tt = on ? target[order[m]] - nw : -1;
+      const int t = tt >= 0 && tt < 32 * TN ? (int)tt : -1;
+      if (__any(t >= 0)) {  // few waves hold a target of theirs
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (t == 32 * i + 8 * (r >> 2) + 4 * half + (r & 3)) zt[m] = acc[i][r];
       }
     }
     float top = neg_inf();
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int c = 32 * i + 8 * j + 4 * half;
-        const float4 b4 = *(const float4*)(lds + (at + c) * 4);
-        const float b[4] = {b4.x, b4.y, b4.z, b4.w};
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          float z = acc[i][4 * j + q] + b[q];
-          if constexpr (!LABEL)
-            if (t == c + q) zt[m] = z;
-          z = nw + c + q < n ? z : neg_inf();
-          acc[i][4 * j + q] = z;
-          top = fmaxf(top, z);
-        }
-      }
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float safe = top == neg_inf() ? 0.f : top;
+    // sum of all exp(z - top), the largest one's 1 among them; where the others are less than 2^-6 of it that sum has lost their last
+    // bits, and they are added up again without it
     float rest = 0.f;
-    int same = 0;
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const float z = acc[i][r];
-        const bool is = z == top;
-        rest += is ? 0.f : __builtin_amdgcn_exp2f((z - safe) * 1.4426950408889634f);
-        same += is;
-      }
+      for (int r = 0; r < 16; ++r) rest += __builtin_amdgcn_exp2f((acc[i][r] - safe) * 1.4426950408889634f);
     rest += __shfl_xor(rest, 32, 64);
-    same += __shfl_xor(same, 32, 64);
-    // columns that share the largest value: one of them is `m`, the others count as exp(0); without a finite value none does
-    rest = top == neg_inf() ? (rest == rest ? 0.f : rest) : rest + (float)(same - 1);
+    rest -= 1.f;
+    if (__any(!(rest >= 0.015625f))) {
+      float again = 0.f;
+      int same = 0;
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const bool is = acc[i][r] == top;
+          again += is ? 0.f : __builtin_amdgcn_exp2f((acc[i][r] - safe) * 1.4426950408889634f);
+          same += is;
+        }
+      again += __shfl_xor(again, 32, 64);
+      same += __shfl_xor(same, 32, 64);
+      if (!(rest >= 0.015625f)) rest = again + (float)(same - 1);
+    }
+    if (top == neg_inf()) rest = rest == rest ? 0.f : rest;  // nothing finite here: a join counts nothing
     if (top == __builtin_inff()) rest = __builtin_nanf("");
     int best = 0x7fffffff;
     if constexpr (LABEL) {
@@ -263,7 +280,7 @@ struct EpiStat {
 #pragma unroll
         for (int r = 15; r >= 0; --r)
           if (acc[i][r] == top) best = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
-      if (odd) {
+      if (__any(odd)) {
         int first = 0x7fffffff;
 #pragma unroll
         for (int i = TN - 1; i >= 0; --i)
@@ -272,7 +289,7 @@ struct EpiStat {
             if (acc[i][r] != acc[i][r]) first = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
         const int other = __shfl_xor(first, 32, 64);
         first = other < first ? other : first;
-        nan = first != 0x7fffffff;
+        nan = odd && first != 0x7fffffff;
         if (nan) best = first;
       }
       if (nan) top = __builtin_nanf("");
@@ -316,39 +333,50 @@ struct EpiDz {
     const int t = tt >= 0 && tt < 32 * TN ? (int)tt : -1;
     float f = scale[0];
     if (g) f *= g[from];
-    const float inv = s.w != s.w ? s.w : s.y * f, hit = s.z * f;
+    const float inv = s.w != s.w ? s.w : s.y * f;
+    const bool tail = nw + 32 * TN > n;
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int c = 32 * i + 8 * j + 4 * half;
-        if (nw + c >= ld) continue;
-        const float4 b4 = *(const float4*)(lds + (at + c) * 4);
-        const float b[4] = {b4.x, b4.y, b4.z, b4.w};
+        if (tail && nw + c >= ld) continue;
         float v[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const float p = __builtin_amdgcn_exp2f((acc[i][4 * j + q] + b[q] - s.x) * 1.4426950408889634f) * inv;
-          v[q] = nw + c + q < n ? (t == c + q ? hit : p) : 0.f;
+        if (bias) {
+          const float4 b = *(const float4*)(lds + (at + c) * 4);
+          acc[i][4 * j] += b.x; acc[i][4 * j + 1] += b.y; acc[i][4 * j + 2] += b.z; acc[i][4 * j + 3] += b.w;
         }
-        uint16_t* to = dz + m * ld + nw + c;
-        if constexpr (NP == 1) {
-          union { ushort4 w; T t[4]; } u;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) u.t[q] = down<T>(v[q]);
-          *(ushort4*)to = u.w;
-        } else {
-          union { ushort4 w; uint16_t t[4]; } u[3];
+        for (int q = 0; q < 4; ++q) v[q] = __builtin_amdgcn_exp2f((acc[i][4 * j + q] - s.x) * 1.4426950408889634f) * inv;
+        if (tail) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint16_t h[3];
-            planes(v[q], h);
-            for (int s3 = 0; s3 < 3; ++s3) u[s3].t[q] = h[s3];
-          }
-#pragma unroll
-          for (int s3 = 0; s3 < 3; ++s3) *(ushort4*)(to + s3 * plane) = u[s3].w;
+          for (int q = 0; q < 4; ++q) v[q] = nw + c + q < n ? v[q] : 0.f;
         }
+        put<4>(dz + m * ld + nw + c, v);
       }
+    if (t >= 0 && (t >> 2 & 1) == half) {  // the target's, over what was stored for it
+      const float hit[1] = {s.z * f};
+      put<1>(dz + m * ld + nw + t, hit);
+    }
+  }
+  template <int N>
+  __device__ __forceinline__ void put(uint16_t* to, const float (&v)[N]) const {
+    if constexpr (NP == 1) {
+      union { uint16_t w[N]; T t[N]; } u;
+#pragma unroll
+      for (int q = 0; q < N; ++q) u.t[q] = down<T>(v[q]);
+      if constexpr (N == 4) *(ushort4*)to = ushort4{u.w[0], u.w[1], u.w[2], u.w[3]};
+      else to[0] = u.w[0];
+    } else {
+      uint16_t h[N][3];
+#pragma unroll
+      for (int q = 0; q < N; ++q) planes(v[q], h[q]);
+#pragma unroll
+      for (int s3 = 0; s3 < 3; ++s3) {
+        if constexpr (N == 4) *(ushort4*)(to + s3 * plane) = ushort4{h[0][s3], h[1][s3], h[2][s3], h[3][s3]};
+        else to[s3 * plane] = h[0][s3];
+      }
+    }
   }
 };
 

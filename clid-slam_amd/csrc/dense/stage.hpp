@@ -82,20 +82,30 @@ __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* 
   __shared__ float sums[8][256 + 8];
   const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8, count = n - c < 8 ? n - c : 8;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < np)
-    for (int64_t m = (int64_t)blockIdx.y * 8 + rr; m < rows; m += (int64_t)gridDim.y * 8) {
-      float v[8];
-      get8(dy + m * lddy + c, v, count);
+  if (c < np) {
+    const int64_t step = (int64_t)gridDim.y * 8;
+    for (int64_t m = (int64_t)blockIdx.y * 8 + rr; m < rows; m += 2 * step) {  // two rows' loads at once
+      const bool two = m + step < rows;
+      float v[2][8], y[2][8];
+      get8(dy + m * lddy + c, v[0], count);
+      if (two) get8(dy + (m + step) * lddy + c, v[1], count);
       if (z) {
-        float y[8];
-        get8(z + m * n + c, y, count);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = q < count ? v[q] * act_slope(y[q], act) : 0.f;
+        get8(z + m * n + c, y[0], count);
+        if (two) get8(z + (m + step) * n + c, y[1], count);
       }
 #pragma unroll
-      for (int q = 0; q < 8; ++q) sum[q] += v[q];
-      if (dst) put8<T>(dst + m * np + c, plane, v);
+      for (int t = 0; t < 2; ++t) {
+        if (t && !two) break;
+        if (z) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[t][q] = q < count ? v[t][q] * act_slope(y[t][q], act) : 0.f;
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) sum[q] += v[t][q];
+        if (dst) put8<T>(dst + (m + t * step) * np + c, plane, v[t]);
+      }
     }
+  }
   if (!part) return;
 #pragma unroll
   for (int q = 0; q < 8; ++q) sums[rr][cg * 8 + q] = sum[q];
@@ -155,7 +165,7 @@ __global__ void __launch_bounds__(1024) k_colsum_join(const float* part, int blo
   out[c] = down<T>((alpha ? *alpha : 1.f) * s);
 }
 inline int row_blocks(int64_t rows, int n) {
-  const int64_t cols = (n + 255) / 256, want = 1024 / cols + 1, most = (rows + 63) / 64;
+  const int64_t cols = (n + 255) / 256, want = 2048 / cols + 1, most = (rows + 15) / 16;
   return (int)(most < want ? most : want);
 }
 
@@ -214,15 +224,15 @@ constexpr int kCus = 256;
 
 // Which tile, and into how many parts k is cut: the cheapest by an estimate of the time.  A CU works through its blocks one
 // after the other (rounds of 256 blocks) at a rate that grows with the tile, since a larger tile reads less LDS and memory per
-// product; a part costs its sums' trip through memory and back, and a launch.  The rates are those of 8192 x 2048 x 8192 bf16 (tiles 64,
-// 128, 256: 487, 416, 270 us) and 2048 x 1024 x 8192 fp32 (280, 219, 198 us); a cut costs 13 us at 2048 x 1024 x 1024 bf16 in two parts
-// (13.3 -> 26.6 us) and gains at 128 x 8192 x 1024 in eight (42.7 -> 16.7 us).
+// product; a part costs its sums' trip through memory and back, and a launch.  The rates are about those of 8192 x 2048 x 8192 bf16 (tiles
+// 64, 128, 256: 474, 396, 256 us) and 2048 x 1024 x 8192 fp32 (274, 209, 194 us); a cut costs 13 us at 2048 x 1024 x 1024 bf16 in two
+// parts (13.3 -> 26.6 us) and gains at 128 x 8192 x 1024 in eight (40 -> 17.7 us).
 struct Plan {
   int size, splits;
 };
 template <int NP>
 inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
-  constexpr double rate[3] = {NP == 3 ? 2.9e12 : 2.2e12, NP == 3 ? 3.7e12 : 2.6e12, NP == 3 ? 4.1e12 : 4.0e12};  // plane products' FLOP/s of a CU
+  constexpr double rate[3] = {NP == 3 ? 2.6e12 : 2.3e12, NP == 3 ? 3.7e12 : 2.8e12, NP == 3 ? 4.2e12 : 4.6e12};  // plane products' FLOP/s of a CU
   Plan best = {0, 1};
   double least = 1e300;
   for (int size = 0; size <= 2; ++size) {
@@ -233,7 +243,7 @@ inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
       const double rounds = (double)((tiles * s + kCus - 1) / kCus);
       const double share = (double)((steps + s - 1) / s) * bk;
       double t = rounds * (2.0 * bm * bn * share * (NP == 3 ? 6 : 1) / rate[size] + 1e-6);
-      if (s > 1) t += 6e-6 + (double)s * m * n * 8 / 3e12;
+      if (s > 1) t += 6e-6 + (double)s * m * n * 8 / 4e12;
       if (t < least) {
         least = t;
         best = {size, s};
