@@ -376,11 +376,11 @@ extern "C" int64_t clid_ce_workspace(const clid_ce_args* a) {
 extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
   const char* me = "clid_ce_fwd";
   if (!ce_ok(a)) return bad(me, "bad argument");
-  if (!a->saved || (a->rows && (!a->x || !a->w || !a->target || a->ldx < a->k || a->ldw < a->k)) ||
+  if (!a->saved || (uintptr_t)a->saved % 256 || (a->rows && (!a->x || !a->w || !a->target || a->ldx < a->k || a->ldw < a->k)) ||
       (!a->loss_out && !(a->reduction == CLID_REDUCE_NONE && a->rows == 0)))
     return bad(me, "bad pointer or row stride");
   const int64_t need = clid_ce_workspace(a);
-  if (a->rows && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  if (a->rows && !ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n) && a->rows) rc = narrow_ce(a, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = ce_fwd<T>(a, (hipStream_t)stream););
@@ -397,9 +397,9 @@ extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
   const char* me = "clid_ce_bwd";
   if (!ce_ok(a)) return bad(me, "bad argument");
   if (a->rows == 0) return bad(me, "no rows");
-  if (!a->x || !a->w || !a->target || !a->saved || !a->g || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
+  if (!a->x || !a->w || !a->target || !a->saved || (uintptr_t)a->saved % 256 || !a->g || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
   const int64_t need = clid_ce_bwd_workspace(a);
-  if (!a->ws || a->ws_bytes < need) return bad(me, "workspace too small");
+  if (!ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_ce_bwd(a, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = ce_bwd<T>(a, (hipStream_t)stream););
@@ -420,7 +420,7 @@ extern "C" int clid_label_fwd(const clid_label_args* a, void* stream) {
   if (a->rows == 0) return CLID_OK;
   if (!a->x || !a->w || !a->label || !a->log_prob || a->ldx < a->k || a->ldw < a->k) return bad(me, "bad pointer or row stride");
   const int64_t need = clid_label_workspace(a);
-  if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  if (!ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_label(a, (hipStream_t)stream);
   else if (is_few(a->rows)) rc = few_label(a, (hipStream_t)stream);

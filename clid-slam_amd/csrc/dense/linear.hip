@@ -98,7 +98,7 @@ extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
   if (a->rows == 0) return CLID_OK;
   if (!a->x || !a->w || !a->y || a->ldx < a->k || a->ldw < a->k || (a->residual && a->ldr < a->n)) return bad(me, "bad pointer or row stride");
   const int64_t need = clid_linear_workspace(a);
-  if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  if (!ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_linear(a, (hipStream_t)stream);
   else if (is_few(a->rows)) rc = few_linear(a, (hipStream_t)stream);
@@ -119,7 +119,7 @@ extern "C" int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream) {
   if (a->rows == 0) return bad(me, "no rows");
   if (!a->x || !a->w || !a->dy || a->ldx < a->k || a->ldw < a->k || a->lddy < a->n || (!a->z && a->act != CLID_ACT_NONE)) return bad(me, "bad pointer or row stride");
   const int64_t need = clid_linear_bwd_workspace(a);
-  if (need && (!a->ws || a->ws_bytes < need)) return bad(me, "workspace too small");
+  if (!ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_linear_bwd(a, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = bwd<T>(a, (hipStream_t)stream););

@@ -310,6 +310,8 @@ inline int bad(const char* what, const char* why) {
   clid_set_error("%s: %s", what, why);
   return CLID_E_ARG;
 }
+// a workspace of `need` bytes as the header asks for it
+inline bool ws_ok(const void* ws, int64_t bytes, int64_t need) { return need == 0 || (ws && bytes >= need && (reinterpret_cast<uintptr_t>(ws) & 255) == 0); }
 inline bool dtype_ok(int d) { return d == CLID_F32 || d == CLID_BF16 || d == CLID_F16; }
 
 }  // namespace clid_dense

@@ -57,19 +57,19 @@ _SIGS = {
     "clid_label_fwd": (C.c_int, [C.POINTER(LabelArgs), _vp]),
 }
 EXPORTS = tuple(_SIGS)
-_bound = None
+_functions = {}
 
 
 def load():
     """The shared library with the dense entry points' signatures set (once)."""
-    global _bound
-    if _bound is None:
-        lib = _lib.load()
+    lib = _lib.load()
+    if not _functions:
+        bound = {}
         for name, (res, args) in _SIGS.items():
-            fn = getattr(lib, name)
+            bound[name] = fn = getattr(lib, name)
             fn.restype, fn.argtypes = res, args
-        _bound = lib
-    return _bound
+        _functions.update(bound)
+    return lib
 
 
 # (The small shapes are over in 10 us on the GPU, so what Python does around a call is kept to what is needed: no tensor is made only to read its
@@ -77,17 +77,18 @@ def load():
 def call(entry: str, workspace: str, args, device) -> None:
     """One entry point on torch's current stream of `device`, with its workspace from torch's allocator: a buffer of this call
     alone, which the allocator gives back in stream order (and keeps for a graph that is being captured)."""
-    if device.index != torch.cuda.current_device():
+    index = device.index
+    if index != torch.cuda.current_device():
         with torch.cuda.device(device):
             return call(entry, workspace, args, device)
-    lib, ref = _bound or load(), C.byref(args)
-    need = getattr(lib, workspace)(ref)
+    fn, ref = _functions or load() and _functions, C.byref(args)
+    need = fn[workspace](ref)
     if need:
         if need < 0:
             _lib.check(int(need), workspace)
         ws = torch.empty(need, dtype=torch.uint8, device=device)
         args.ws, args.ws_bytes = ws.data_ptr(), need
-    rc = getattr(lib, entry)(ref, _lib.stream())
+    rc = fn[entry](ref, _lib.stream())
     if rc:
         _lib.check(rc, entry)
 
@@ -131,7 +132,11 @@ def _like(what, name, t, shape, dtype, device):
 
 
 def wants_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _forward(x, weight, bias, act, residual, keep_z):
