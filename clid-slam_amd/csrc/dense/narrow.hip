@@ -6,7 +6,7 @@
 // softmax is 16 or 32 registers and one exchange between two lanes, with no partial results in memory.  The same registers are the
 // column operand of dx = dz w as they are (the contraction over n takes its columns in that order, and so does the row operand, read from
 // w in LDS).  dw = dz^T x contracts over m: dz goes through LDS once, x is there already; the sums over a wave's rows stay in
-// accumulators, a block's four waves add theirs in LDS, k_narrow_join adds the blocks' in their order.  Nothing is rounded before the
+// accumulators, a block's waves add theirs in LDS, k_narrow_join adds the blocks' in their order.  Nothing is rounded before the
 // results, whatever the type.  The cross entropy's backward pass makes z again rather than keeping anything of it.
 //
 // x comes by 16-byte copies straight to LDS, the next 32 rows' while these are worked on; chunks are permuted within their row so that the
@@ -47,49 +47,62 @@ struct Narrow {
 
 __device__ __forceinline__ f32x16 mfma_f32(float a, float b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, 0, 0, 0); }
 
-// 4 neighbouring values of a row, in one load or store (which need not be aligned) where there are 4
-template <typename T>
-__device__ __forceinline__ void get4(const T* p, float (&v)[4], int count) {
-  T t[4];
-  if (count >= 4) {
-    __builtin_memcpy(t, p, sizeof(t));
+// 32 rows of 32 T fp32 values in a wave's LDS, 16-byte chunks permuted within the row.  The products leave them lane by row (a lane holds row
+// lane % 32, chunks 8 i + 2 j + lane / 32); memory wants them 8 neighbouring values a lane.
+template <int T>
+struct Rows32 {
+  static __device__ __forceinline__ float* chunk(float* tile, int row, int c) { return tile + row * 32 * T + (c ^ (row & (8 * T - 1))) * 4; }
+  static __device__ __forceinline__ void put(float* tile, const f32x16 (&v)[T], int lane) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = up(t[q]);
-  } else {
+    for (int i = 0; i < T; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; ++q) v[q] = q < count ? up(p[q]) : 0.f;
+      for (int j = 0; j < 4; ++j)
+        *(float4*)chunk(tile, lane & 31, 8 * i + 2 * j + (lane >> 5)) = float4{v[i][4 * j], v[i][4 * j + 1], v[i][4 * j + 2], v[i][4 * j + 3]};
   }
-}
-template <typename T>
-__device__ __forceinline__ void put4(T* p, const T (&t)[4], int count) {
-  if (count >= 4) {
-    __builtin_memcpy(p, t, sizeof(t));
-  } else {
+  static __device__ __forceinline__ void get(float* tile, f32x16 (&v)[T], int lane) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q)
-      if (q < count) p[q] = t[q];
+    for (int i = 0; i < T; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float4 f = *(const float4*)chunk(tile, lane & 31, 8 * i + 2 * j + (lane >> 5));
+        v[i][4 * j] = f.x; v[i][4 * j + 1] = f.y; v[i][4 * j + 2] = f.z; v[i][4 * j + 3] = f.w;
+      }
   }
-}
+  // f(row, first column, 8 values) over the tile: one copy of its code, 4 T neighbouring lanes a row
+  template <class F>
+  static __device__ __forceinline__ void each8(float* tile, int lane, const F& f) {
+    const int c = lane % (4 * T);
+#pragma unroll 1
+    for (int row = lane / (4 * T); row < 32; row += 16 / T) {
+      float v[8];
+      float *lo = chunk(tile, row, 2 * c), *hi = chunk(tile, row, 2 * c + 1);
+      *(float4*)v = *(const float4*)lo;
+      *(float4*)(v + 4) = *(const float4*)hi;
+      f(row, 8 * c, v, lo, hi);
+    }
+  }
+};
 
 // TN: 32 columns of z each; KQ: runs of 8 along k
 template <typename T, int TN, int KQ, Do DO>
 struct NarrowShape {
+  static constexpr int max_of(int a, int b) { return a > b ? a : b; }
   static constexpr bool kBwd = DO == Do::LinearBwd || DO == Do::CeBwd;
   static constexpr int kChunkElems = 16 / sizeof(T);
   static constexpr int kChunks = 8 * KQ / kChunkElems;             // of an x row in LDS: 2, 4, 8 or 16
-  static constexpr int kXBuf = 32 * kChunks * 16;                  // 32 rows
-  static constexpr int kXLoads = kXBuf / 1024;
+  static constexpr int kTK = (8 * KQ + 31) / 32;
+  static constexpr int kXLoads = 32 * kChunks * 16 / 1024;
+  // 32 rows; the same place then holds 32 rows of fp32 results on their way out (y, dx)
+  static constexpr int kOutT = DO == Do::Linear ? TN : kBwd ? kTK : 0;
+  static constexpr int kXBuf = max_of(32 * kChunks * 16, 32 * kOutT * 128);
   static constexpr int kMostWaves = kBwd ? 4 : 8;
   static constexpr int kWRow = 8 * KQ + 4;                         // floats
   static constexpr int kWBytes = 32 * TN * kWRow * 4;
-  static constexpr int kZRow = 32 * TN + 4;
-  static constexpr int kZBytes = kBwd ? 32 * kZRow * 4 : 0;
+  static constexpr int kZBytes = kBwd ? 32 * 32 * TN * 4 : 0;
   static constexpr int kWave = 2 * kXBuf + kZBytes;
-  static constexpr int kTK = (8 * KQ + 31) / 32;
   static constexpr int kHead = kWBytes + 32 * TN * 4;
   static constexpr int kSumRow = 32 * kTK + 1, kSums = 32 * TN * kSumRow + 32 * TN;  // a wave's sums for dw and db, floats
   static constexpr int lds(int waves) { return max_of(kHead + waves * kWave, kBwd ? waves * kSums * 4 : waves * 16); }
-  static constexpr int max_of(int a, int b) { return a > b ? a : b; }
   // 16 chunks span the banks once: the rows between them are told apart by the chunk's place
   static __device__ __forceinline__ int place(int row, int c) { return c ^ ((row / (16 / kChunks)) & (kChunks - 1)); }
 };
@@ -174,7 +187,10 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     auto x4 = [&](int q, float (&v)[4]) {  // x[m][8 q + 4 half ..]
       const int k = 8 * q + 4 * half;
       const T* p = (const T*)(xs + (col * S::kChunks + S::place(col, k / S::kChunkElems)) * 16) + k % S::kChunkElems;
-      get4((const T*)__builtin_assume_aligned(p, 4 * sizeof(T)), v, 4);
+      struct alignas(4 * sizeof(T)) Run { T t[4]; };
+      const Run r = *(const Run*)p;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = up(r.t[e]);
     };
     f32x16 z[TN];
     if constexpr (DO != Do::LinearBwd) {
@@ -201,25 +217,15 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     }
 
     if constexpr (DO == Do::Linear) {
-      if (on)
-#pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int n = 32 * i + 8 * j + 4 * half, count = a.n - n;
-            if (count <= 0) continue;
-            float r[4] = {0.f, 0.f, 0.f, 0.f};
-            if (a.res) get4((const T*)a.res + m * a.ldr + n, r, count);
-            T t[4];
-            if (a.z_out) {
-#pragma unroll
-              for (int q = 0; q < 4; ++q) t[q] = keep_z<T>(z[i][4 * j + q]);
-              put4((T*)a.z_out + m * a.n + n, t, count);
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) t[q] = down<T>(act_value(z[i][4 * j + q], a.act) + r[q]);
-            put4((T*)a.y + m * a.n + n, t, count);
-          }
+      const LinearOut<T> o = {nullptr, (const T*)a.res, (T*)a.y, (T*)a.z_out, a.ldr, a.n, a.act};
+      float* tile = (float*)xs;  // x is done with
+      Rows32<TN>::put(tile, z, lane);
+      __builtin_amdgcn_wave_barrier();
+      Rows32<TN>::each8(tile, lane, [&](int row, int c, float (&v)[8], float*, float*) {
+        const float none[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};  // the bias is in z
+        if (m0 + row < a.rows) o.eight(v, none, m0 + row, c, 0);
+      });
+      __builtin_amdgcn_wave_barrier();
     }
 
     // a row's statistics: the largest z, its column, sum over the others of exp(z - largest), the target's z
@@ -300,23 +306,20 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     if constexpr (S::kBwd) {
       // z becomes dz
       if constexpr (DO == Do::LinearBwd) {
+        Rows32<TN>::each8(zbuf, lane, [&](int row, int c, float (&v)[8], float* lo, float* hi) {
+          const int count = m0 + row < a.rows ? a.n - c : 0;
+          get8((const T*)a.dy + (m0 + row) * a.lddy + c, v, count);
+          if (a.z_in) {
+            float y[8];
+            get8((const T*)a.z_in + (m0 + row) * a.n + c, y, count);
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int n = 32 * i + 8 * j + 4 * half, count = on ? a.n - n : 0;
-            float v[4] = {0.f, 0.f, 0.f, 0.f}, y[4];
-            if (count > 0) {
-              get4((const T*)a.dy + m * a.lddy + n, v, count);
-              if (a.z_in) {
-                get4((const T*)a.z_in + m * a.n + n, y, count);
-#pragma unroll
-                for (int q = 0; q < 4; ++q) v[q] = q < count ? v[q] * act_slope(y[q], a.act) : 0.f;
-              }
-            }
-#pragma unroll
-            for (int q = 0; q < 4; ++q) z[i][4 * j + q] = v[q];
+            for (int q = 0; q < 8; ++q) v[q] = q < count ? v[q] * act_slope(y[q], a.act) : 0.f;
           }
+          *(float4*)lo = *(const float4*)v;
+          *(float4*)hi = *(const float4*)(v + 4);
+        });
+        __builtin_amdgcn_wave_barrier();
+        Rows32<TN>::get(zbuf, z, lane);
       } else {
         float f = 0.f;
         if (counts) f = a.reduction == CLID_REDUCE_NONE ? a.g[m] : a.reduction == CLID_REDUCE_MEAN ? a.g[0] / fmaxf(a.total[1], 1.f) : a.g[0];
@@ -334,14 +337,29 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
       for (int i = 0; i < TN; ++i)
 #pragma unroll
         for (int r = 0; r < 16; ++r) sum_b[i][r] += z[i][r];
+      if constexpr (DO == Do::CeBwd) Rows32<TN>::put(zbuf, z, lane);
+      __builtin_amdgcn_wave_barrier();
+      // rows that do not count are zeros whatever they hold
+      const uint32_t live = DO == Do::CeBwd ? (uint32_t)__ballot(counts) : 0xffffffffu;
       if (a.want_w) {
 #pragma unroll
-        for (int i = 0; i < TN; ++i)
+        for (int s = 0; s < 16; ++s) {
+          const int mm = 2 * s + half;
+          float xv[TK];
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *(float4*)(zbuf + col * S::kZRow + 32 * i + 8 * j + 4 * half) = float4{z[i][4 * j], z[i][4 * j + 1], z[i][4 * j + 2], z[i][4 * j + 3]};
+          for (int t = 0; t < TK; ++t) {
+            const int k = 32 * t + col;
+            xv[t] = 0.f;
+            if ((8 * KQ >= 32 || k < 8 * KQ) && (live >> mm & 1)) xv[t] = up(((const T*)(xs + (mm * S::kChunks + S::place(mm, k / S::kChunkElems)) * 16))[k % S::kChunkElems]);
+          }
+#pragma unroll
+          for (int i = 0; i < TN; ++i) {
+            const float zv = Rows32<TN>::chunk(zbuf, mm, 8 * i + (col >> 2))[col & 3];
+#pragma unroll
+            for (int t = 0; t < TK; ++t) sum_w[i][t] = mfma_f32(zv, xv[t], sum_w[i][t]);
+          }
+        }
       }
-      __builtin_amdgcn_wave_barrier();
       if (a.dx) {
         f32x16 d[TK];
 #pragma unroll
@@ -359,40 +377,18 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
               d[t] = mfma_f32(8 * KQ >= 32 || k < 8 * KQ ? w[n * S::kWRow + k] : 0.f, z[i][r], d[t]);
             }
           }
-        if (on)
+        __builtin_amdgcn_wave_barrier();
+        float* tile = (float*)xs;  // x is done with
+        Rows32<TK>::put(tile, d, lane);
+        __builtin_amdgcn_wave_barrier();
+        Rows32<TK>::each8(tile, lane, [&](int row, int c, float (&v)[8], float*, float*) {
+          if (m0 + row >= a.rows) return;
+          const bool zero = DO == Do::CeBwd && !(live >> row & 1);
+          T t[8];
 #pragma unroll
-          for (int t = 0; t < TK; ++t)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int k = 32 * t + 8 * j + 4 * half, count = a.k - k;
-              if (count <= 0) continue;
-              const bool zero = DO == Do::CeBwd && !counts;
-              T v[4];
-#pragma unroll
-              for (int q = 0; q < 4; ++q) v[q] = down<T>(zero ? 0.f : d[t][4 * j + q]);
-              put4((T*)a.dx + m * a.k + k, v, count);
-            }
-      }
-      if (a.want_w) {
-        // rows that do not count are zeros whatever they hold
-        const uint32_t live = DO == Do::CeBwd ? (uint32_t)__ballot(counts) : 0xffffffffu;
-#pragma unroll
-        for (int s = 0; s < 16; ++s) {
-          const int mm = 2 * s + half;
-          float xv[TK];
-#pragma unroll
-          for (int t = 0; t < TK; ++t) {
-            const int k = 32 * t + col;
-            xv[t] = 0.f;
-            if ((8 * KQ >= 32 || k < 8 * KQ) && (live >> mm & 1)) xv[t] = up(((const T*)(xs + (mm * S::kChunks + S::place(mm, k / S::kChunkElems)) * 16))[k % S::kChunkElems]);
-          }
-#pragma unroll
-          for (int i = 0; i < TN; ++i) {
-            const float zv = zbuf[mm * S::kZRow + 32 * i + col];
-#pragma unroll
-            for (int t = 0; t < TK; ++t) sum_w[i][t] = mfma_f32(zv, xv[t], sum_w[i][t]);
-          }
-        }
+          for (int q = 0; q < 8; ++q) t[q] = down<T>(zero ? 0.f : v[q]);
+          out8((T*)a.dx + (m0 + row) * a.k + c, t, a.k - c);
+        });
       }
       __builtin_amdgcn_wave_barrier();
     }
