@@ -185,7 +185,7 @@ int launch_stat(const Product& g, int size, const T* bias, const int64_t* target
 template <typename T>
 int launch_dz(const Product& g, int size, const EpiDz<T, 0, Kind<T>::NP>& e, hipStream_t s) {
   constexpr int NP = Kind<T>::NP;
-#define DZ(S) launch_one<T, S, false, false>(g, EpiDz<T, Tile<NP, S>::BN, NP>{e.bias, e.target, e.order, e.stat, e.scale, e.g, e.dz, e.v0, e.n, e.ld, e.plane}, s)
+#define DZ(S) launch_one<T, S, false, false>(g, EpiDz<T, Tile<NP, S>::BN, NP>{e.bias, e.target, e.order, e.stat, e.scale, e.g, e.dz, e.v0, e.n, e.ld}, s)
   return size == 2 ? DZ(2) : size == 1 ? DZ(1) : DZ(0);
 #undef DZ
 }
@@ -271,7 +271,7 @@ struct CeBwd {
     constexpr int NP = Kind<T>::NP;
     Ws ws(a->ws);
     piece = piece_of<T>(a);
-    ld = up8(piece);
+    ld = padded<T>(piece);
     pz = plan<NP>(a->rows, piece, a->k, false);
     px = plan<NP>(a->rows, a->k, piece, true);
     pw = plan<NP>(piece, a->k, a->rows, true);
@@ -301,13 +301,13 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
   const Operand x = stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, v.order, live);
   const Operand w = stage<T>(a->w, a->ldw, a->n, a->k, f.w, s);
   for (int64_t v0 = 0; v0 < a->n; v0 += f.piece) {
-    const int64_t nv = a->n - v0 < f.piece ? a->n - v0 : f.piece, ld = up8(nv);
+    const int64_t nv = a->n - v0 < f.piece ? a->n - v0 : f.piece, ld = padded<T>(nv);
     Operand wv = w;
     wv.p += v0 * w.ld;
-    const Operand dz = {(const uint16_t*)f.dz, ld, a->rows * ld};
+    const Operand dz = {(const uint16_t*)f.dz, ld * NP};
     Product gz = {x, wv, a->rows, nv, up8(a->k), live, 0, 1, 0, 0};
     int rc = launch_dz<T>(gz, f.pz.size, {a->bias ? (const T*)a->bias + v0 : nullptr, a->target, v.order, v.stat, scale,
-                                          a->reduction == CLID_REDUCE_NONE ? a->g : nullptr, (uint16_t*)f.dz, v0, nv, ld, a->rows * ld}, s);
+                                          a->reduction == CLID_REDUCE_NONE ? a->g : nullptr, (uint16_t*)f.dz, v0, nv, ld}, s);
     if (rc != CLID_OK) return rc;
     if (a->dx) {
       const bool last = v0 + nv == a->n;
@@ -326,7 +326,7 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
       if (rc != CLID_OK) return rc;
     }
     if (a->db) {
-      hipLaunchKernelGGL(k_colsum<T>, dim3((unsigned)((ld + 255) / 256), f.blocks), dim3(256), 0, s, (const uint16_t*)f.dz, a->rows, live, (int)nv, (int)ld, a->rows * ld, (float*)f.sums);
+      hipLaunchKernelGGL(k_colsum<T>, dim3((unsigned)((ld + 255) / 256), f.blocks), dim3(256), 0, s, (const uint16_t*)f.dz, a->rows, live, (int)nv, (int)ld, (float*)f.sums);
       hipLaunchKernelGGL(k_colsum_join<T>, dim3((unsigned)((nv + 63) / 64)), dim3(1024), 0, s, (const float*)f.sums, f.blocks, (int)nv, (const float*)(scale + 1), (T*)a->db + v0);
     }
   }

@@ -112,7 +112,7 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
 
 // ---- host: argument checks ----------------------------------------------------------------------------------------------
 inline bool sizes_ok(int64_t rows, int32_t k, int32_t n) {
-  return rows >= 0 && rows < (int64_t(1) << 31) && k >= 1 && n >= 1 && k < (1 << 22) && n < (1 << 22) &&
+  return rows >= 0 && rows < (int64_t(1) << 31) && k >= 1 && n >= 1 && k < (1 << 20) && n < (1 << 20) &&
          rows * (k > n ? k : n) <= (int64_t(1) << 40) && int64_t(k) * n <= (int64_t(1) << 40);
 }
 inline int64_t up256(int64_t v) { return (v + 255) & ~int64_t(255); }

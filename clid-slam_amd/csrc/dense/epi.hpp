@@ -314,7 +314,7 @@ struct EpiDz {
   const float* scale;  // [0]: what every row is multiplied by
   const float* g;      // per-row factor, by original row, or NULL
   uint16_t* dz;
-  int64_t v0, n, ld, plane;  // columns v0 .. v0 + n, ld: n up to 8 (zeros there)
+  int64_t v0, n, ld;  // columns v0 .. v0 + n; ld: n padded (zeros there)
   static constexpr bool kThroughLds = false;
   __device__ __forceinline__ void prepare(int64_t n0, char* lds) const { stage_bias(bias, n0, n, BN, lds); }
   template <int TM, int TN>
@@ -352,11 +352,11 @@ struct EpiDz {
 #pragma unroll
           for (int q = 0; q < 4; ++q) v[q] = nw + c + q < n ? v[q] : 0.f;
         }
-        put<4>(dz + m * ld + nw + c, v);
+        put<4>(dz + m * ld * NP + column<NP>(nw) + (NP == 3 ? 96 * i + 8 * j + 4 * half : c), v);
       }
     if (t >= 0 && (t >> 2 & 1) == half) {  // the target's, over what was stored for it
       const float hit[1] = {s.z * f};
-      put<1>(dz + m * ld + nw + t, hit);
+      put<1>(dz + m * ld * NP + column<NP>(nw) + (NP == 3 ? (t >> 5) * 96 + (t & 31) : t), hit);
     }
   }
   template <int N>
@@ -373,8 +373,8 @@ struct EpiDz {
       for (int q = 0; q < N; ++q) planes(v[q], h[q]);
 #pragma unroll
       for (int s3 = 0; s3 < 3; ++s3) {
-        if constexpr (N == 4) *(ushort4*)(to + s3 * plane) = ushort4{h[0][s3], h[1][s3], h[2][s3], h[3][s3]};
-        else to[s3 * plane] = h[0][s3];
+        if constexpr (N == 4) *(ushort4*)(to + s3 * 32) = ushort4{h[0][s3], h[1][s3], h[2][s3], h[3][s3]};
+        else to[s3 * 32] = h[0][s3];
       }
     }
   }

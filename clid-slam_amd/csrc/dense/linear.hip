@@ -39,7 +39,7 @@ struct Bwd {
   explicit Bwd(const clid_linear_bwd_args* a) {
     Ws ws(a->ws);
     own_dz = (a->dx || a->dw) && (a->act != CLID_ACT_NONE || !direct<T>(a->dy, a->lddy, a->n));
-    dz = ws.take(own_dz ? Kind<T>::NP * a->rows * up8(a->n) * 2 : 0);
+    dz = ws.take(own_dz ? Kind<T>::NP * a->rows * padded<T>(a->n) * 2 : 0);
     w = ws.take(a->dx ? stage_bytes<T>(a->w, a->ldw, a->n, a->k) : 0);
     x = ws.take(a->dw ? stage_bytes<T>(a->x, a->ldx, a->rows, a->k) : 0);
     blocks = row_blocks(a->rows, a->n);
@@ -55,13 +55,13 @@ struct Bwd {
 template <typename T>
 int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
   const Bwd<T> f(a);
-  const int np = (int)up8(a->n);
+  const int np = (int)padded<T>(a->n);
   const T* z = a->act == CLID_ACT_NONE ? nullptr : (const T*)a->z;
-  Operand dz = {(const uint16_t*)a->dy, a->lddy, 0};
-  if (f.own_dz) dz = {(const uint16_t*)f.dz, np, a->rows * np};
+  Operand dz = {(const uint16_t*)a->dy, a->lddy};
+  if (f.own_dz) dz = {(const uint16_t*)f.dz, np * Kind<T>::NP};
   if (f.own_dz || a->db) {
     hipLaunchKernelGGL(k_dz<T>, dim3((np + 255) / 256, f.blocks), dim3(256), 0, s, (const T*)a->dy, a->lddy, z, a->rows, a->n, a->act,
-                       f.own_dz ? (uint16_t*)f.dz : nullptr, np, a->rows * np,
+                       f.own_dz ? (uint16_t*)f.dz : nullptr, np,
                        a->db ? (float*)f.sums : nullptr);
     if (a->db)
       hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);

@@ -13,11 +13,13 @@ template <> struct Kind<bf16> { static constexpr int NP = 1; static constexpr bo
 template <> struct Kind<f16> { static constexpr int NP = 1; static constexpr bool F16 = true; using E = f16; };
 
 inline int64_t up8(int64_t v) { return (v + 7) & ~int64_t(7); }
+// columns of a copy that the tiles read: zeros up to a whole chunk, or a whole block of planes
+template <typename T> inline int64_t padded(int64_t cols) { return Kind<T>::NP == 3 ? (cols + 31) & ~int64_t(31) : up8(cols); }
 constexpr int64_t kLdMost = int64_t(1) << 22;  // a tile's offsets stay under 2^31 bytes
 
 // 8 values as the planes of T at to (aligned to 16 bytes)
 template <typename T>
-__device__ __forceinline__ void put8(uint16_t* to, int64_t plane, const float (&v)[8]) {
+__device__ __forceinline__ void put8(uint16_t* to, const float (&v)[8]) {
   if constexpr (Kind<T>::NP == 1) {
     union { uint4 w; T t[8]; } u;
 #pragma unroll
@@ -33,21 +35,21 @@ __device__ __forceinline__ void put8(uint16_t* to, int64_t plane, const float (&
       for (int s = 0; s < 3; ++s) u[s].t[q] = h[s];
     }
 #pragma unroll
-    for (int s = 0; s < 3; ++s) *(uint4*)(to + s * plane) = u[s].w;
+    for (int s = 0; s < 3; ++s) *(uint4*)(to + s * 32) = u[s].w;
   }
 }
-// rows of src (in `order`, as many as are live) -> planes with rows of kp values, zeros behind k
+// rows of src (in `order`, as many as are live) -> rows of kp values in planes, zeros behind k
 template <typename T>
-__global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t rows, int k, const int32_t* order, const int32_t* live,
-                                               uint16_t* dst, int kp, int64_t plane) {
+__global__ void __launch_bounds__(256) k_stage(const T* src, int64_t ld, int64_t rows, int k, const int32_t* order, const int32_t* live, uint16_t* dst, int kp) {
   if (live) rows = *live < rows ? *live : rows;
+  constexpr int NP = Kind<T>::NP;
   const int per = kp / 8;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / per;
     const int c = (int)(i - r * per) * 8;
     float v[8];
     get8(src + (order ? (int64_t)order[r] : r) * ld + c, v, k - c < 8 ? k - c : 8);
-    put8<T>(dst + r * kp + c, plane, v);
+    put8<T>(dst + r * kp * NP + column<NP>(c), v);
   }
 }
 
@@ -63,22 +65,21 @@ inline bool direct(const void* p, int64_t ld, int k) {
 }
 template <typename T>
 inline int64_t stage_bytes(const void* p, int64_t ld, int64_t rows, int k, bool always = false) {
-  return direct<T>(p, ld, k) && !always ? 0 : up256(Kind<T>::NP * rows * up8(k) * 2);
+  return direct<T>(p, ld, k) && !always ? 0 : up256(Kind<T>::NP * rows * padded<T>(k) * 2);
 }
 template <typename T>
 inline Operand stage(const void* p, int64_t ld, int64_t rows, int k, char* ws, hipStream_t s, bool always = false, const int32_t* order = nullptr,
                      const int32_t* live = nullptr) {
-  if (direct<T>(p, ld, k) && !always) return {(const uint16_t*)p, ld, 0};
-  const int64_t kp = up8(k);
-  hipLaunchKernelGGL(k_stage<T>, grid_for(rows * kp / 8), dim3(256), 0, s, (const T*)p, ld, rows, k, order, live, (uint16_t*)ws, (int)kp, rows * kp);
-  return {(const uint16_t*)ws, kp, rows * kp};
+  if (direct<T>(p, ld, k) && !always) return {(const uint16_t*)p, ld};
+  const int64_t kp = padded<T>(k);
+  hipLaunchKernelGGL(k_stage<T>, grid_for(rows * kp / 8), dim3(256), 0, s, (const T*)p, ld, rows, k, order, live, (uint16_t*)ws, (int)kp);
+  return {(const uint16_t*)ws, kp * Kind<T>::NP};
 }
 
 // dz = dy act'(z) -> planes with rows of np values (dst may be NULL: the sums alone), and its column sums over blocks of rows ->
 // part[row block][n].  A block takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows.
 template <typename T>
-__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* z, int64_t rows, int n, int act, uint16_t* dst, int np,
-                                            int64_t plane, float* part) {
+__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* z, int64_t rows, int n, int act, uint16_t* dst, int np, float* part) {
   __shared__ float sums[8][256 + 8];
   const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8, count = n - c < 8 ? n - c : 8;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
@@ -102,7 +103,7 @@ __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* 
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q) sum[q] += v[t][q];
-        if (dst) put8<T>(dst + (m + t * step) * np + c, plane, v[t]);
+        if (dst) put8<T>(dst + (m + t * step) * np * Kind<T>::NP + column<Kind<T>::NP>(c), v[t]);
       }
     }
   }
@@ -120,7 +121,7 @@ __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* 
 }
 // column sums of planes, as k_dz's
 template <typename T>
-__global__ void __launch_bounds__(256) k_colsum(const uint16_t* src, int64_t rows, const int32_t* live, int n, int np, int64_t plane, float* part) {
+__global__ void __launch_bounds__(256) k_colsum(const uint16_t* src, int64_t rows, const int32_t* live, int n, int np, float* part) {
   __shared__ float sums[8][256 + 8];
   if (live) rows = *live < rows ? *live : rows;
   const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8;
@@ -131,7 +132,7 @@ __global__ void __launch_bounds__(256) k_colsum(const uint16_t* src, int64_t row
 #pragma unroll
       for (int s = Kind<T>::NP - 1; s >= 0; --s) {
         union { uint4 w; typename Kind<T>::E t[8]; } u;
-        u.w = *(const uint4*)(src + s * plane + m * np + c);
+        u.w = *(const uint4*)(src + m * np * Kind<T>::NP + column<Kind<T>::NP>(c) + s * 32);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] += up(u.t[q]);
       }

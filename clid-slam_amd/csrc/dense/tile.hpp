@@ -3,7 +3,8 @@
 // Operands.  P and Q lie in memory either with k contiguous (rows of a layer's input, a weight) or with k as the row (KS: the
 // same matrices seen from the gradients' products); both go through LDS as they lie, and the fragments of a KS operand are
 // turned on the way out of LDS (ds_read_b64_tr_b16), so no transposed copy is ever made.
-// fp32 operands come as NP = 3 bf16 planes, hi + mid + lo = v exactly (8 bits each, by truncation): six plane products
+// fp32 operands come as NP = 3 bf16 planes, hi + mid + lo = v exactly (8 bits each, by truncation), 32 columns' hi, their mid, their lo in
+// turn, so that a row's copy to LDS is 192 neighbouring bytes and not three times 64 (half a cache line each): six plane products
 // (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave out less than 2^-22 of |p q| and run at the bf16 rate, 2.5 PFLOP/s / 6 =
 // 417 TFLOP/s against 157 of the fp32 matrix instructions.  Infinities behave: planes() below.
 //
@@ -32,10 +33,13 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 
 struct Operand {
-  const uint16_t* p;  // plane 0
-  int64_t ld;         // elements between rows
-  int64_t plane;      // elements between planes
+  const uint16_t* p;
+  int64_t ld;  // elements between rows, the planes' included
 };
+
+// where column c (a multiple of 8) of a row begins, in elements; plane s is 32 s behind it
+template <int NP>
+__host__ __device__ __forceinline__ int64_t column(int64_t c) { return NP == 3 ? (c >> 5) * 96 + (c & 31) : c; }
 
 struct Product {
   Operand p, q;
@@ -87,75 +91,66 @@ __device__ __forceinline__ s16x4 turned(const char* __restrict__ at) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
 }
 
-// R rows (m or n) x BK of one operand in LDS, NP planes
+// R rows (m or n) x BK of one operand in LDS, all planes
 template <int R, int BK, int NP, bool KS, int WAVES>
 struct Side {
-  static constexpr int kBytes = R * BK * 2;                  // of a plane
-  static constexpr int kLoads = (kBytes / 1024 + WAVES - 1) / WAVES;  // 16-byte loads per lane and plane: all waves issue as many ...
-  static constexpr bool kWhole = kBytes % (1024 * WAVES) == 0;        // ... some of them, where this is false, of nothing into LDS that nobody reads
-  static constexpr int kChunks = KS ? R / 8 : BK / 8;        // 16-byte chunks of an LDS row
-  static_assert(kBytes % 1024 == 0, "whole loads of a wave");
+  static_assert(NP == 1 || BK == 32, "a step of fp32 is a block of planes");
+  static constexpr int kBytes = R * BK * 2 * NP;
+  static constexpr int kLoads = kBytes / 1024 / WAVES;        // 16-byte loads per lane
+  static constexpr int kChunks = (KS ? R : BK) * NP / 8;      // 16-byte chunks of an LDS row
+  static_assert(kBytes % (1024 * WAVES) == 0, "whole loads");
 
-  // where chunk c of LDS row `row` lies
+  // Where chunk c of LDS row `row` lies.  Reads are free of bank conflicts where 16 lanes hit all of 256 bytes once: one chunk of 16
+  // rows, or (KS) 64 bytes of four rows.
   static __device__ __forceinline__ int place(int row, int c) {
     if constexpr (KS) {
-      // a fragment read takes 64 bytes of rows k .. k + 3 and k + 8 .. k + 11
+      if constexpr (NP == 3) return c ^ ((R == 64 ? row >> 1 & 1 : row & 3) << 2);
       if constexpr (kChunks >= 32) return c ^ ((((row >> 1) & 4) | (row & 3)) << 2);
       if constexpr (kChunks == 16) return c ^ ((row & 3) << 2);
       return c ^ (((row >> 1) & 1) << 2);
     } else {
-      // 16 lanes read together, one chunk of 16 rows: 256 bytes, every bank once
+      if constexpr (NP == 3) return c ^ ((row >> 2) & 3);  // 12 chunks a row: four rows go round the banks three times
       return c ^ ((row / (16 / kChunks)) & (kChunks - 1));
     }
   }
 
-  uint32_t at[kLoads];  // byte offset of this lane's loads within the tile of plane 0
+  uint32_t at[kLoads];  // byte offset of this lane's loads within the tile
 
   // first: the tile's first row (m or n); rows: how many there are
   __device__ __forceinline__ void init(const Operand& o, int64_t first, int64_t rows, int wave, int lane) {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
-      if (!kWhole && c * 16 >= kBytes) {
-        at[i] = kOutside;
-      } else if constexpr (KS) {
-        at[i] = first + chunk * 8 < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
-      } else {
-        at[i] = first + row < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
-      }
+      const int64_t of = KS ? (NP == 3 ? chunk / 12 * 32 : chunk * 8) : row;  // the row of m or n that it belongs to
+      at[i] = first + of < rows ? uint32_t(row) * uint32_t(o.ld * 2) + chunk * 16 : kOutside;
     }
   }
 
-  // copies the tile at k0 .. k0 + BK of plane s to LDS, all of it below k: nothing to check but at[]
-  __device__ __forceinline__ void load(const uint16_t* base, int s, char* lds, char* nowhere, int wave) const {
+  // copies a step of the tile to LDS, all of it below k: nothing to check but at[]
+  __device__ __forceinline__ void load(const uint16_t* base, char* lds, int wave) const {
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) copy16(base, 0x7fffffffu, at[i], place_of(i, s, lds, nowhere, wave));
+    for (int i = 0; i < kLoads; ++i) copy16(base, 0x7fffffffu, at[i], lds + (i * WAVES + wave) * 1024);
   }
   // the last step of a share that is no multiple of BK: rows (or chunks) from k on are zeros
-  __device__ __forceinline__ void load_last(const uint16_t* base, int s, char* lds, char* nowhere, int wave, int lane, int left) const {
+  __device__ __forceinline__ void load_last(const uint16_t* base, char* lds, int wave, int lane, int left) const {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
       const int c = (i * WAVES + wave) * 64 + lane, row = c / kChunks, chunk = place(row, c % kChunks);
-      copy16(base, 0x7fffffffu, (KS ? row : chunk * 8) < left ? at[i] : kOutside, place_of(i, s, lds, nowhere, wave));
+      copy16(base, 0x7fffffffu, (KS ? row : (NP == 3 ? chunk % 4 : chunk) * 8) < left ? at[i] : kOutside, lds + (i * WAVES + wave) * 1024);
     }
   }
-  static __device__ __forceinline__ char* place_of(int i, int s, char* lds, char* nowhere, int wave) {
-    const int at = (i * WAVES + wave) * 1024;
-    return kWhole || at < kBytes ? lds + s * kBytes + at : nowhere;
-  }
 
-  // this lane's 8 values of k (16 kk + 8 (lane / 32) ..) of row 32 t + lane % 32
+  // this lane's 8 values of k (16 kk + 8 (lane / 32) ..) of row 32 t + lane % 32, plane s
   static __device__ __forceinline__ s16x8 fragment(const char* lds, int s, int first, int kk, int lane) {
     if constexpr (!KS) {
-      const int row = first + (lane & 31), c = 2 * kk + (lane >> 5);
-      return *(const s16x8*)(lds + s * kBytes + (row * kChunks + place(row, c)) * 16);
+      const int row = first + (lane & 31), c = s * 4 + 2 * kk + (lane >> 5);
+      return *(const s16x8*)(lds + (row * kChunks + place(row, c)) * 16);
     } else {
       // 16 lanes together read 4 rows (k) of 16 columns; lane i of them gets column i of the four rows
       const int i = lane & 15, k = 16 * kk + 8 * (lane >> 5) + (i >> 2), col = first + ((lane >> 4) & 1) * 16 + (i & 3) * 4;
-      const char* at0 = lds + s * kBytes + (k * kChunks + place(k, col >> 3)) * 16 + (col & 4) * 2;
-      const char* at1 = lds + s * kBytes + ((k + 4) * kChunks + place(k + 4, col >> 3)) * 16 + (col & 4) * 2;
-      const s16x4 a = turned(at0);
-      const s16x4 b = turned(at1);
+      const int c = NP == 3 ? (first >> 5) * 12 + s * 4 + ((col & 31) >> 3) : col >> 3;
+      const s16x4 a = turned(lds + (k * kChunks + place(k, c)) * 16 + (col & 4) * 2);
+      const s16x4 b = turned(lds + ((k + 4) * kChunks + place(k + 4, c)) * 16 + (col & 4) * 2);
       return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
     }
   }
@@ -168,8 +163,7 @@ template <int TM, int TN> constexpr int kRowsLds = (TM > 1 ? 64 : 32) * (32 * TN
 // LDS in front of the bias: the stages, later the waves' rows
 template <int NP, int BM, int BN, int BK, int WM, int WN, int STAGES>
 constexpr int tile_lds() {
-  const bool whole = BM * BK * 2 % (1024 * WM * WN) == 0 && BN * BK * 2 % (1024 * WM * WN) == 0;
-  const int stages = STAGES * NP * (BM + BN) * BK * 2 + (whole ? 0 : 1024), rows = WM * WN * kRowsLds<BM / WM / 32, BN / WN / 32>;
+  const int stages = STAGES * NP * (BM + BN) * BK * 2, rows = WM * WN * kRowsLds<BM / WM / 32, BN / WN / 32>;
   return stages > rows ? stages : rows;
 }
 
@@ -190,8 +184,8 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   using SideP = Side<BM, BK, NP, PKS, WAVES>;
   using SideQ = Side<BN, BK, NP, QKS, WAVES>;
-  constexpr int kStage = NP * (SideP::kBytes + SideQ::kBytes);
-  constexpr int kNowhere = STAGES * kStage, kBias = tile_lds<NP, BM, BN, BK, WM, WN, STAGES>();
+  constexpr int kStage = SideP::kBytes + SideQ::kBytes;
+  constexpr int kBias = tile_lds<NP, BM, BN, BK, WM, WN, STAGES>();
   extern __shared__ __align__(16) char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int wm = wave / WN, wn = wave % WN;
@@ -210,8 +204,9 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   const int first = split * per, steps = first + per < steps_all ? per : steps_all > first ? steps_all - first : 0;
   const int last = (int)(rows_k - (int64_t)(first + steps - 1) * BK < BK ? rows_k - (int64_t)(first + steps - 1) * BK : BK);  // values of the last step
 
-  // rows of a KS operand are as long as its matrix, padded to 8
-  const int64_t lim_m = PKS ? (rows_m + 7) / 8 * 8 : rows_m, lim_n = QKS ? (g.n + 7) / 8 * 8 : g.n;
+  // rows of a KS operand are as long as its matrix, padded
+  constexpr int64_t kPad = NP == 3 ? 31 : 7;
+  const int64_t lim_m = PKS ? (rows_m + kPad) & ~kPad : rows_m, lim_n = QKS ? (g.n + kPad) & ~kPad : g.n;
   SideP sp;
   SideQ sq;
   sp.init(g.p, m0, lim_m, wave, lane);
@@ -224,25 +219,19 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
 
-  constexpr int kLoads = NP * (SideP::kLoads + SideQ::kLoads);  // of a lane and step
-  const int64_t p_step = (PKS ? BK * g.p.ld : BK), q_step = (QKS ? BK * g.q.ld : BK);
-  const uint16_t* p_at = g.p.p + (PKS ? m0 : m0 * g.p.ld) + first * p_step;
-  const uint16_t* q_at = g.q.p + (QKS ? n0 : n0 * g.q.ld) + first * q_step;
+  constexpr int kLoads = SideP::kLoads + SideQ::kLoads;  // of a lane and step
+  const int64_t p_step = PKS ? BK * g.p.ld : BK * NP, q_step = QKS ? BK * g.q.ld : BK * NP;
+  const uint16_t* p_at = g.p.p + (PKS ? column<NP>(m0) : m0 * g.p.ld) + first * p_step;
+  const uint16_t* q_at = g.q.p + (QKS ? column<NP>(n0) : n0 * g.q.ld) + first * q_step;
   int loaded = 0;
   auto load = [&]() {  // the next step's
     char* buf = lds + loaded % STAGES * kStage;
     if (loaded + 1 < steps || last == BK) {
-#pragma unroll
-      for (int s = 0; s < NP; ++s) {
-        sp.load(p_at + s * g.p.plane, s, buf, lds + kNowhere, wave);
-        sq.load(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, lds + kNowhere, wave);
-      }
+      sp.load(p_at, buf, wave);
+      sq.load(q_at, buf + SideP::kBytes, wave);
     } else {
-#pragma unroll
-      for (int s = 0; s < NP; ++s) {
-        sp.load_last(p_at + s * g.p.plane, s, buf, lds + kNowhere, wave, lane, last);
-        sq.load_last(q_at + s * g.q.plane, s, buf + NP * SideP::kBytes, lds + kNowhere, wave, lane, last);
-      }
+      sp.load_last(p_at, buf, wave, lane, last);
+      sq.load_last(q_at, buf + SideP::kBytes, wave, lane, last);
     }
     ++loaded;
     p_at += p_step;
@@ -257,7 +246,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
 #pragma unroll
       for (int j = 0; j < TM; ++j) f.p[s][j] = SideP::fragment(buf, s, (wm * TM + j) * 32, kk, lane);
 #pragma unroll
-      for (int i = 0; i < TN; ++i) f.q[s][i] = SideQ::fragment(buf + NP * SideP::kBytes, s, (wn * TN + i) * 32, kk, lane);
+      for (int i = 0; i < TN; ++i) f.q[s][i] = SideQ::fragment(buf + SideP::kBytes, s, (wn * TN + i) * 32, kk, lane);
     }
   };
   auto multiply = [&](const Frags& f) {

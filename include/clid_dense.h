@@ -11,7 +11,7 @@
  *   - dtype (CLID_F32 / CLID_BF16 / CLID_F16) is that of x, w, bias, residual, y and of the gradients; sums, softmax statistics,
  *     losses and log-probabilities are fp32;
  *   - `ws` has at least clid_*_workspace() bytes, 256-byte aligned, and holds nothing between calls;
- *   - rows >= 0, k >= 1, n >= 1, each matrix at most 2^40 elements; rows < 2^31, k, n < 2^22.
+ *   - rows >= 0, k >= 1, n >= 1, each matrix at most 2^40 elements; rows < 2^31, k, n < 2^20.
  */
 #ifndef CLID_DENSE_H
 #define CLID_DENSE_H

@@ -52,6 +52,14 @@ def test_entry_points_refuse_bad_arguments():
         a = make(rows=1 << 31, k=8, n=4)
         assert getattr(lib, fn)(C.byref(a), None) == -1
         assert getattr(lib, fn)(None, None) == -1
+    # a workspace that is too small, or not aligned as the header asks (never launched: the addresses are no memory)
+    a = L.CeArgs(x=4096, w=4096, target=4096, saved=4096, loss_out=4096, ldx=100, ldw=100, rows=4, k=100, n=100, reduction=1)
+    need = lib.clid_ce_workspace(C.byref(a))
+    assert need > 0 and need % 256 == 0
+    for a.ws, a.ws_bytes in ((4096, need - 1), (4097, need), (None, need)):
+        assert lib.clid_ce_fwd(C.byref(a), None) == -1 and b"workspace" in lib.clid_last_error()
+    a.saved = 4097
+    assert lib.clid_ce_fwd(C.byref(a), None) == -1
     for fn in ("clid_linear_workspace", "clid_linear_bwd_workspace", "clid_ce_workspace", "clid_ce_bwd_workspace", "clid_label_workspace"):
         assert getattr(lib, fn)(None) < 0
 
@@ -181,6 +189,95 @@ def test_label(shape, dtype):
 
 def gamma_of(n):
     return ref.gamma(n)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(4096, 264, 4100), (333, 8200, 260), (260, 72, 20011), (4099, 1000, 40)], ids=str)
+def test_large_tiles_and_cuts(shape, dtype):
+    """Sizes that take the larger tiles, and k cut into parts."""
+    m, k, n = shape
+    dt = TYPES[dtype]
+    gen = generator(m + n)
+    x, w, b = (normal(gen, m, k).to(dt).requires_grad_(), (normal(gen, n, k) * k ** -0.5).to(dt).requires_grad_(), normal(gen, n).to(dt).requires_grad_())
+    r, dy, t = normal(gen, m, n).to(dt), normal(gen, m, n).to(dt), torch.randint(0, n, (m,), generator=gen, device="cuda")
+    t[::3] = -100
+    y = linear_act(x, w, b, activation="gelu", residual=r)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, [x, w, b], dy))) | {"y": y}
+    for name, (v, tol) in ref.linear(x, w, b, r, "gelu", dy).items():
+        ref.close(got[name], v, tol, name)
+    g = torch.full((), 256.0, device="cuda")
+    loss = linear_cross_entropy(x, w, b, t)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(loss, [x, w, b], g))) | {"loss": loss}
+    for name, (v, tol) in ref.cross_entropy(x, w, b, t, -100, "mean", g).items():
+        ref.close(got[name], v, tol, "cross entropy " + name)
+    label, _ = linear_label(x, w, b)
+    _, _, z, ez = ref.logits(x, w, b)
+    top = z.topk(2, dim=1)
+    clear = top.values[:, 0] - top.values[:, 1] > 2 * ez.amax(1)
+    # (how many rows are clear says nothing about the kernel, only that the comparison is not empty: two largest of normal logits are
+    # about 0.3 apart, and 2 ez reaches 0.06 at k = 8200)
+    assert torch.equal(label[clear], top.indices[clear, 0]) and clear.float().mean() > 0.5
+
+
+@gpu
+@pytest.mark.parametrize("dtype,m", [("bf16", 8192), ("f16", 7000), ("f32", 4096)])
+def test_cross_entropy_in_several_pieces(dtype, m):
+    """A backward pass whose dz takes more than one piece of the classes (512 MB of it)."""
+    k, n, dt, gen = 24, 40003, TYPES[dtype], generator(17)
+    x, w, b = (normal(gen, m, k).to(dt).requires_grad_(), (normal(gen, n, k) * k ** -0.5).to(dt).requires_grad_(), normal(gen, n).to(dt).requires_grad_())
+    t = torch.randint(0, n, (m,), generator=gen, device="cuda")
+    g = normal(gen, m).abs()
+    loss = linear_cross_entropy(x, w, b, t, reduction="none")
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(loss, [x, w, b], g))) | {"loss": loss}
+    for name, (v, tol) in ref.cross_entropy(x, w, b, t, -100, "none", g).items():
+        ref.close(got[name], v, tol, name)
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(5, 8, 9), (5, 100, 70), (200, 100, 70)], ids=str)
+def test_infinities_stay_infinities(shape):
+    """What a plain product gives: an infinity in x times a weight's sign, NaN where it meets a zero, nothing in the other rows."""
+    m, k, n = shape
+    for dt in TYPES.values():
+        gen = generator(m)
+        x, w = normal(gen, m, k).to(dt), normal(gen, n, k).to(dt)
+        w[:, 3] = 1.0
+        w[0, 3] = 0.0
+        w[1, 3] = -0.5
+        x[1, 3], x[2, 3], x[4, 3] = float("inf"), -float("inf"), float("nan")
+        y = linear_act(x, w)
+        want = x.double() @ w.double().t()
+        assert torch.equal(torch.isnan(y), torch.isnan(want)) and torch.equal(torch.isinf(y), torch.isinf(want))
+        odd = torch.isinf(want)
+        assert torch.equal(y[odd].double(), want[odd])
+
+
+@gpu
+def test_calls_from_two_threads():
+    import threading
+
+    gen = generator(8)
+    x, w, t = normal(gen, 700, 96), normal(gen, 130, 96), torch.randint(0, 130, (700,), generator=gen, device="cuda")
+    want = [linear_act(x, w, activation="gelu"), linear_cross_entropy(x, w, None, t), *linear_label(x, w)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = [linear_act(x, w, activation="gelu"), linear_cross_entropy(x, w, None, t), *linear_label(x, w)]
+                s.synchronize()
+                if not all(torch.equal(a, q) for a, q in zip(got, want)):
+                    wrong.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not wrong
 
 
 @gpu
