@@ -6,7 +6,7 @@
 // fp32 operands come as NP = 3 bf16 planes, hi + mid + lo = v exactly (8 bits each, by truncation), 32 columns' hi, their mid, their lo in
 // turn, so that a row's copy to LDS is 192 neighbouring bytes and not three times 64 (half a cache line each): six plane products
 // (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave out less than 2^-22 of |p q| and run at the bf16 rate, 2.5 PFLOP/s / 6 =
-// 417 TFLOP/s against 157 of the fp32 matrix instructions.  Infinities behave: planes() below.
+// 417 TFLOP/s against 157 of the fp32 matrix instructions.
 //
 // Tiles.  One block computes BM x BN with WM x WN waves, each 32 x 32 x 16 instructions on a (BM / WM) x (BN / WN) part.  Per step
 // of BK along k the block copies both tiles from memory straight to LDS (16 bytes a lane, buffer loads whose bounds check turns
@@ -66,22 +66,20 @@ __device__ __forceinline__ void copy16(const void* base, uint32_t bound, uint32_
   __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (__attribute__((address_space(3))) void*)lds, 16, offset, 0, 0, 0);
 }
 
-// v as three bf16 planes.  Each is the one before's remainder cut to 8 bits, so they have v's sign and their sum is v.  A plane that
-// comes out as 0 is 2^-126 with v's sign instead, and an infinity's planes are all infinite: then an infinity in the other operand
-// meets no zero that is not a zero of the matrix, and all six products have the sign of the one that they stand for.
+// v as three bf16 planes, each the one before's remainder cut to 8 bits: their sum is v.  An infinity or a NaN has it all in the first, whose
+// products have sums of their own (k_tile); a value under 2^-133 keeps at least its sign there.
 __device__ __forceinline__ void planes(float v, uint16_t (&h)[3]) {
-  const uint32_t b = __float_as_uint(v), sign = b & 0x80000000u;
-  if ((b & 0x7f800000u) == 0x7f800000u || (b & 0x7fffffffu) == 0) {
-    h[0] = h[1] = h[2] = (uint16_t)((b >> 16) | ((b & 0xffffu) ? 1 : 0));  // inf, 0, or a NaN that stays one
+  const uint32_t b = __float_as_uint(v);
+  if ((b & 0x7f800000u) == 0x7f800000u) {
+    h[0] = (uint16_t)((b >> 16) | ((b & 0x7fffffu) ? 0x40 : 0));
+    h[1] = h[2] = 0;
     return;
   }
   const float r1 = v - __uint_as_float(b & 0xffff0000u);
   const uint32_t b1 = __float_as_uint(r1) & 0xffff0000u;
-  const uint32_t b2 = __float_as_uint(r1 - __uint_as_float(b1)) & 0xffff0000u;
-  const uint16_t tiny = (uint16_t)((sign | 0x00800000u) >> 16);
-  h[0] = (b >> 16) & 0x7fff ? (uint16_t)(b >> 16) : tiny;
-  h[1] = b1 & 0x7fffffffu ? (uint16_t)(b1 >> 16) : tiny;
-  h[2] = b2 & 0x7fffffffu ? (uint16_t)(b2 >> 16) : tiny;
+  h[0] = (uint16_t)((b >> 16) | ((b & 0x7fff0000u) == 0 && (b & 0xffffu) ? 1 : 0));
+  h[1] = (uint16_t)(b1 >> 16);
+  h[2] = (uint16_t)(__float_as_uint(r1 - __uint_as_float(b1)) >> 16);
 }
 
 // 4 rows of 16 columns turned: lane i of 16 gives the address of 4 columns of row i / 4 and gets column i of the four rows.  (__restrict__
@@ -211,13 +209,17 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   SideQ sq;
   sp.init(g.p, m0, lim_m, wave, lane);
   sq.init(g.q, n0, lim_n, wave, lane);
-  f32x16 acc[TM][TN];
+  // fp32: hi hi has sums of its own, and the five smaller products theirs, 2^-8 of it: one rounding of the large sum a step and not six
+  f32x16 acc[TM][TN], small[NP == 3 ? TM : 1][NP == 3 ? TN : 1];
 #pragma unroll
   for (int j = 0; j < TM; ++j)
 #pragma unroll
     for (int i = 0; i < TN; ++i)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[j][i][r] = 0.f;
+      for (int r = 0; r < 16; ++r) {
+        acc[j][i][r] = 0.f;
+        if constexpr (NP == 3) small[j][i][r] = 0.f;
+      }
 
   constexpr int kLoads = SideP::kLoads + SideQ::kLoads;  // of a lane and step
   const int64_t p_step = PKS ? BK * g.p.ld : BK * NP, q_step = QKS ? BK * g.q.ld : BK * NP;
@@ -250,14 +252,19 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
     }
   };
   auto multiply = [&](const Frags& f) {
-    constexpr int kPairs = NP == 3 ? 6 : 1;
-    constexpr int kP[6] = {0, 2, 1, 0, 1, 0}, kQ[6] = {2, 0, 1, 1, 0, 0};  // the small products first
+    if constexpr (NP == 3) {
+      constexpr int kP[5] = {0, 2, 1, 0, 1}, kQ[5] = {2, 0, 1, 1, 0};
 #pragma unroll
-    for (int t = 0; t < kPairs; ++t)
+      for (int t = 0; t < 5; ++t)
 #pragma unroll
-      for (int j = 0; j < TM; ++j)
+        for (int j = 0; j < TM; ++j)
 #pragma unroll
-        for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(f.q[NP == 1 ? 0 : kQ[t]][i], f.p[NP == 1 ? 0 : kP[t]][j], acc[j][i]);
+          for (int i = 0; i < TN; ++i) small[j][i] = mfma<F16>(f.q[kQ[t]][i], f.p[kP[t]][j], small[j][i]);
+    }
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int i = 0; i < TN; ++i) acc[j][i] = mfma<F16>(f.q[0][i], f.p[0][j], acc[j][i]);
   };
   // Step s + 1 is there for this wave when nothing but the loads of the steps behind it is under way, and for every wave behind the barrier,
   // where also nobody reads step s any more: its part of LDS is the next load's.
@@ -271,6 +278,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   // product of step s to do while the first fragments of step s + 1 come.
   constexpr int KK = BK / 16;
   constexpr bool kAcross = STAGES >= 3;  // (two stages: the copy is too late for that)
+  constexpr bool kTwo = !(NP == 3 && !kAcross);  // (fp32's large tile has no registers for two: 14 of them would be spilled)
   Frags f[2];
   auto step = [&](int s, auto parity) {
     constexpr int kFirst = decltype(parity)::value;
@@ -278,6 +286,15 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
     if constexpr (!kAcross) {
       arrive(false);
       read(buf, 0, f[kFirst]);
+    }
+    if constexpr (!kTwo) {
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        if (kk) read(buf, kk, f[0]);
+        if (kk == 0 && s + STAGES - 1 < steps) load();
+        multiply(f[0]);
+      }
+      return;
     }
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -310,6 +327,18 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
         if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
       }
     }
+  }
+  if constexpr (NP == 3) {
+#pragma unroll
+    for (int j = 0; j < TM; ++j)
+#pragma unroll
+      for (int i = 0; i < TN; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          // an infinity times another operand's plane that is zero made a NaN of the small sum only
+          const float v = acc[j][i][r];
+          acc[j][i][r] = fabsf(v) <= 3.4028235e38f ? v + small[j][i][r] : v;
+        }
   }
   if (Epi::kThroughLds || steps == 0) __syncthreads();  // LDS is the epilogue's; what prepare() left there is seen
 
