@@ -371,6 +371,7 @@ extern "C" int64_t clid_ce_saved(const clid_ce_args* a) {
 extern "C" int64_t clid_ce_workspace(const clid_ce_args* a) {
   if (!ce_ok(a)) return bad("clid_ce_workspace", "bad argument");
   if (is_narrow(a->k, a->n) && a->rows) return narrow_ce_bytes(a);
+  if (is_few(a->rows) && a->rows) return few_ce_bytes(a);
   BY_DTYPE(a->dtype, return CeFwd<T>(a).bytes;);
 }
 extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
@@ -383,6 +384,7 @@ extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
   if (a->rows && !ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n) && a->rows) rc = narrow_ce(a, (hipStream_t)stream);
+  else if (is_few(a->rows) && a->rows) rc = few_ce(a, Saved(a).stat, Saved(a).total, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = ce_fwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);
@@ -391,6 +393,7 @@ extern "C" int clid_ce_fwd(const clid_ce_args* a, void* stream) {
 extern "C" int64_t clid_ce_bwd_workspace(const clid_ce_args* a) {
   if (!ce_ok(a)) return bad("clid_ce_bwd_workspace", "bad argument");
   if (is_narrow(a->k, a->n)) return narrow_ce_bwd_bytes(a);
+  if (is_few(a->rows)) return few_ce_bwd_bytes(a);
   BY_DTYPE(a->dtype, return CeBwd<T>(a).bytes;);
 }
 extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
@@ -402,6 +405,7 @@ extern "C" int clid_ce_bwd(const clid_ce_args* a, void* stream) {
   if (!ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_ce_bwd(a, (hipStream_t)stream);
+  else if (is_few(a->rows)) rc = few_ce_bwd(a, Saved(a).stat, Saved(a).total, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = ce_bwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);

@@ -4,6 +4,9 @@
 // w goes from memory to the matrix instruction's registers directly: lane l of a wave holds 16 bytes of row l % 16 of a tile, 4 lanes 64
 // neighbouring bytes of it, and the same of x as the column operand (32 k of 16 bits: 16 x 16 x 32; 16 k of fp32: four 16 x 16 x 4, exact
 // fp32).  No LDS in the loop, four steps of loads in flight.  A block's waves share the tile's k; their sums meet in LDS in their order.
+// The cross entropy's backward pass makes z again the same way, leaves dz in fp32 (32 rows of it are small) and takes both products on the fp32
+// matrix instruction (16 x 16 x 4), w and dw in 16 bytes a lane of 256 neighbouring ones: with few rows nothing averages a rounding of
+// dz away, and the products cost nothing beside the weight's bytes.
 // Where n is large a wave takes 4 tiles at once (one read of x for four of w) and a block goes through many, keeping running softmax
 // statistics, so that a head of 131072 classes leaves one partial result per block.
 #include "stage.hpp"
@@ -54,11 +57,11 @@ __device__ __forceinline__ void few_tile(const Few& a, int64_t n0, int k_from, i
   for (int j = 0; j < MT; ++j) x[j] = (const T*)a.x + (j * 16 + row < a.m ? j * 16 + row : a.m - 1) * a.ldx + kk;  // rows that are not there: the last one's
 #pragma unroll
   for (int i = 0; i < NT; ++i) w[i] = (const T*)a.w + (n0 + i * 16 + row < a.n ? n0 + i * 16 + row : a.n - 1) * a.ldw + kk;
-  f32x4 acc[NT][MT];
+  f32x4 acc[2][NT][MT];  // every other step's: half as many roundings in a row
 #pragma unroll
   for (int i = 0; i < NT; ++i)
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < MT; ++j) acc[0][i][j] = acc[1][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
   int k = k_from;
   constexpr int kDeep = NT == 1 ? 8 : 4;
   for (; k + kDeep * F::kStep <= k_to; k += kDeep * F::kStep) {
@@ -75,7 +78,7 @@ __device__ __forceinline__ void few_tile(const Few& a, int64_t n0, int k_from, i
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = mfma16(fw[u][i], fx[u][j], acc[i][j]);
+        for (int j = 0; j < MT; ++j) acc[u & 1][i][j] = mfma16(fw[u][i], fx[u][j], acc[u & 1][i][j]);
   }
   for (; k < k_to; k += F::kStep) {
     F fw[NT], fx[MT];
@@ -93,7 +96,7 @@ __device__ __forceinline__ void few_tile(const Few& a, int64_t n0, int k_from, i
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) acc[i][j] = mfma16(fw[i], fx[j], acc[i][j]);
+      for (int j = 0; j < MT; ++j) acc[0][i][j] = mfma16(fw[i], fx[j], acc[0][i][j]);
   }
   // lane: column m = lane % 16, rows 4 (lane / 16) ..
 #pragma unroll
@@ -101,7 +104,7 @@ __device__ __forceinline__ void few_tile(const Few& a, int64_t n0, int k_from, i
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) lds[(j * 16 * NT + i * 16 + 4 * (lane >> 4) + r) * kFewRow + row] = acc[i][j][r];
+      for (int r = 0; r < 4; ++r) lds[(j * 16 * NT + i * 16 + 4 * (lane >> 4) + r) * kFewRow + row] = acc[0][i][j][r] + acc[1][i][j][r];
 }
 // wave's share of k, in whole steps
 template <typename T>
@@ -132,9 +135,9 @@ __global__ void __launch_bounds__(NT == 1 ? 1024 : 256) k_few_linear(Few a, Line
   }
 }
 
-// part[block][m]: running statistics of the block's columns
+// part[block][m]: running statistics of the block's columns; zt[m]: the target's z, where there are targets
 template <typename T, int MT, int NT>
-__global__ void __launch_bounds__(256) k_few_label(Few a, const T* bias, Stat* part) {
+__global__ void __launch_bounds__(256) k_few_stat(Few a, const T* bias, const int64_t* target, float* zt, Stat* part) {
   extern __shared__ __align__(16) char lds[];
   constexpr int kTile = MT * NT * 16 * kFewRow, kEach = 16 / MT;  // 256 threads: 16 MT rows, kEach threads each
   float* sums = (float*)lds;
@@ -143,7 +146,7 @@ __global__ void __launch_bounds__(256) k_few_label(Few a, const T* bias, Stat* p
   few_share<T>(a, wave, 4, &from, &to);
   const int m = threadIdx.x / kEach, sub = threadIdx.x % kEach;
   Stat s = {neg_inf(), 0.f, 0x7fffffff};
-  const int64_t tiles = (a.n + 16 * NT - 1) / (16 * NT);
+  const int64_t tiles = (a.n + 16 * NT - 1) / (16 * NT), t = target && m < a.m ? target[m] : -1;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
     few_tile<T, MT, NT>(a, tile * 16 * NT, from, to, threadIdx.x & 63, sums + wave * kTile);
     __syncthreads();
@@ -154,6 +157,7 @@ __global__ void __launch_bounds__(256) k_few_label(Few a, const T* bias, Stat* p
         const int at = ((m >> 4) * 16 * NT + n) * kFewRow + (m & 15);
         const float z = sums[at] + sums[kTile + at] + sums[2 * kTile + at] + sums[3 * kTile + at] + (bias ? up(bias[col]) : 0.f);
         s = join(s, {z, z != z ? z : 0.f, (int)col});
+        if (t == col) zt[m] = z;
       }
     __syncthreads();
   }
@@ -198,21 +202,263 @@ int few_linear(const clid_linear_args* a, hipStream_t s) {
   });
 }
 
-static int few_label_blocks(int64_t n) {
+static int few_blocks(int64_t n) {
   const int64_t tiles = (n + 63) / 64;
   return (int)(tiles < 4 * kCus ? tiles : 4 * kCus);
 }
-int64_t few_label_bytes(const clid_label_args* a) { return up256((int64_t)few_label_blocks(a->n) * a->rows * (int64_t)sizeof(Stat)); }
+int64_t few_label_bytes(const clid_label_args* a) { return up256((int64_t)few_blocks(a->n) * a->rows * (int64_t)sizeof(Stat)); }
 int few_label(const clid_label_args* a, hipStream_t s) {
-  const int blocks = few_label_blocks(a->n);
+  const int blocks = few_blocks(a->n);
   BY_DTYPE(a->dtype, {
     const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
     Stat* part = (Stat*)a->ws;
-    if (a->rows <= 16) hipLaunchKernelGGL((k_few_label<T, 1, 4>), dim3(blocks), dim3(256), 4 * 64 * kFewRow * 4, s, f, (const T*)a->bias, part);
-    else hipLaunchKernelGGL((k_few_label<T, 2, 4>), dim3(blocks), dim3(256), 8 * 64 * kFewRow * 4, s, f, (const T*)a->bias, part);
+    if (a->rows <= 16) hipLaunchKernelGGL((k_few_stat<T, 1, 4>), dim3(blocks), dim3(256), 4 * 64 * kFewRow * 4, s, f, (const T*)a->bias, (const int64_t*)nullptr, (float*)nullptr, part);
+    else hipLaunchKernelGGL((k_few_stat<T, 2, 4>), dim3(blocks), dim3(256), 8 * 64 * kFewRow * 4, s, f, (const T*)a->bias, (const int64_t*)nullptr, (float*)nullptr, part);
     hipLaunchKernelGGL(k_few_label_join, dim3((unsigned)a->rows), dim3(256), 0, s, (const Stat*)part, blocks, (int)a->rows, a->label, a->log_prob);
     return CLID_OK;
   });
+}
+
+
+// ---- cross entropy ----------------------------------------------------------------------------------------------------------
+
+// a row's statistics joined (32 threads a row), its loss, and the sums: one block
+__global__ void __launch_bounds__(1024) k_few_loss(const Stat* part, int blocks, const float* zt, const int64_t* target, int rows, int n, int64_t ignore,
+                                                   int reduction, float4* stat, float* total, float* loss_out) {
+  __shared__ double sums[32];
+  __shared__ int counts[32];
+  const int m = threadIdx.x >> 5, sub = threadIdx.x & 31;
+  Stat s = {neg_inf(), 0.f, 0x7fffffff};
+  if (m < rows)
+#pragma unroll 4
+    for (int b = sub; b < blocks; b += 32) s = join(s, part[(int64_t)b * rows + m]);
+  for (int d = 1; d < 32; d <<= 1) s = join(s, {__shfl_xor(s.m, d, 64), __shfl_xor(s.r, d, 64), __shfl_xor(s.at, d, 64)});
+  if (sub == 0) {
+    double l = 0.0;
+    int c = 0;
+    if (m < rows) {
+      const int64_t t = target[m];
+      float loss = 0.f;
+      if (t != ignore) {
+        loss = t >= 0 && t < n ? (s.m - zt[m]) + log1pf(s.r) : __builtin_nanf("");
+        c = 1;
+      }
+      stat[m] = {s.m, 1.f / (1.f + s.r), expm1f(-loss), loss};
+      if (reduction == CLID_REDUCE_NONE) loss_out[m] = loss;
+      l = loss;
+    }
+    sums[m] = l;
+    counts[m] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x) return;
+  double l = 0.0;
+  int c = 0;
+  for (int i = 0; i < 32; ++i) {
+    l += sums[i];
+    c += counts[i];
+  }
+  total[0] = (float)l;
+  total[1] = (float)c;
+  if (reduction == CLID_REDUCE_MEAN) loss_out[0] = c ? (float)(l / c) : 0.f;
+  if (reduction == CLID_REDUCE_SUM) loss_out[0] = (float)l;
+}
+
+// dz[m][np] in fp32 (zeros behind n, and in rows that do not count or are not there up to 16 MT), db
+template <typename T, int MT, int NT>
+__global__ void __launch_bounds__(256) k_few_dz(Few a, const T* bias, const int64_t* target, int64_t ignore, const float4* stat, const float* g, int reduction,
+                                                const float* total, float* dz, int64_t np, T* db) {
+  extern __shared__ __align__(16) char lds[];
+  constexpr int kTile = MT * NT * 16 * kFewRow, kCols = 16 * NT, kGroups = 256 / kCols;
+  float* sums = (float*)lds;
+  __shared__ float sb[kGroups][kCols];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int from, to;
+  few_share<T>(a, wave, 4, &from, &to);
+  const int64_t n0 = (int64_t)blockIdx.x * kCols;
+  few_tile<T, MT, NT>(a, n0, from, to, threadIdx.x & 63, sums + wave * kTile);
+  __syncthreads();
+  const int n = threadIdx.x % kCols, group = threadIdx.x / kCols;
+  const int64_t col = n0 + n;
+  const float b = bias && col < a.n ? up(bias[col]) : 0.f;
+  float all = 0.f;
+  for (int m = group; m < 16 * MT; m += kGroups) {
+    float v = 0.f;
+    if (m < a.m && col < a.n && target[m] != ignore) {
+      const float4 s = stat[m];
+      const int at = ((m >> 4) * kCols + n) * kFewRow + (m & 15);
+      const float z = sums[at] + sums[kTile + at] + sums[2 * kTile + at] + sums[3 * kTile + at] + b;
+      const float f = reduction == CLID_REDUCE_NONE ? g[m] : reduction == CLID_REDUCE_MEAN ? g[0] / fmaxf(total[1], 1.f) : g[0];
+      v = f * (s.w != s.w ? s.w : target[m] == col ? s.z : __builtin_amdgcn_exp2f((z - s.x) * 1.4426950408889634f) * s.y);
+    }
+    dz[m * np + col] = v;
+    all += v;
+  }
+  sb[group][n] = all;
+  __syncthreads();
+  if (db && group == 0 && col < a.n) {
+    for (int i = 1; i < kGroups; ++i) all += sb[i][n];
+    db[col] = down<T>(all);
+  }
+}
+
+// dx: block (128 columns of k, share of n) -> part[share][16 MT][k up to 128].  Lane l: 8 neighbouring columns 8 (l % 16) of row 4 (l / 16) + c of 16
+// rows of w, c = 0 .. 3; instruction j takes column j of the eight.
+template <typename T, int MT>
+__global__ void __launch_bounds__(256) k_few_dx(Few a, const float* dz, int64_t np, int64_t per, float* part) {
+  __shared__ float sums[3][MT * 16][128 + 4];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const int k0 = blockIdx.x * 128 + 8 * i, count = a.k - k0;
+  const int64_t v_end = (blockIdx.y + 1) * per < np ? (blockIdx.y + 1) * per : np;
+  f32x4 acc[MT][8];
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[t][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+  for (int64_t v = blockIdx.y * per + wave * 16; v < v_end; v += 64) {  // np is a multiple of 64
+    float w[4][8], d[MT][4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t row = v + 4 * q + c;
+      get8((const T*)a.w + row * a.ldw + k0, w[c], row < a.n ? count : 0);
+    }
+#pragma unroll
+    for (int t = 0; t < MT; ++t) *(float4*)d[t] = *(const float4*)(dz + (t * 16 + i) * np + v + 4 * q);
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[t][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(d[t][c], w[c][j], acc[t][j], 0, 0, 0);
+  }
+  // lane: rows 4 q + r, columns 8 i + j
+  if (wave)
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sums[wave - 1][t * 16 + 4 * q + r][8 * i + j] = acc[t][j][r];
+  __syncthreads();
+  if (wave) return;
+  const int64_t kp = (int64_t)gridDim.x * 128;
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int m = t * 16 + 4 * q + r;
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = acc[t][j][r] + sums[0][m][8 * i + j] + sums[1][m][8 * i + j] + sums[2][m][8 * i + j];
+      out8(part + (blockIdx.y * (int64_t)(16 * MT) + m) * kp + k0, v, 8);
+    }
+}
+template <typename T>
+__global__ void __launch_bounds__(256) k_few_dx_join(const float* part, int shares, int rows16, int64_t kp, int rows, int k, const int64_t* target, int64_t ignore, T* dx) {
+  const int64_t e = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (e >= (int64_t)rows * k) return;
+  const int m = (int)(e / k), c = (int)(e - (int64_t)m * k);
+  float s = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < shares; ++i) s += part[((int64_t)i * rows16 + m) * kp + c];
+  dx[e] = down<T>(target[m] == ignore ? 0.f : s);
+}
+
+// dw: a wave holds its 128 columns of x and walks 16 rows of dw at a time
+template <typename T, int MT>
+__global__ void __launch_bounds__(256) k_few_dw(Few a, const int64_t* target, int64_t ignore, const float* dz, int64_t np, T* dw) {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+  const int k0 = blockIdx.x * 128 + 8 * i, count = a.k - k0;
+  float x[4 * MT][8];
+#pragma unroll
+  for (int s = 0; s < 4 * MT; ++s) {
+    const int m = 4 * s + q;
+    const bool on = m < a.m && target[m] != ignore;  // a row that does not count is zeros whatever it holds
+    get8((const T*)a.x + (int64_t)m * a.ldx + k0, x[s], on ? count : 0);
+  }
+  for (int64_t v = ((int64_t)blockIdx.y * 4 + wave) * 16; v < np; v += (int64_t)gridDim.y * 64) {
+    float d[4 * MT];
+#pragma unroll
+    for (int s = 0; s < 4 * MT; ++s) d[s] = dz[(4 * s + q) * np + v + i];
+    f32x4 acc[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < 4 * MT; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) acc[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(d[s], x[s][j], acc[j], 0, 0, 0);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int64_t row = v + 4 * q + r;
+      T t[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) t[j] = down<T>(acc[j][r]);
+      if (row < a.n) out8(dw + row * a.k + k0, t, count);
+    }
+  }
+}
+
+int64_t few_ce_bytes(const clid_ce_args* a) { return up256((int64_t)few_blocks(a->n) * a->rows * (int64_t)sizeof(Stat)) + up256(a->rows * 4); }
+int few_ce(const clid_ce_args* a, float4* stat, float* total, hipStream_t s) {
+  const int blocks = few_blocks(a->n);
+  Stat* part = (Stat*)a->ws;
+  float* zt = (float*)((char*)a->ws + up256((int64_t)blocks * a->rows * (int64_t)sizeof(Stat)));
+  BY_DTYPE(a->dtype, {
+    const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
+    if (a->rows <= 16) hipLaunchKernelGGL((k_few_stat<T, 1, 4>), dim3(blocks), dim3(256), 4 * 64 * kFewRow * 4, s, f, (const T*)a->bias, a->target, zt, part);
+    else hipLaunchKernelGGL((k_few_stat<T, 2, 4>), dim3(blocks), dim3(256), 8 * 64 * kFewRow * 4, s, f, (const T*)a->bias, a->target, zt, part);
+  });
+  hipLaunchKernelGGL(k_few_loss, dim3(1), dim3(1024), 0, s, (const Stat*)part, blocks, (const float*)zt, a->target, (int)a->rows, a->n, a->ignore_index,
+                     a->reduction, stat, total, a->loss_out);
+  return CLID_OK;
+}
+
+struct FewBwd {
+  int64_t np, kp, per;
+  int mt, shares;
+  char *dz, *part;
+  int64_t bytes;
+  explicit FewBwd(const clid_ce_args* a) {
+    Ws ws(a->ws);
+    np = (a->n + 63) / 64 * 64;
+    kp = (a->k + 127) / 128 * 128;
+    mt = a->rows <= 16 ? 1 : 2;
+    // blocks of 128 columns of k and of shares of n: about 4 a CU, a share 256 rows of w at least
+    int64_t want = 4 * kCus / (kp / 128), most = (np + 255) / 256;
+    shares = (int)(want < 1 ? 1 : want < most ? want : most);
+    per = ((np + shares - 1) / shares + 63) / 64 * 64;
+    shares = (int)((np + per - 1) / per);
+    dz = ws.take(16 * mt * np * 4);
+    part = ws.take(a->dx ? (int64_t)shares * 16 * mt * kp * 4 : 0);
+    bytes = ws.used;
+  }
+};
+int64_t few_ce_bwd_bytes(const clid_ce_args* a) { return FewBwd(a).bytes; }
+template <typename T, int MT>
+static void few_bwd_launch(const clid_ce_args* a, const FewBwd& b, const float4* stat, const float* total, hipStream_t s) {
+  const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
+  float* dz = (float*)b.dz;
+  const unsigned kb = (unsigned)(b.kp / 128);
+  hipLaunchKernelGGL((k_few_dz<T, MT, 4>), dim3((unsigned)(b.np / 64)), dim3(256), 4 * MT * 64 * kFewRow * 4, s, f, (const T*)a->bias, a->target, a->ignore_index, stat,
+                     a->g, a->reduction, total, dz, b.np, (T*)a->db);
+  if (a->dx) {
+    hipLaunchKernelGGL((k_few_dx<T, MT>), dim3(kb, (unsigned)b.shares), dim3(256), 0, s, f, (const float*)dz, b.np, b.per, (float*)b.part);
+    hipLaunchKernelGGL(k_few_dx_join<T>, dim3((unsigned)((a->rows * a->k + 255) / 256)), dim3(256), 0, s, (const float*)b.part, b.shares, 16 * MT, b.kp, (int)a->rows, a->k,
+                       a->target, a->ignore_index, (T*)a->dx);
+  }
+  if (a->dw) {
+    const int64_t tiles = b.np / 64, want = 8 * kCus / kb + 1;
+    hipLaunchKernelGGL((k_few_dw<T, MT>), dim3(kb, (unsigned)(tiles < want ? tiles : want)), dim3(256), 0, s, f, a->target, a->ignore_index, (const float*)dz, b.np, (T*)a->dw);
+  }
+}
+int few_ce_bwd(const clid_ce_args* a, const float4* stat, const float* total, hipStream_t s) {
+  const FewBwd b(a);
+  BY_DTYPE(a->dtype, {
+    if (b.mt == 1) few_bwd_launch<T, 1>(a, b, stat, total, s);
+    else few_bwd_launch<T, 2>(a, b, stat, total, s);
+  });
+  return CLID_OK;
 }
 
 }  // namespace clid_dense

@@ -205,6 +205,10 @@ inline bool is_few(int64_t rows) { return rows <= 32; }
 int few_linear(const clid_linear_args* a, hipStream_t s);
 int64_t few_label_bytes(const clid_label_args* a);
 int few_label(const clid_label_args* a, hipStream_t s);
+int64_t few_ce_bytes(const clid_ce_args* a);
+int few_ce(const clid_ce_args* a, float4* stat, float* total, hipStream_t s);
+int64_t few_ce_bwd_bytes(const clid_ce_args* a);
+int few_ce_bwd(const clid_ce_args* a, const float4* stat, const float* total, hipStream_t s);
 
 // ---- tiles --------------------------------------------------------------------------------------------------------------
 template <int NP, int SIZE> struct Tile;

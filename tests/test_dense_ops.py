@@ -136,7 +136,7 @@ def test_linear_act(shape, act, dtype):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("reduction", list(L.REDUCTIONS))
 @pytest.mark.parametrize("shape", [(1, 1, 1), (1, 8, 2), (5, 11, 21), (64, 64, 21), (130, 72, 64), (33, 100, 1000), (257, 130, 333), (7, 512, 4099),
-                                   (600, 64, 513), (1, 300, 2000)], ids=str)
+                                   (600, 64, 513), (1, 300, 2000), (16, 200, 1500), (17, 129, 130), (32, 1031, 700)], ids=str)
 @pytest.mark.parametrize("ignored", [0.0, 0.5, 1.0])
 def test_cross_entropy(shape, reduction, dtype, ignored):
     m, k, n = shape
