@@ -74,17 +74,13 @@ __device__ __forceinline__ float act_slope(float z, int act) {
   }
 }
 
-// z as the backward pass gets it (clid_linear_args.z_out): rounding to 16 bits must not turn a slope of 1 into one of 0 (a tiny z
-// becoming 0) nor a finite z into an infinity (z p (1 - p) of silu is inf * 0 there)
-template <typename T> __device__ __forceinline__ T keep_z(float z);
+// z as the backward pass gets it (clid_linear_args.z_out): fp32, or fp16 for both 16-bit types (a slope is wrong by the rounding of z times
+// its own slope, 2^-12 |z| in fp16, 2^-9 |z| in bf16; beyond 65504 every slope is constant).  Rounding must not turn a slope of 1 into one of
+// 0 (a tiny z becoming 0) nor a finite z into an infinity (z p (1 - p) of silu is inf * 0 there).
+template <typename T> struct KeptZ { using Z = f16; };
+template <> struct KeptZ<float> { using Z = float; };
+template <typename Z> __device__ __forceinline__ Z keep_z(float z);
 template <> __device__ __forceinline__ float keep_z<float>(float z) { return z; }
-template <> __device__ __forceinline__ bf16 keep_z<bf16>(float z) {
-  bf16 h = down<bf16>(z);
-  const float b = up(h);
-  if (b == 0.f && z != 0.f) h = down<bf16>(copysignf(9.1835496e-41f, z));             // 2^-133, the smallest bf16
-  if (fabsf(b) > 3.3895314e38f && fabsf(z) <= 3.4028235e38f) h = down<bf16>(copysignf(3.3895314e38f, z));  // its largest
-  return h;
-}
 template <> __device__ __forceinline__ f16 keep_z<f16>(float z) {
   f16 h = down<f16>(z);
   const float b = up(h);

@@ -38,13 +38,15 @@ __device__ __forceinline__ void out8(T* p, const T (&t)[8], int count) {
 // z + bias -> act -> + residual -> y, and z for the backward pass
 template <typename T>
 struct LinearOut {
+  using Z = typename KeptZ<T>::Z;
   const T *bias, *res;
-  T *y, *z;
+  T* y;
+  Z* z;
   int64_t ldr, n;
   int act;
   __device__ __forceinline__ void one(float v, int64_t m, int64_t c) const {
     v += bias ? up(bias[c]) : 0.f;
-    if (z) z[m * n + c] = keep_z<T>(v);
+    if (z) z[m * n + c] = keep_z<Z>(v);
     y[m * n + c] = down<T>(act_value(v, act) + (res ? up(res[m * ldr + c]) : 0.f));
   }
   // v: sums at row m, columns c ..; b: their bias
@@ -57,9 +59,10 @@ struct LinearOut {
 #pragma unroll
     for (int q = 0; q < 8; ++q) v[q] += b[q];
     if (z) {
+      Z k[8];
 #pragma unroll
-      for (int q = 0; q < 8; ++q) t[q] = keep_z<T>(v[q]);
-      out8(z + m * n + c, t, count);
+      for (int q = 0; q < 8; ++q) k[q] = keep_z<Z>(v[q]);
+      out8(z + m * n + c, k, count);
     }
 #pragma unroll
     for (int q = 0; q < 8; ++q) t[q] = down<T>(act_value(v[q], act) + r[q]);

@@ -190,7 +190,7 @@ static int few_linear_launch(const Few& f, const LinearOut<T>& o, int waves, hip
 int few_linear(const clid_linear_args* a, hipStream_t s) {
   BY_DTYPE(a->dtype, {
     const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
-    const LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (T*)a->z_out, a->ldr, a->n, a->act};
+    const LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (KeptZ<T>::Z*)a->z_out, a->ldr, a->n, a->act};
     const int steps = (a->k + Frag<T>::kStep - 1) / Frag<T>::kStep;
     if (a->n >= 64 * 1024) {  // 1024 blocks of 64 columns
       const int waves = steps >= 16 ? 4 : steps >= 8 ? 2 : 1;

@@ -25,7 +25,7 @@ template <typename T>
 int fwd(const clid_linear_args* a, hipStream_t s) {
   const Fwd<T> f(a);
   Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
-  LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (T*)a->z_out, a->ldr, a->n, a->act};
+  LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (typename KeptZ<T>::Z*)a->z_out, a->ldr, a->n, a->act};
   return launch_out<T, false, false>(g, f.p, o, f.part, s);
 }
 
@@ -56,13 +56,16 @@ template <typename T>
 int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
   const Bwd<T> f(a);
   const int np = (int)padded<T>(a->n);
-  const T* z = a->act == CLID_ACT_NONE ? nullptr : (const T*)a->z;
   Operand dz = {(const uint16_t*)a->dy, a->lddy};
   if (f.own_dz) dz = {(const uint16_t*)f.dz, np * Kind<T>::NP};
   if (f.own_dz || a->db) {
-    hipLaunchKernelGGL(k_dz<T>, dim3((np + 255) / 256, f.blocks), dim3(256), 0, s, (const T*)a->dy, a->lddy, z, a->rows, a->n, a->act,
-                       f.own_dz ? (uint16_t*)f.dz : nullptr, np,
-                       a->db ? (float*)f.sums : nullptr);
+    const auto launch = [&](auto* z) {
+      using Z = std::remove_const_t<std::remove_pointer_t<decltype(z)>>;
+      hipLaunchKernelGGL((k_dz<T, Z>), dim3((np + 255) / 256, f.blocks), dim3(256), 0, s, (const T*)a->dy, a->lddy, a->act == CLID_ACT_NONE ? nullptr : z, a->rows, a->n,
+                         a->act, f.own_dz ? (uint16_t*)f.dz : nullptr, np, a->db ? (float*)f.sums : nullptr);
+    };
+    if (a->z_is_y) launch((const T*)a->z);
+    else launch((const typename KeptZ<T>::Z*)a->z);
     if (a->db)
       hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
   }

@@ -28,7 +28,7 @@ struct Narrow {
   const void *res, *dy, *z_in;
   void *y, *z_out;
   int64_t ldr, lddy;
-  int act;
+  int act, z_is_y;
   // LinearBwd, CeBwd
   void* dx;
   float* part;  // [blocks][n k + n]: sums for dw and db
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     }
 
     if constexpr (DO == Do::Linear) {
-      const LinearOut<T> o = {nullptr, (const T*)a.res, (T*)a.y, (T*)a.z_out, a.ldr, a.n, a.act};
+      const LinearOut<T> o = {nullptr, (const T*)a.res, (T*)a.y, (typename KeptZ<T>::Z*)a.z_out, a.ldr, a.n, a.act};
       float* tile = (float*)xs;  // x is done with
       Rows32<TN>::put(tile, z, lane);
       __builtin_amdgcn_wave_barrier();
@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
           get8((const T*)a.dy + (m0 + row) * a.lddy + c, v, count);
           if (a.z_in) {
             float y[8];
-            get8((const T*)a.z_in + (m0 + row) * a.n + c, y, count);
+            if (a.z_is_y) get8((const T*)a.z_in + (m0 + row) * a.n + c, y, count);
+            else get8((const typename KeptZ<T>::Z*)a.z_in + (m0 + row) * a.n + c, y, count);
 #pragma unroll
             for (int q = 0; q < 8; ++q) v[q] = q < count ? v[q] * act_slope(y[q], a.act) : 0.f;
           }
@@ -570,7 +571,7 @@ int64_t narrow_linear_bwd_bytes(const clid_linear_bwd_args* c) { return part_byt
 int narrow_linear_bwd(const clid_linear_bwd_args* c, hipStream_t s) {
   BY_DTYPE(c->dtype, {
     Narrow a = narrow_args<T>(c->x, c->ldx, c->w, c->ldw, nullptr, c->rows, c->k, c->n);
-    a.dy = c->dy; a.lddy = c->lddy; a.z_in = c->act == CLID_ACT_NONE ? nullptr : c->z; a.act = c->act;
+    a.dy = c->dy; a.lddy = c->lddy; a.z_in = c->act == CLID_ACT_NONE ? nullptr : c->z; a.act = c->act; a.z_is_y = c->z_is_y;
     a.dx = c->dx; a.part = (float*)c->ws; a.want_w = c->dw != nullptr;
     return narrow_bwd<T, Do::LinearBwd>(a, c->dw, c->db, s);
   });

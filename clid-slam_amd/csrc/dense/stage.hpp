@@ -78,8 +78,8 @@ inline Operand stage(const void* p, int64_t ld, int64_t rows, int k, char* ws, h
 
 // dz = dy act'(z) -> planes with rows of np values (dst may be NULL: the sums alone), and its column sums over blocks of rows ->
 // part[row block][n].  A block takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows.
-template <typename T>
-__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const T* z, int64_t rows, int n, int act, uint16_t* dst, int np, float* part) {
+template <typename T, typename Z>
+__global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const Z* z, int64_t rows, int n, int act, uint16_t* dst, int np, float* part) {
   __shared__ float sums[8][256 + 8];
   const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8, count = n - c < 8 ? n - c : 8;
   float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

@@ -27,7 +27,7 @@ class LinearArgs(C.Structure):
 class LinearBwdArgs(C.Structure):
     _fields_ = [("x", _vp), ("w", _vp), ("dy", _vp), ("z", _vp), ("dx", _vp), ("dw", _vp), ("db", _vp),
                 ("ldx", _i64), ("ldw", _i64), ("lddy", _i64), ("rows", _i64),
-                ("k", _i32), ("n", _i32), ("dtype", _i32), ("act", _i32), ("ws", _vp), ("ws_bytes", _i64)]
+                ("k", _i32), ("n", _i32), ("dtype", _i32), ("act", _i32), ("z_is_y", _i32), ("reserved", _i32), ("ws", _vp), ("ws_bytes", _i64)]
 
 
 class CeArgs(C.Structure):
@@ -145,7 +145,7 @@ def _forward(x, weight, bias, act, residual, keep_z):
     r, ldr = (None, n) if residual is None else rows_of(residual, n)
     b = None if bias is None else bias.contiguous()
     y = torch.empty((*x.shape[:-1], n), dtype=x.dtype, device=x.device)
-    z = torch.empty_like(y) if keep_z else None
+    z = torch.empty(y.shape, dtype=torch.float32 if x.dtype == torch.float32 else torch.float16, device=x.device) if keep_z else None
     rows = x2.shape[0]
     if rows:
         call("clid_linear_fwd", "clid_linear_workspace",
@@ -161,7 +161,7 @@ class _LinearAct(torch.autograd.Function):
         # (float16 excepted: a z under 2^-25 would be 0 in y)
         sign_of_y = act in (ACTIVATIONS["relu"], ACTIVATIONS["leaky_relu"]) and residual is None and x.dtype != torch.float16
         y, z = _forward(x, weight, bias, act, residual, act != 0 and not sign_of_y)
-        ctx.act = act
+        ctx.act, ctx.z_is_y = act, int(sign_of_y)
         ctx.save_for_backward(x, weight, y if sign_of_y else z)
         return y
 
@@ -184,7 +184,7 @@ class _LinearAct(torch.autograd.Function):
         elif need_x or need_w or need_b:
             call("clid_linear_bwd", "clid_linear_bwd_workspace",
                  LinearBwdArgs(x2.data_ptr(), w.data_ptr(), dy2.data_ptr(), _lib.ptr(z), _lib.ptr(dx), _lib.ptr(dw), _lib.ptr(db), ldx, ldw,
-                               lddy, rows, k, n, DTYPES[dtype], ctx.act), device)
+                               lddy, rows, k, n, DTYPES[dtype], ctx.act, ctx.z_is_y), device)
         return dx, dw, db, (dy if need_r else None), None
 
 

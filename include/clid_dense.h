@@ -32,8 +32,9 @@ extern "C" {
 #define CLID_ACT_GELU 3       /* z Phi(z), the erf form */
 #define CLID_ACT_SILU 4       /* z / (1 + exp(-z)) */
 
-/* y = act(x w^T + bias) + residual.  z_out (may be NULL): x w^T + bias in dtype for the backward pass -- nearest, except that a
- * non-zero z never becomes 0 and a finite one never becomes infinite, so that its activation's slope stays the right one. */
+/* y = act(x w^T + bias) + residual.  z_out (may be NULL): x w^T + bias for the backward pass, in fp32 or, where dtype has 16 bits, in
+ * fp16 (also for bf16: a slope needs the bits more than the range) -- nearest, except that a non-zero z never becomes 0 and a finite
+ * one never becomes infinite, so that its activation's slope stays the right one. */
 typedef struct clid_linear_args {
   const void *x, *w, *bias, *residual; /* [rows][k], [n][k], [n] or NULL, [rows][n] or NULL */
   void *y, *z_out;                     /* [rows][n], [rows][n] or NULL (both dense: ld = n) */
@@ -46,15 +47,15 @@ typedef struct clid_linear_args {
 int64_t clid_linear_workspace(const clid_linear_args* a);
 int clid_linear_fwd(const clid_linear_args* a, void* stream);
 
-/* dz = dy act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz.  z (dense) is z_out of the forward call; for relu and
- * leaky_relu without a residual it may be y, whose sign is z's; NULL for CLID_ACT_NONE.  dx, dw, db: NULL where not wanted.
+/* dz = dy act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz.  z (dense) is z_out of the forward call, or with
+ * z_is_y (relu and leaky_relu without a residual) its y, whose sign is z's; NULL for CLID_ACT_NONE.  dx, dw, db: NULL where not wanted.
  * dz is rounded to dtype between the products (fp32: not at all). */
 typedef struct clid_linear_bwd_args {
   const void *x, *w, *dy, *z;
   void *dx, *dw, *db; /* dense: [rows][k], [n][k], [n] */
   int64_t ldx, ldw, lddy;
   int64_t rows;
-  int32_t k, n, dtype, act;
+  int32_t k, n, dtype, act, z_is_y, reserved;
   void* ws;
   int64_t ws_bytes;
 } clid_linear_bwd_args;

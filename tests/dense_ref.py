@@ -66,7 +66,8 @@ def linear(x, w, b, r, name, dy=None):
     if dy is not None:
         dy = dy.double()
         dz = dy * slope
-        e_slope = s2 * rounded(z, ez, dt) + 16 * U
+        kept = torch.float32 if dt == torch.float32 else torch.float16  # what the backward pass has of z
+        e_slope = s2 * rounded(z, ez, kept) + 16 * U
         edz = rounded(dz, dy.abs() * e_slope, dt)  # the products take dz in dt
         out |= gradients(x, w, dz, edz, dt)
     return out
