@@ -2,6 +2,7 @@
 // choice of tile.
 #pragma once
 #include <atomic>
+#include <type_traits>
 
 #include "epi.hpp"
 
@@ -231,7 +232,8 @@ constexpr int kCus = 256;
 // after the other (rounds of 256 blocks) at a rate that grows with the tile, since a larger tile reads less LDS and memory per
 // product; a part costs its sums' trip through memory and back, and a launch.  The rates are about those of 8192 x 2048 x 8192 bf16 (tiles
 // 64, 128, 256: 474, 396, 256 us) and 2048 x 1024 x 8192 fp32 (274, 209, 194 us); a cut costs 13 us at 2048 x 1024 x 1024 bf16 in two
-// parts (13.3 -> 26.6 us) and gains at 128 x 8192 x 1024 in eight (40 -> 17.7 us).
+// parts (13.3 -> 26.6 us) and gains at 128 x 8192 x 1024 in eight (40 -> 17.7 us).  Nor is it faster than the operands come, every tile's own,
+// out of the L2s: 14 TB/s (333 x 50024 x 768 bf16: 112 us in 7 parts of tile 64, 57 in 32 of tile 256).
 struct Plan {
   int size, splits;
 };
@@ -248,6 +250,8 @@ inline Plan plan(int64_t m, int64_t n, int64_t k, bool may_split) {
       const double rounds = (double)((tiles * s + kCus - 1) / kCus);
       const double share = (double)((steps + s - 1) / s) * bk;
       double t = rounds * (2.0 * bm * bn * share * (NP == 3 ? 6 : 1) / rate[size] + 1e-6);
+      const double traffic = (double)tiles * (bm + bn) * k * 2 * NP / 14e12;
+      if (t < traffic) t = traffic;
       if (s > 1) t += 6e-6 + (double)s * m * n * 8 / 4e12;
       if (t < least) {
         least = t;

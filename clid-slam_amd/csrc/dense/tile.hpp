@@ -19,8 +19,6 @@
 // Blocks.  Block ids go round the 8 XCDs in turn; consecutive tiles of one XCD share rows of Q (8 of them, then the next m), so that an
 // XCD's 32 CUs work on an 8 x 4 patch of tiles out of their own L2.
 #pragma once
-#include <type_traits>
-
 #include "dense.hpp"
 
 namespace clid_dense {
@@ -277,55 +275,39 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
   // The fragments of a product are read while the one before is multiplied, also across the barrier: the matrix pipes have the last
   // product of step s to do while the first fragments of step s + 1 come.
   constexpr int KK = BK / 16;
-  constexpr bool kAcross = STAGES >= 3;  // (two stages: the copy is too late for that)
-  constexpr bool kTwo = !(NP == 3 && !kAcross);  // (fp32's large tile has no registers for two: 14 of them would be spilled)
+  static_assert(KK % 2 == 0, "a step's first fragments are f[0]");
+  constexpr bool kAcross = STAGES >= 3;         // (two stages: the copy is too late for that)
+  constexpr bool kAhead = NP == 1 || kAcross;   // (fp32's large tile has no registers for two: 14 of them would be spilled)
   Frags f[2];
-  auto step = [&](int s, auto parity) {
-    constexpr int kFirst = decltype(parity)::value;
-    const char* buf = lds + s % STAGES * kStage;
-    if constexpr (!kAcross) {
-      arrive(false);
-      read(buf, 0, f[kFirst]);
-    }
-    if constexpr (!kTwo) {
-#pragma unroll
-      for (int kk = 0; kk < KK; ++kk) {
-        if (kk) read(buf, kk, f[0]);
-        if (kk == 0 && s + STAGES - 1 < steps) load();
-        multiply(f[0]);
-      }
-      return;
-    }
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      Frags &now = f[(kFirst + kk) & 1], &next = f[(kFirst + kk + 1) & 1];
-      if (KK == 1 && s + STAGES - 1 < steps) load();
-      if (kk + 1 < KK) {
-        read(buf, kk + 1, next);
-      } else if (kAcross && s + 1 < steps) {
-        arrive(s + STAGES - 1 < steps);
-        read(lds + (s + 1) % STAGES * kStage, 0, next);
-      }
-      if (KK > 1 && kk == 0 && s + STAGES - 1 < steps) load();
-      multiply(now);
-      __builtin_amdgcn_sched_barrier(0);  // without it the compiler moves reads back to their use
-    }
-  };
   for (int s = 0; s < STAGES - 1; ++s)
     if (s < steps) load();
   epi.prepare(n0, lds + kBias);
-  if (steps > 0) {
-    if constexpr (kAcross) {
-      arrive(steps >= STAGES - 1);
-      read(lds, 0, f[0]);
+  if (kAcross && steps > 0) {
+    arrive(steps >= STAGES - 1);
+    read(lds, 0, f[0]);
+  }
+  for (int s = 0; s < steps; ++s) {
+    const char* buf = lds + s % STAGES * kStage;
+    if constexpr (!kAcross) {
+      arrive(false);
+      read(buf, 0, f[0]);
     }
-    if constexpr (KK % 2 == 0) {
-      for (int s = 0; s < steps; ++s) step(s, std::integral_constant<int, 0>());
-    } else {
-      for (int s = 0; s < steps; s += 2) {
-        step(s, std::integral_constant<int, 0>());
-        if (s + 1 < steps) step(s + 1, std::integral_constant<int, 1>());
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      Frags &now = f[kAhead ? kk & 1 : 0], &next = f[(kk + 1) & 1];
+      if constexpr (kAhead) {
+        if (kk + 1 < KK) {
+          read(buf, kk + 1, next);
+        } else if (kAcross && s + 1 < steps) {
+          arrive(s + STAGES - 1 < steps);
+          read(lds + (s + 1) % STAGES * kStage, 0, next);
+        }
+      } else if (kk) {
+        read(buf, kk, now);
       }
+      if (kk == 0 && s + STAGES - 1 < steps) load();  // behind the reads that the products wait for
+      multiply(now);
+      if constexpr (kAhead) __builtin_amdgcn_sched_barrier(0);  // without it the compiler moves reads back to their use
     }
   }
   if constexpr (NP == 3) {
