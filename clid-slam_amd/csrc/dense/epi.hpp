@@ -333,7 +333,7 @@ struct EpiDz {
     const int64_t from = order[m];
     const float4 s = stat[m];
     const int64_t tt = target[from] - v0 - nw;
-    const int t = tt >= 0 && tt < 32 * TN ? (int)tt : -1;
+    const int t = tt >= 0 && tt < 32 * TN && tt < n - nw ? (int)tt : -1;  // (a class that is not there: the row is NaN by stat)
     float f = scale[0];
     if (g) f *= g[from];
     const float inv = s.w != s.w ? s.w : s.y * f;

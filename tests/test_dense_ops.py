@@ -325,6 +325,25 @@ def test_cross_entropy_of_masked_classes_and_bad_targets():
 
 
 @gpu
+@pytest.mark.parametrize("m,k,n", [(40, 100, 72), (40, 100, 65), (40, 24, 70), (300, 96, 264), (20, 100, 72), (300, 16, 21)])
+def test_a_target_behind_the_last_class_reaches_its_own_row_only(m, k, n):
+    """Targets n .. n + 200 (in the last tile's empty columns, and behind them): NaN in their rows, nothing in the others'."""
+    for dt in TYPES.values():
+        gen = generator(n)
+        x, w = normal(gen, m, k).to(dt).requires_grad_(), (normal(gen, n, k) * k ** -0.5).to(dt).requires_grad_()
+        target = torch.randint(0, n, (m,), generator=gen, device="cuda")
+        bad = torch.arange(m, device="cuda") % 3 == 2  # the last row of some sizes among them
+        target[bad] = n + 7 * torch.arange(int(bad.sum()), device="cuda") % 200
+        target[2], target[m - 1], bad[m - 1] = n, n + 1, True
+        loss = linear_cross_entropy(x, w, None, target, reduction="none")
+        gx = torch.autograd.grad(loss, x, torch.ones(m, device="cuda"))[0]
+        good = ~bad
+        want = ref.cross_entropy(x[good], w, None, target[good], -100, "sum", torch.ones((), device="cuda"))
+        ref.close(gx[good], *want["dx"], "dx")
+        assert torch.isnan(gx[bad]).all() and torch.equal(torch.isnan(loss), bad)
+
+
+@gpu
 def test_no_rows_and_leading_dimensions():
     for dt in TYPES.values():
         x = torch.zeros(0, 16, device="cuda", dtype=dt, requires_grad=True)
