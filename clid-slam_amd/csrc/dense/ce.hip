@@ -60,37 +60,39 @@ __global__ void __launch_bounds__(1024) k_order(const int64_t* target, int64_t r
   if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) order[rows] = before + total;
 }
 
-// a row's strips joined: 16 rows a block, 32 threads a row; the block's sum of losses
+// blocks of at most 1024 threads that one launch takes (2^32 threads); what is left they walk
+constexpr int64_t kMostJoins = int64_t(1) << 21;
+
+// a row's strips joined: 16 rows a block and turn, 32 threads a row; the block's sum of losses
 __global__ void __launch_bounds__(512) k_loss_rows(const float2* part, int strips, const float* zt, const int64_t* target, const int32_t* order,
                                                    int64_t rows, int n, float4* stat, float* loss_none, double* sums) {
   __shared__ float pm[32][kJoinRows], pr[32][kJoinRows];
   const int64_t live = order[rows];
   const int row = threadIdx.x % kJoinRows, g = threadIdx.x / kJoinRows;
-  const int64_t j = (int64_t)blockIdx.x * kJoinRows + row;
-  if ((int64_t)blockIdx.x * kJoinRows >= live) {
-    if (threadIdx.x == 0) sums[blockIdx.x] = 0.0;
-    return;
-  }
-  Stat s = {neg_inf(), 0.f, 0};
-  if (j < live)
-#pragma unroll 4
-    for (int i = g; i < strips; i += 32) {
-      const float2 p = part[(int64_t)i * rows + j];
-      s = join(s, {p.x, p.y, 0});
-    }
-  pm[g][row] = s.m;
-  pr[g][row] = s.r;
-  __syncthreads();
-  if (g) return;
   double sum = 0.0;
-  if (j < live) {
-    for (int i = 1; i < 32; ++i) s = join(s, {pm[i][row], pr[i][row], 0});
-    const int64_t m = order[j], t = target[m];
-    const float loss = t >= 0 && t < n ? (s.m - zt[j]) + log1pf(s.r) : __builtin_nanf("");
-    stat[j] = {s.m, 1.f / (1.f + s.r), expm1f(-loss), loss};
-    if (loss_none) loss_none[m] = loss;
-    sum = loss;
+  for (int64_t j0 = (int64_t)blockIdx.x * kJoinRows; j0 < live; j0 += (int64_t)gridDim.x * kJoinRows) {
+    const int64_t j = j0 + row;
+    Stat s = {neg_inf(), 0.f, 0};
+    if (j < live)
+#pragma unroll 4
+      for (int i = g; i < strips; i += 32) {
+        const float2 p = part[(int64_t)i * rows + j];
+        s = join(s, {p.x, p.y, 0});
+      }
+    __syncthreads();  // the turn before has been read
+    pm[g][row] = s.m;
+    pr[g][row] = s.r;
+    __syncthreads();
+    if (g == 0 && j < live) {
+      for (int i = 1; i < 32; ++i) s = join(s, {pm[i][row], pr[i][row], 0});
+      const int64_t m = order[j], t = target[m];
+      const float loss = t >= 0 && t < n ? (s.m - zt[j]) + log1pf(s.r) : __builtin_nanf("");
+      stat[j] = {s.m, 1.f / (1.f + s.r), expm1f(-loss), loss};
+      if (loss_none) loss_none[m] = loss;
+      sum += loss;
+    }
   }
+  if (g) return;
   for (int d = kJoinRows / 2; d; d >>= 1) sum += __shfl_xor(sum, d, 64);
   if (threadIdx.x == 0) sums[blockIdx.x] = sum;
 }
@@ -115,21 +117,24 @@ __global__ void __launch_bounds__(256) k_label_join(const float2* part, const in
   __shared__ float pm[16][16], pr[16][16];
   __shared__ int pa[16][16];
   const int row = threadIdx.x & 15, g = threadIdx.x >> 4;
-  const int64_t m = (int64_t)blockIdx.x * 16 + row;
-  Stat s = {neg_inf(), 0.f, 0x7fffffff};
-  if (m < rows)
-    for (int i = g; i < strips; i += 16) {
-      const float2 p = part[(int64_t)i * rows + m];
-      s = join(s, {p.x, p.y, part_at[(int64_t)i * rows + m]});
-    }
-  pm[g][row] = s.m;
-  pr[g][row] = s.r;
-  pa[g][row] = s.at;
-  __syncthreads();
-  if (g || m >= rows) return;
-  for (int i = 1; i < 16; ++i) s = join(s, {pm[i][row], pr[i][row], pa[i][row]});
-  label[m] = s.at;
-  log_prob[m] = s.m == neg_inf() ? __builtin_nanf("") : -log1pf(s.r);
+  for (int64_t m0 = (int64_t)blockIdx.x * 16; m0 < rows; m0 += (int64_t)gridDim.x * 16) {
+    const int64_t m = m0 + row;
+    Stat s = {neg_inf(), 0.f, 0x7fffffff};
+    if (m < rows)
+      for (int i = g; i < strips; i += 16) {
+        const float2 p = part[(int64_t)i * rows + m];
+        s = join(s, {p.x, p.y, part_at[(int64_t)i * rows + m]});
+      }
+    __syncthreads();  // the turn before has been read
+    pm[g][row] = s.m;
+    pr[g][row] = s.r;
+    pa[g][row] = s.at;
+    __syncthreads();
+    if (g || m >= rows) continue;
+    for (int i = 1; i < 16; ++i) s = join(s, {pm[i][row], pr[i][row], pa[i][row]});
+    label[m] = s.at;
+    log_prob[m] = s.m == neg_inf() ? __builtin_nanf("") : -log1pf(s.r);
+  }
 }
 
 // scale[0]: what dz is multiplied by as it is stored, scale[1]: what its products are multiplied by.  mean and sum: the one factor
@@ -221,7 +226,8 @@ struct CeFwd {
     Ws ws(a->ws);
     p = plan<Kind<T>::NP>(a->rows, a->n, a->k, false);
     strips = (a->n + strip_width<T>(p.size) - 1) / strip_width<T>(p.size);
-    joins = (int)((a->rows + kJoinRows - 1) / kJoinRows);
+    const int64_t j = (a->rows + kJoinRows - 1) / kJoinRows;
+    joins = (int)(j < kMostJoins ? j : kMostJoins);
     x = ws.take(stage_bytes<T>(a->x, a->ldx, a->rows, a->k, true));
     w = ws.take(stage_bytes<T>(a->w, a->ldw, a->n, a->k));
     counts = ws.take((a->rows + kRowsPer - 1) / kRowsPer * 4);
@@ -358,7 +364,8 @@ int label(const clid_label_args* a, hipStream_t s) {
   Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
   const int rc = launch_stat<T, true>(g, f.p.size, (const T*)a->bias, nullptr, nullptr, (float2*)f.part, (int32_t*)f.at, nullptr, s);
   if (rc != CLID_OK) return rc;
-  hipLaunchKernelGGL(k_label_join, dim3((unsigned)((a->rows + 15) / 16)), dim3(256), 0, s, (const float2*)f.part, (const int32_t*)f.at, f.strips, a->rows, a->label, a->log_prob);
+  const int64_t joins = (a->rows + 15) / 16;
+  hipLaunchKernelGGL(k_label_join, dim3((unsigned)(joins < kMostJoins ? joins : kMostJoins)), dim3(256), 0, s, (const float2*)f.part, (const int32_t*)f.at, f.strips, a->rows, a->label, a->log_prob);
   return CLID_OK;
 }
 

@@ -1,6 +1,7 @@
 """The dense operators (linear_act, linear_cross_entropy, linear_label) against plain 64-bit forms (dense_ref.py), their refusals,
 and a run of them together through Decoder and the mesher."""
 import ctypes as C
+import math
 import os
 import re
 import subprocess
@@ -503,6 +504,31 @@ def test_large_offsets():
     assert torch.equal(label[rows], (x[rows].double() @ w.double().t()).argmax(1))
     label[rows] = 0
     assert not label.any()
+
+
+@gpu
+def test_more_rows_than_threads_of_one_launch():
+    """2^28 + 100 rows: a thread for every 16th of a row would be more than 2^32."""
+    m, k, n = (1 << 28) + 100, 1, 65
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    w = (torch.arange(n, device="cuda") / 32)[:, None].to(torch.bfloat16)
+    rows = torch.tensor([0, 1, 77, (1 << 25) + 3, (1 << 27) + 5, 1 << 28, m - 1], device="cuda")
+    x[rows] = 1.0
+    label, log_prob = linear_label(x, w)
+    assert (label[rows] == n - 1).all()
+    lp = torch.log_softmax(w.double()[:, 0], 0)[-1]
+    assert (log_prob[rows].double() - lp).abs().max() <= (ref.gamma(n) + 16 * ref.U) * lp.abs()
+    label[rows] = 0
+    assert not label.any()  # all zeros: the lowest class
+    log_prob[rows] = log_prob[2].item()
+    assert (log_prob == log_prob[2]).all() and abs(log_prob[2].item() + math.log(n)) <= 32 * ref.U * math.log(n)
+    del label, log_prob
+    target = torch.zeros(m, dtype=torch.int64, device="cuda")
+    loss = linear_cross_entropy(x, w, None, target, reduction="none")
+    zero = math.log(n)
+    assert (loss[rows].double() + torch.log_softmax(w.double()[:, 0], 0)[0]).abs().max() <= (ref.gamma(n) + 32 * ref.U) * 5
+    loss[rows] = loss[2].item()
+    assert (loss == loss[2]).all() and abs(loss[2].item() - zero) <= 32 * ref.U * zero
 
 
 def head_config():
