@@ -50,7 +50,10 @@ class _LinearCrossEntropy(torch.autograd.Function):
         loss = torch.empty(target.shape if reduction == 0 else (), dtype=torch.float32, device=dev)
         args = linear.CeArgs(x2.data_ptr(), w.data_ptr(), _lib.ptr(b), t.data_ptr(), None, loss.data_ptr(), None, None, None, None, ldx, ldw,
                              rows, ignore_index, k, n, linear.DTYPES[x.dtype], reduction)
-        saved = torch.empty(linear.load().clid_ce_saved(args), dtype=torch.uint8, device=dev)
+        need = linear.load().clid_ce_saved(args)
+        if need < 0:
+            _lib.check(int(need), "clid_ce_saved")
+        saved = torch.empty(need, dtype=torch.uint8, device=dev)
         args.saved = saved.data_ptr()
         if rows or reduction:
             linear.call("clid_ce_fwd", "clid_ce_workspace", args, dev)
@@ -99,4 +102,7 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index: int = -100, redu
         raise RuntimeError(f"linear_cross_entropy: target must be int64 or int32 on {x.device}")
     if target.shape != x.shape[:-1]:
         raise RuntimeError(f"linear_cross_entropy: target must have shape {tuple(x.shape[:-1])}, got {tuple(target.shape)}")
-    return _LinearCrossEntropy.apply(x, weight, bias, target, int(ignore_index), linear.REDUCTIONS[reduction])
+    ignore_index = int(ignore_index)
+    if not -(1 << 63) <= ignore_index < 1 << 63:
+        raise RuntimeError(f"linear_cross_entropy: ignore_index must be an int64, got {ignore_index}")
+    return _LinearCrossEntropy.apply(x, weight, bias, target, ignore_index, linear.REDUCTIONS[reduction])

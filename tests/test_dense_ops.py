@@ -402,6 +402,18 @@ def test_refusals_on_the_gpu():
 
 
 @gpu
+def test_sizes_and_numbers_out_of_range_are_refused():
+    x, w = torch.zeros(2, 1 << 20, device="cuda"), torch.zeros(3, 1 << 20, device="cuda")
+    t = torch.zeros(2, dtype=torch.int64, device="cuda")
+    for f in (lambda: linear_act(x, w), lambda: linear_label(x, w), lambda: linear_cross_entropy(x, w, None, t)):
+        with pytest.raises(RuntimeError, match="bad argument"):
+            f()
+    for index in (1 << 63, -(1 << 63) - 1, (1 << 64) - 1):
+        with pytest.raises(RuntimeError, match="ignore_index"):
+            linear_cross_entropy(x[:, :8], w[:, :8], None, t, ignore_index=index)
+
+
+@gpu
 @pytest.mark.parametrize("op", ["linear", "cross_entropy"])
 def test_gradients_against_differences(op):
     """The directional derivative against (f(+h) - f(-h)) / 2h in fp32: its truncation is h^2 / 6 times the third derivative along
