@@ -23,7 +23,7 @@ enum class Do { Linear, LinearBwd, Ce, CeBwd, Label };
 struct Narrow {
   const void *x, *w, *bias;
   int64_t ldx, ldw, rows;
-  int k, n, x_wide;
+  int k, n, x_wide, work;  // work: waves of a block that take rows; the others help with w and with the sums
   // Linear, LinearBwd
   const void *res, *dy, *z_in;
   void *y, *z_out;
@@ -83,6 +83,18 @@ struct Rows32 {
   }
 };
 
+// f with the activation as a constant of its type: one branch where many values have the same
+template <class F>
+__device__ __forceinline__ void by_act(int act, const F& f) {
+  switch (act) {
+    case CLID_ACT_RELU: return f(std::integral_constant<int, CLID_ACT_RELU>{});
+    case CLID_ACT_LEAKY_RELU: return f(std::integral_constant<int, CLID_ACT_LEAKY_RELU>{});
+    case CLID_ACT_GELU: return f(std::integral_constant<int, CLID_ACT_GELU>{});
+    case CLID_ACT_SILU: return f(std::integral_constant<int, CLID_ACT_SILU>{});
+    default: return;
+  }
+}
+
 // TN: 32 columns of z each; KQ: runs of 8 along k
 template <typename T, int TN, int KQ, Do DO>
 struct NarrowShape {
@@ -92,23 +104,26 @@ struct NarrowShape {
   static constexpr int kChunks = 8 * KQ / kChunkElems;             // of an x row in LDS: 2, 4, 8 or 16
   static constexpr int kTK = (8 * KQ + 31) / 32;
   static constexpr int kXLoads = 32 * kChunks * 16 / 1024;
-  // 32 rows; the same place then holds 32 rows of fp32 results on their way out (y, dx)
-  static constexpr int kOutT = DO == Do::Linear ? TN : kBwd ? kTK : 0;
-  static constexpr int kXBuf = max_of(32 * kChunks * 16, 32 * kOutT * 128);
-  static constexpr int kMostWaves = kBwd ? 4 : 8;
+  // 32 rows; the same place then holds 32 rows of y on their way out
+  static constexpr int kXBuf = max_of(32 * kChunks * 16, DO == Do::Linear ? 32 * TN * 128 : 0);
+  // Backward passes have one place for x (the next rows' copy starts when dw has read these, and runs under dx), so that 8 waves fit a CU and one
+  // multiplies while another waits.  1048576 x 64 -> 64 fp32, forward and backward: cross entropy 523 us with 4 waves and two places, 415 this
+  // way, a layer with gelu 639 and 440.
+  static constexpr int kXBufs = kBwd ? 1 : 2;
+  static constexpr int kMostWaves = 8;
   static constexpr int kWRow = 8 * KQ + 4;                         // floats
   static constexpr int kWBytes = 32 * TN * kWRow * 4;
-  static constexpr int kZBytes = kBwd ? 32 * 32 * TN * 4 : 0;
-  static constexpr int kWave = 2 * kXBuf + kZBytes;
+  static constexpr int kZBytes = kBwd ? 32 * 32 * max_of(TN, kTK) * 4 : 0;  // dz, then dx on its way out
+  static constexpr int kWave = kXBufs * kXBuf + kZBytes;
   static constexpr int kHead = kWBytes + 32 * TN * 4;
   static constexpr int kSumRow = 32 * kTK + 1, kSums = 32 * TN * kSumRow + 32 * TN;  // a wave's sums for dw and db, floats
-  static constexpr int lds(int waves) { return max_of(kHead + waves * kWave, kBwd ? waves * kSums * 4 : waves * 16); }
+  static constexpr int lds(int work) { return max_of(kHead + work * kWave, kBwd ? work * kSums * 4 : kMostWaves * 16); }
   // 16 chunks span the banks once: the rows between them are told apart by the chunk's place
   static __device__ __forceinline__ int place(int row, int c) { return c ^ ((row / (16 / kChunks)) & (kChunks - 1)); }
 };
 
 template <typename T, int TN, int KQ, Do DO>
-__global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ? 4 : 8)) k_narrow(Narrow a) {
+__global__ void __launch_bounds__(512) k_narrow(Narrow a) {
   using S = NarrowShape<T, TN, KQ, DO>;
   constexpr int TK = S::kTK;
   extern __shared__ __align__(16) char lds[];
@@ -117,7 +132,7 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int waves = blockDim.x >> 6;
   char* xbuf = lds + S::kHead + wave * S::kWave;
-  float* zbuf = (float*)(xbuf + 2 * S::kXBuf);
+  float* zbuf = (float*)(xbuf + S::kXBufs * S::kXBuf);
   const T* x = (const T*)a.x;
 
   // copies' offsets, the same for every 32 rows
@@ -147,8 +162,8 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     }
   };
 
-  const int64_t strips = (a.rows + 31) / 32, step = (int64_t)gridDim.x * waves;
-  int64_t strip = (int64_t)blockIdx.x * waves + wave;
+  const int64_t strips = (a.rows + 31) / 32, step = (int64_t)gridDim.x * a.work;
+  int64_t strip = wave < a.work ? (int64_t)blockIdx.x * a.work + wave : strips;
   if (a.x_wide && strip < strips) fetch(strip * 32, xbuf);
 #pragma unroll 4
   for (int e = threadIdx.x; e < 32 * TN * KQ; e += blockDim.x) {  // 8 values each
@@ -162,27 +177,32 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
   __syncthreads();
 
   f32x16 sum_w[S::kBwd ? TN : 1][S::kBwd ? TK : 1];
-  float sum_b[S::kBwd ? TN : 1][16];
+  float sum_b[TN];  // column 32 i + lane % 32, every other row
   if constexpr (S::kBwd) {
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+    for (int i = 0; i < TN; ++i) {
+      sum_b[i] = 0.f;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        sum_b[i][r] = 0.f;
+      for (int r = 0; r < 16; ++r)
 #pragma unroll
         for (int t = 0; t < TK; ++t) sum_w[i][t][r] = 0.f;
-      }
+    }
   }
   double loss_sum = 0.0;
   int counted = 0;
 
   for (int turn = 0; strip < strips; strip += step, turn ^= 1) {
-    char* xs = xbuf + turn * S::kXBuf;
+    // Backward passes: LDS addresses are made anew each turn.  Kept from one turn to the next, as the compiler would, they take 100 registers and
+    // other values are spilled for them.
+    int here = threadIdx.x & 63;
+    if constexpr (S::kBwd) asm volatile("" : "+v"(here));
+    const int lane = here, col = lane & 31, half = lane >> 5;
+    char* xs = S::kXBufs == 2 ? xbuf + turn * S::kXBuf : xbuf;
     const int64_t m0 = strip * 32, m = m0 + col;
     const bool on = m < a.rows;
     if (!a.x_wide) fetch(m0, xs);
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // these rows' copies; no read of them moves above it
-    if (a.x_wide && strip + step < strips) fetch((strip + step) * 32, xbuf + (turn ^ 1) * S::kXBuf);
+    if (S::kXBufs == 2 && a.x_wide && strip + step < strips) fetch((strip + step) * 32, xbuf + (turn ^ 1) * S::kXBuf);
 
     auto x4 = [&](int q, float (&v)[4]) {  // x[m][8 q + 4 half ..]
       const int k = 8 * q + 4 * half;
@@ -306,19 +326,32 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     if constexpr (S::kBwd) {
       // z becomes dz
       if constexpr (DO == Do::LinearBwd) {
-        Rows32<TN>::each8(zbuf, lane, [&](int row, int c, float (&v)[8], float* lo, float* hi) {
-          const int count = m0 + row < a.rows ? a.n - c : 0;
-          get8((const T*)a.dy + (m0 + row) * a.lddy + c, v, count);
-          if (a.z_in) {
-            float y[8];
-            if (a.z_is_y) get8((const T*)a.z_in + (m0 + row) * a.n + c, y, count);
-            else get8((const typename KeptZ<T>::Z*)a.z_in + (m0 + row) * a.n + c, y, count);
+        // all loads first
+        constexpr int kEach = 2 * TN;
+        const int c = lane % (4 * TN) * 8;
+        float v[kEach][8], y[kEach][8];
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = q < count ? v[q] * act_slope(y[q], a.act) : 0.f;
-          }
-          *(float4*)lo = *(const float4*)v;
-          *(float4*)hi = *(const float4*)(v + 4);
+        for (int e = 0; e < kEach; ++e) {
+          const int64_t at = m0 + lane / (4 * TN) + e * (16 / TN);
+          const int count = at < a.rows ? a.n - c : 0;
+          get8((const T*)a.dy + at * a.lddy + c, v[e], count);
+          if (!a.z_in) continue;
+          if (a.z_is_y) get8((const T*)a.z_in + at * a.n + c, y[e], count);
+          else get8((const typename KeptZ<T>::Z*)a.z_in + at * a.n + c, y[e], count);
+        }
+        if (a.z_in) by_act(a.act, [&](auto act) {
+#pragma unroll
+          for (int e = 0; e < kEach; ++e)
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+              v[e][q] = m0 + lane / (4 * TN) + e * (16 / TN) < a.rows && c + q < a.n ? v[e][q] * act_slope(y[e][q], act) : 0.f;
         });
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) {
+          const int row = lane / (4 * TN) + e * (16 / TN);
+          *(float4*)Rows32<TN>::chunk(zbuf, row, c / 4) = *(const float4*)v[e];
+          *(float4*)Rows32<TN>::chunk(zbuf, row, c / 4 + 1) = *(const float4*)(v[e] + 4);
+        }
         __builtin_amdgcn_wave_barrier();
         Rows32<TN>::get(zbuf, z, lane);
       } else {
@@ -334,32 +367,35 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
             z[i][r] = counts && n < a.n ? (n == target ? hit : p) : 0.f;
           }
       }
-#pragma unroll
-      for (int i = 0; i < TN; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum_b[i][r] += z[i][r];
       if constexpr (DO == Do::CeBwd) Rows32<TN>::put(zbuf, z, lane);
       __builtin_amdgcn_wave_barrier();
       // rows that do not count are zeros whatever they hold
       const uint32_t live = DO == Do::CeBwd ? (uint32_t)__ballot(counts) : 0xffffffffu;
-      if (a.want_w) {
 #pragma unroll
-        for (int s = 0; s < 16; ++s) {
-          const int mm = 2 * s + half;
-          float xv[TK];
+      for (int s = 0; s < 16; ++s) {
+        const int mm = 2 * s + half;
+        float zv[TN];
 #pragma unroll
-          for (int t = 0; t < TK; ++t) {
-            const int k = 32 * t + col;
-            xv[t] = 0.f;
-            if ((8 * KQ >= 32 || k < 8 * KQ) && (live >> mm & 1)) xv[t] = up(((const T*)(xs + (mm * S::kChunks + S::place(mm, k / S::kChunkElems)) * 16))[k % S::kChunkElems]);
-          }
-#pragma unroll
-          for (int i = 0; i < TN; ++i) {
-            const float zv = Rows32<TN>::chunk(zbuf, mm, 8 * i + (col >> 2))[col & 3];
-#pragma unroll
-            for (int t = 0; t < TK; ++t) sum_w[i][t] = mfma_f32(zv, xv[t], sum_w[i][t]);
-          }
+        for (int i = 0; i < TN; ++i) {
+          zv[i] = Rows32<TN>::chunk(zbuf, mm, 8 * i + (col >> 2))[col & 3];
+          sum_b[i] += zv[i];
         }
+        if (!a.want_w) continue;
+        float xv[TK];
+#pragma unroll
+        for (int t = 0; t < TK; ++t) {
+          const int k = 32 * t + col;
+          xv[t] = 0.f;
+          if ((8 * KQ >= 32 || k < 8 * KQ) && (live >> mm & 1)) xv[t] = up(((const T*)(xs + (mm * S::kChunks + S::place(mm, k / S::kChunkElems)) * 16))[k % S::kChunkElems]);
+        }
+#pragma unroll
+        for (int i = 0; i < TN; ++i)
+#pragma unroll
+          for (int t = 0; t < TK; ++t) sum_w[i][t] = mfma_f32(zv[i], xv[t], sum_w[i][t]);
+      }
+      if (a.x_wide && strip + step < strips) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // nothing reads these rows any more
+        fetch((strip + step) * 32, xs);
       }
       if (a.dx) {
         f32x16 d[TK];
@@ -379,10 +415,9 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
             }
           }
         __builtin_amdgcn_wave_barrier();
-        float* tile = (float*)xs;  // x is done with
-        Rows32<TK>::put(tile, d, lane);
+        Rows32<TK>::put(zbuf, d, lane);  // dw is done with dz
         __builtin_amdgcn_wave_barrier();
-        Rows32<TK>::each8(tile, lane, [&](int row, int c, float (&v)[8], float*, float*) {
+        Rows32<TK>::each8(zbuf, lane, [&](int row, int c, float (&v)[8], float*, float*) {
           if (m0 + row >= a.rows) return;
           const bool zero = DO == Do::CeBwd && !(live >> row & 1);
           T t[8];
@@ -418,27 +453,31 @@ __global__ void __launch_bounds__(64 * (DO == Do::LinearBwd || DO == Do::CeBwd ?
     __syncthreads();
     constexpr int kRow = S::kSumRow, kMine = S::kSums;
     float* mine = (float*)lds + wave * kMine;
+    if (wave < a.work)
 #pragma unroll
-    for (int i = 0; i < TN; ++i)
+      for (int i = 0; i < TN; ++i) {
+        const float b = sum_b[i] + __shfl_xor(sum_b[i], 32, 64);
+        if (half == 0) mine[32 * TN * kRow + 32 * i + col] = b;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int n = 32 * i + 8 * (r >> 2) + 4 * half + (r & 3);
-        float b = sum_b[i][r];
-        for (int d = 16; d; d >>= 1) b += __shfl_xor(b, d, 64);  // over the 32 rows
-        if (col == 0) mine[32 * TN * kRow + n] = b;
+        for (int r = 0; r < 16; ++r)
 #pragma unroll
-        for (int t = 0; t < TK; ++t) mine[n * kRow + 32 * t + col] = sum_w[i][t][r];
+          for (int t = 0; t < TK; ++t) mine[(32 * i + 8 * (r >> 2) + 4 * half + (r & 3)) * kRow + 32 * t + col] = sum_w[i][t][r];
       }
     __syncthreads();
     const float* all = (const float*)lds;
-    const int nk = a.n * a.k;
-    float* out = a.part + (int64_t)blockIdx.x * (nk + a.n);
-    for (int e = threadIdx.x; e < nk + a.n; e += blockDim.x) {
-      const int from = e < nk ? e / a.k * kRow + e % a.k : 32 * TN * kRow + (e - nk);
+    float* out = a.part + (int64_t)blockIdx.x * (a.n * a.k + a.n);
+    const auto total = [&](int from) {
       float t = 0.f;
-      for (int i = 0; i < waves; ++i) t += all[i * kMine + from];
-      out[e] = t;
-    }
+      for (int i = 0; i < a.work; ++i) t += all[i * kMine + from];
+      return t;
+    };
+    if (a.want_w)
+#pragma unroll 4
+      for (int e = threadIdx.x; e < a.n * 32 * TK; e += blockDim.x) {
+        const int n = e / (32 * TK), k = e % (32 * TK);
+        if (k < a.k) out[n * a.k + k] = total(n * kRow + k);
+      }
+    for (int n = threadIdx.x; n < a.n; n += blockDim.x) out[a.n * a.k + n] = total(32 * TN * kRow + n);
   }
 }
 
@@ -448,7 +487,7 @@ __global__ void __launch_bounds__(1024) k_narrow_join(const float* part, int blo
   __shared__ float p[16][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6, all = nk + n;
   float s = 0.f;
-  if (c < all)
+  if (c < nk ? dw != nullptr : c < all)  // (without dw nothing was left of it)
 #pragma unroll 8
     for (int b = g; b < blocks; b += 16) s += part[(int64_t)b * all + c];
   p[g][threadIdx.x & 63] = s;
@@ -486,11 +525,12 @@ __global__ void __launch_bounds__(256) k_narrow_total(const double* sums, int bl
   if (reduction == CLID_REDUCE_SUM) loss_out[0] = (float)s;
 }
 
-// 32 rows a wave and turn.  As many blocks as CUs (two or more a CU where few waves fit one): a block's copy of w serves all its turns,
+// 32 rows a wave and turn.  Where there is at most one block a CU it has all 8 waves, however few take rows: the others help to bring w and to add
+// up (1000 x 64 -> 64 fp32, layer and gradients: 24 us, 44 without that and with divisions in the sums' last loop).  As many blocks as CUs (two or more a CU where few waves fit one): a block's copy of w serves all its turns,
 // and no second round of blocks waits behind the first.  Of the waves a block may have, as many as leave the busiest CU the fewest turns:
 // 98304 rows of 64 -> 64 fp32 take two turns of 6 waves (8 waves: half the CUs two turns, the others one).
 struct NarrowGrid {
-  int waves, blocks;
+  int work, waves, blocks;  // waves of a block that take rows, all of them
 };
 template <class S>
 NarrowGrid narrow_grid(int64_t rows) {
@@ -510,16 +550,18 @@ NarrowGrid narrow_grid(int64_t rows) {
   if (fit > 8 / waves) fit = 8 / waves;  // 8 waves a CU
   if (fit < 1) fit = 1;
   const int64_t most = (int64_t)kCus * fit;
-  return {waves, (int)(b < most ? b : most)};
+  const int blocks = (int)(b < most ? b : most);
+  return {waves, blocks <= kCus ? S::kMostWaves : waves, blocks};
 }
 
 template <typename T, int TN, int KQ, Do DO>
-int narrow_launch(const Narrow& a, hipStream_t s) {
+int narrow_launch(Narrow a, hipStream_t s) {
   using S = NarrowShape<T, TN, KQ, DO>;
   static_assert(S::lds(S::kMostWaves) <= 160 * 1024, "a block fits a CU");
   const NarrowGrid g = narrow_grid<S>(a.rows);
   auto k = k_narrow<T, TN, KQ, DO>;
-  const int lds = S::lds(g.waves), rc = allow_lds((const void*)k, S::lds(S::kMostWaves));
+  a.work = g.work;
+  const int lds = S::lds(g.work), rc = allow_lds((const void*)k, S::lds(S::kMostWaves));
   if (rc != CLID_OK) return rc;
   hipLaunchKernelGGL(k, dim3(g.blocks), dim3(64 * g.waves), lds, s, a);
   return g.blocks;
