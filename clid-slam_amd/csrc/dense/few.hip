@@ -302,6 +302,28 @@ __global__ void __launch_bounds__(256) k_few_dz(Few a, const T* bias, const int6
   }
 }
 
+// a layer's: dz = dy act'(z)
+template <int MT>
+__global__ void __launch_bounds__(256) k_few_linear_dz(const float* dy, int64_t lddy, const float* z, int rows, int64_t n, int act, float* dz, int64_t np, float* db) {
+  __shared__ float sums[4][64];
+  const int c = threadIdx.x & 63, group = threadIdx.x >> 6;
+  const int64_t col = (int64_t)blockIdx.x * 64 + c;
+  float all = 0.f;
+#pragma unroll
+  for (int m = group; m < 16 * MT; m += 4) {
+    float v = 0.f;
+    if (m < rows && col < n) {
+      v = dy[m * lddy + col];
+      if (z) v *= act_slope(z[m * n + col], act);
+    }
+    dz[m * np + col] = v;
+    all += v;
+  }
+  sums[group][c] = all;
+  __syncthreads();
+  if (db && group == 0 && col < n) db[col] = all + sums[1][c] + sums[2][c] + sums[3][c];
+}
+
 // dx: block (128 columns of k, share of n) -> part[share][16 MT][k up to 128].  Lane l: 8 neighbouring columns 8 (l % 16) of row 4 (l / 16) + c of 16
 // rows of w, c = 0 .. 3; instruction j takes column j of the eight.
 template <typename T, int MT>
@@ -362,7 +384,7 @@ __global__ void __launch_bounds__(256) k_few_dx_join(const float* part, int shar
   float s = 0.f;
 #pragma unroll 8
   for (int i = 0; i < shares; ++i) s += part[((int64_t)i * rows16 + m) * kp + c];
-  dx[e] = down<T>(target[m] == ignore ? 0.f : s);
+  dx[e] = down<T>(target && target[m] == ignore ? 0.f : s);
 }
 
 // dw: a wave holds its 128 columns of x and walks 16 rows of dw at a time
@@ -374,7 +396,7 @@ __global__ void __launch_bounds__(256) k_few_dw(Few a, const int64_t* target, in
 #pragma unroll
   for (int s = 0; s < 4 * MT; ++s) {
     const int m = 4 * s + q;
-    const bool on = m < a.m && target[m] != ignore;  // a row that does not count is zeros whatever it holds
+    const bool on = m < a.m && !(target && target[m] == ignore);  // a row that does not count is zeros whatever it holds
     get8((const T*)a.x + (int64_t)m * a.ldx + k0, x[s], on ? count : 0);
   }
   for (int64_t v = ((int64_t)blockIdx.y * 4 + wave) * 16; v < np; v += (int64_t)gridDim.y * 64) {
@@ -419,45 +441,70 @@ struct FewBwd {
   int mt, shares;
   char *dz, *part;
   int64_t bytes;
-  explicit FewBwd(const clid_ce_args* a) {
-    Ws ws(a->ws);
-    np = (a->n + 63) / 64 * 64;
-    kp = (a->k + 127) / 128 * 128;
-    mt = a->rows <= 16 ? 1 : 2;
+  FewBwd(void* base, int64_t rows, int32_t k, int32_t n, bool dx) {
+    Ws ws(base);
+    np = ((int64_t)n + 63) / 64 * 64;
+    kp = ((int64_t)k + 127) / 128 * 128;
+    mt = rows <= 16 ? 1 : 2;
     // blocks of 128 columns of k and of shares of n: about 4 a CU, a share 256 rows of w at least
     int64_t want = 4 * kCus / (kp / 128), most = (np + 255) / 256;
     shares = (int)(want < 1 ? 1 : want < most ? want : most);
     per = ((np + shares - 1) / shares + 63) / 64 * 64;
     shares = (int)((np + per - 1) / per);
     dz = ws.take(16 * mt * np * 4);
-    part = ws.take(a->dx ? (int64_t)shares * 16 * mt * kp * 4 : 0);
+    part = ws.take(dx ? (int64_t)shares * 16 * mt * kp * 4 : 0);
     bytes = ws.used;
   }
 };
-int64_t few_ce_bwd_bytes(const clid_ce_args* a) { return FewBwd(a).bytes; }
+// dx and dw of the dz in the workspace; target NULL: every row counts
 template <typename T, int MT>
-static void few_bwd_launch(const clid_ce_args* a, const FewBwd& b, const float4* stat, const float* total, hipStream_t s) {
-  const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
-  float* dz = (float*)b.dz;
+static void few_products(const Few& f, const FewBwd& b, const int64_t* target, int64_t ignore, void* dx, void* dw, hipStream_t s) {
+  const float* dz = (const float*)b.dz;
   const unsigned kb = (unsigned)(b.kp / 128);
-  hipLaunchKernelGGL((k_few_dz<T, MT, 4>), dim3((unsigned)(b.np / 64)), dim3(256), 4 * MT * 64 * kFewRow * 4, s, f, (const T*)a->bias, a->target, a->ignore_index, stat,
-                     a->g, a->reduction, total, dz, b.np, (T*)a->db);
-  if (a->dx) {
-    hipLaunchKernelGGL((k_few_dx<T, MT>), dim3(kb, (unsigned)b.shares), dim3(256), 0, s, f, (const float*)dz, b.np, b.per, (float*)b.part);
-    hipLaunchKernelGGL(k_few_dx_join<T>, dim3((unsigned)((a->rows * a->k + 255) / 256)), dim3(256), 0, s, (const float*)b.part, b.shares, 16 * MT, b.kp, (int)a->rows, a->k,
-                       a->target, a->ignore_index, (T*)a->dx);
+  if (dx) {
+    hipLaunchKernelGGL((k_few_dx<T, MT>), dim3(kb, (unsigned)b.shares), dim3(256), 0, s, f, dz, b.np, b.per, (float*)b.part);
+    hipLaunchKernelGGL(k_few_dx_join<T>, dim3((unsigned)(((int64_t)f.m * f.k + 255) / 256)), dim3(256), 0, s, (const float*)b.part, b.shares, 16 * MT, b.kp, f.m, f.k, target,
+                       ignore, (T*)dx);
   }
-  if (a->dw) {
+  if (dw) {
     const int64_t tiles = b.np / 64, want = 8 * kCus / kb + 1;
-    hipLaunchKernelGGL((k_few_dw<T, MT>), dim3(kb, (unsigned)(tiles < want ? tiles : want)), dim3(256), 0, s, f, a->target, a->ignore_index, (const float*)dz, b.np, (T*)a->dw);
+    hipLaunchKernelGGL((k_few_dw<T, MT>), dim3(kb, (unsigned)(tiles < want ? tiles : want)), dim3(256), 0, s, f, target, ignore, dz, b.np, (T*)dw);
   }
 }
+
+int64_t few_ce_bwd_bytes(const clid_ce_args* a) { return FewBwd(nullptr, a->rows, a->k, a->n, a->dx).bytes; }
+template <typename T, int MT>
+static void few_ce_bwd_launch(const clid_ce_args* a, const FewBwd& b, const float4* stat, const float* total, hipStream_t s) {
+  const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
+  hipLaunchKernelGGL((k_few_dz<T, MT, 4>), dim3((unsigned)(b.np / 64)), dim3(256), 4 * MT * 64 * kFewRow * 4, s, f, (const T*)a->bias, a->target, a->ignore_index, stat,
+                     a->g, a->reduction, total, (float*)b.dz, b.np, (T*)a->db);
+  few_products<T, MT>(f, b, a->target, a->ignore_index, a->dx, a->dw, s);
+}
 int few_ce_bwd(const clid_ce_args* a, const float4* stat, const float* total, hipStream_t s) {
-  const FewBwd b(a);
+  const FewBwd b(a->ws, a->rows, a->k, a->n, a->dx);
   BY_DTYPE(a->dtype, {
-    if (b.mt == 1) few_bwd_launch<T, 1>(a, b, stat, total, s);
-    else few_bwd_launch<T, 2>(a, b, stat, total, s);
+    if (b.mt == 1) few_ce_bwd_launch<T, 1>(a, b, stat, total, s);
+    else few_ce_bwd_launch<T, 2>(a, b, stat, total, s);
   });
+  return CLID_OK;
+}
+
+// A layer's backward pass, fp32 only: the tiles' planes of w cost more than the products (layer and gradients, gelu, 1 and 32 rows: 4096 -> 8192 in tiles
+// 196 and 218 us, here 83 and 133; 1024 -> 1000: 31 and 39, 22 and 31).  16-bit operands go to the tiles as they lie (bf16 4096 -> 8192: tiles 58
+// and 72 us, here 62 and 118).
+int64_t few_linear_bwd_bytes(const clid_linear_bwd_args* a) { return FewBwd(nullptr, a->rows, a->k, a->n, a->dx).bytes; }
+template <int MT>
+static void few_linear_bwd_launch(const clid_linear_bwd_args* a, const FewBwd& b, hipStream_t s) {
+  const Few f = {a->x, a->w, a->ldx, a->ldw, (int)a->rows, a->k, a->n};
+  // z and y are both fp32: z_is_y makes no difference
+  hipLaunchKernelGGL((k_few_linear_dz<MT>), dim3((unsigned)(b.np / 64)), dim3(256), 0, s, (const float*)a->dy, a->lddy, a->act == CLID_ACT_NONE ? nullptr : (const float*)a->z,
+                     (int)a->rows, a->n, a->act, (float*)b.dz, b.np, (float*)a->db);
+  few_products<float, MT>(f, b, nullptr, 0, a->dx, a->dw, s);
+}
+int few_linear_bwd(const clid_linear_bwd_args* a, hipStream_t s) {
+  const FewBwd b(a->ws, a->rows, a->k, a->n, a->dx);
+  if (b.mt == 1) few_linear_bwd_launch<1>(a, b, s);
+  else few_linear_bwd_launch<2>(a, b, s);
   return CLID_OK;
 }
 

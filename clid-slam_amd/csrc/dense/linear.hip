@@ -114,6 +114,7 @@ extern "C" int clid_linear_fwd(const clid_linear_args* a, void* stream) {
 extern "C" int64_t clid_linear_bwd_workspace(const clid_linear_bwd_args* a) {
   if (!args_ok(a)) return bad("clid_linear_bwd_workspace", "bad argument");
   if (is_narrow(a->k, a->n)) return narrow_linear_bwd_bytes(a);
+  if (a->dtype == CLID_F32 && is_few(a->rows) && a->rows) return few_linear_bwd_bytes(a);
   BY_DTYPE(a->dtype, return Bwd<T>(a).bytes;);
 }
 extern "C" int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream) {
@@ -125,6 +126,7 @@ extern "C" int clid_linear_bwd(const clid_linear_bwd_args* a, void* stream) {
   if (!ws_ok(a->ws, a->ws_bytes, need)) return bad(me, "workspace too small or not aligned to 256 bytes");
   int rc = CLID_OK;
   if (is_narrow(a->k, a->n)) rc = narrow_linear_bwd(a, (hipStream_t)stream);
+  else if (a->dtype == CLID_F32 && is_few(a->rows)) rc = few_linear_bwd(a, (hipStream_t)stream);
   else BY_DTYPE(a->dtype, rc = bwd<T>(a, (hipStream_t)stream););
   if (rc != CLID_OK) return rc;
   DENSE_CHECK_LAUNCH(me);

@@ -190,7 +190,8 @@ inline int allow_lds(const void* kernel, int bytes) {
   return CLID_OK;
 }
 
-// n, k <= 64 (narrow.hip)
+// n, k <= 64 (narrow.hip; in tiles, 64 -> 64: fp32 98304 rows 51 us against 25, layer and gradients 157 against 68, cross entropy and gradients
+// 212 against 68; bf16 35, 103, 153 against 23, 69, 69.  Only 1000 bf16 rows are as quick in tiles: 7 us against 9)
 inline bool is_narrow(int32_t k, int32_t n) { return k <= 64 && n <= 64; }
 int narrow_linear(const clid_linear_args* a, hipStream_t s);
 int64_t narrow_linear_bwd_bytes(const clid_linear_bwd_args* a);
@@ -201,9 +202,14 @@ int64_t narrow_ce_bwd_bytes(const clid_ce_args* a);
 int narrow_ce_bwd(const clid_ce_args* a, hipStream_t s);
 int narrow_label(const clid_label_args* a, hipStream_t s);
 
-// at most 32 rows (few.hip)
+// at most 32 rows (few.hip; the instruction's two column blocks.  In tiles, 4096 -> 8192 and 2048 -> 65536: fp32 one row 114 and 426 us against 25
+// and 106, 32 rows 118 and 447 against 46 and 138; bf16 one row 26 and 44 against 14 and 45, label 34 and 94 against 27 and 51; bf16 with 32 rows
+// is even or behind (26 and 46 against 26 and 59; label 33 and 94 against 37 and 65).  The cross entropy stays here for its fp32 dz also where
+// tiles are quicker: bf16 32 rows, with gradients, 113 and 322 us against 158 and 469)
 inline bool is_few(int64_t rows) { return rows <= 32; }
 int few_linear(const clid_linear_args* a, hipStream_t s);
+int64_t few_linear_bwd_bytes(const clid_linear_bwd_args* a);
+int few_linear_bwd(const clid_linear_bwd_args* a, hipStream_t s);
 int64_t few_label_bytes(const clid_label_args* a);
 int few_label(const clid_label_args* a, hipStream_t s);
 int64_t few_ce_bytes(const clid_ce_args* a);
