@@ -1,13 +1,14 @@
 // The dense operators at a point decoder's own widths, n <= 64 and k <= 64: memory bound, so x is read once and everything else happens in
 // registers.
 //
-// A wave takes 32 rows at a time; the weight lies in LDS.  z = x w^T on the fp32 matrix instruction (32 x 32 x 2) with the rows of w as its
-// row operand: a lane then holds one row m of x and of z, element (i, r) being column 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4.  A row's
-// softmax is 16 or 32 registers and one exchange between two lanes, with no partial results in memory.  The same registers are the
-// column operand of dx = dz w as they are (the contraction over n takes its columns in that order, and so does the row operand, read from
-// w in LDS).  dw = dz^T x contracts over m: dz goes through LDS once, x is there already; the sums over a wave's rows stay in
-// accumulators, a block's waves add theirs in LDS, k_narrow_join adds the blocks' in their order.  Nothing is rounded before the
-// results, whatever the type.  The cross entropy's backward pass makes z again rather than keeping anything of it.
+// A wave takes 32 rows at a time; the weight lies in LDS.  z = x w^T on the matrix instruction of x's type, with the rows of w as its row operand:
+// a lane then holds one row m of x and of z, element (i, r) being column 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4.  (32 x 32 x 2 for fp32;
+// 32 x 32 x 16 for 16 bits: 1048576 x 64 -> 64 bf16 gelu 87 us, 3.1 TB/s, label 50, and 140 and 106 by the fp32 one, whose products take 16 times
+// as long.)  A row's softmax is 16 or 32 registers and one exchange between two lanes, with no partial results in memory.  The same
+// registers are the column operand of dx = dz w as they are (fp32 instruction; the contraction over n takes its columns in that order, and so
+// does the row operand, read from w in LDS).  dw = dz^T x contracts over m: dz goes through LDS once, x is there already; the sums over a
+// wave's rows stay in accumulators, a block's waves add theirs in LDS, k_narrow_join adds the blocks' in their order.  Nothing is
+// rounded before the results, whatever the type.  The cross entropy's backward pass makes z again rather than keeping anything of it.
 //
 // x comes by 16-byte copies straight to LDS, the next 32 rows' while these are worked on; chunks are permuted within their row so that the
 // lanes' reads fall on different banks.  (By 16-byte loads to registers, each of 32 rows' 32 bytes: 1048576 x 64 -> 21 fp32 label 140 us, 77 us
@@ -111,8 +112,8 @@ struct NarrowShape {
   // way, a layer with gelu 639 and 440.
   static constexpr int kXBufs = kBwd ? 1 : 2;
   static constexpr int kMostWaves = 8;
-  static constexpr int kWRow = 8 * KQ + 4;                         // floats
-  static constexpr int kWBytes = 32 * TN * kWRow * 4;
+  static constexpr int kWRow = 8 * KQ + kChunkElems;               // elements: rows that are read together start on different banks
+  static constexpr int kWBytes = 32 * TN * kWRow * (int)sizeof(T);
   static constexpr int kZBytes = kBwd ? 32 * 32 * max_of(TN, kTK) * 4 : 0;  // dz, then dx on its way out
   static constexpr int kWave = kXBufs * kXBuf + kZBytes;
   static constexpr int kHead = kWBytes + 32 * TN * 4;
@@ -127,7 +128,7 @@ __global__ void __launch_bounds__(512) k_narrow(Narrow a) {
   using S = NarrowShape<T, TN, KQ, DO>;
   constexpr int TK = S::kTK;
   extern __shared__ __align__(16) char lds[];
-  float* w = (float*)lds;
+  T* w = (T*)lds;
   float* bias = (float*)(lds + S::kWBytes);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
   const int waves = blockDim.x >> 6;
@@ -170,8 +171,10 @@ __global__ void __launch_bounds__(512) k_narrow(Narrow a) {
     const int n = e / KQ, k = e % KQ * 8;
     float v[8];
     get8((const T*)a.w + n * a.ldw + k, v, n < a.n ? a.k - k : 0);
-    *(float4*)(w + n * S::kWRow + k) = float4{v[0], v[1], v[2], v[3]};
-    *(float4*)(w + n * S::kWRow + k + 4) = float4{v[4], v[5], v[6], v[7]};
+    struct alignas(16) Run { T t[8]; } run;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) run.t[q] = down<T>(v[q]);
+    *(Run*)(w + n * S::kWRow + k) = run;
   }
   for (int n = threadIdx.x; n < 32 * TN; n += blockDim.x) bias[n] = a.bias && n < a.n ? up(((const T*)a.bias)[n]) : 0.f;
   __syncthreads();
@@ -204,14 +207,6 @@ __global__ void __launch_bounds__(512) k_narrow(Narrow a) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // these rows' copies; no read of them moves above it
     if (S::kXBufs == 2 && a.x_wide && strip + step < strips) fetch((strip + step) * 32, xbuf + (turn ^ 1) * S::kXBuf);
 
-    auto x4 = [&](int q, float (&v)[4]) {  // x[m][8 q + 4 half ..]
-      const int k = 8 * q + 4 * half;
-      const T* p = (const T*)(xs + (col * S::kChunks + S::place(col, k / S::kChunkElems)) * 16) + k % S::kChunkElems;
-      struct alignas(4 * sizeof(T)) Run { T t[4]; };
-      const Run r = *(const Run*)p;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = up(r.t[e]);
-    };
     f32x16 z[TN];
     if constexpr (DO != Do::LinearBwd) {
 #pragma unroll
@@ -221,17 +216,25 @@ __global__ void __launch_bounds__(512) k_narrow(Narrow a) {
           const float4 b4 = *(const float4*)(bias + 32 * i + 8 * j + 4 * half);
           z[i][4 * j] = b4.x; z[i][4 * j + 1] = b4.y; z[i][4 * j + 2] = b4.z; z[i][4 * j + 3] = b4.w;
         }
+      if constexpr (sizeof(T) == 2) {
 #pragma unroll
-      for (int q = 0; q < KQ; ++q) {
-        float xv[4];
-        x4(q, xv);
+        for (int q = 0; q < KQ; q += 2) {
+          const s16x8 xv = *(const s16x8*)(xs + (col * S::kChunks + S::place(col, q + half)) * 16);
 #pragma unroll
-        for (int i = 0; i < TN; ++i) {
-          const float4 w4 = *(const float4*)(w + (32 * i + col) * S::kWRow + 8 * q + 4 * half);
-          z[i] = mfma_f32(w4.x, xv[0], z[i]);
-          z[i] = mfma_f32(w4.y, xv[1], z[i]);
-          z[i] = mfma_f32(w4.z, xv[2], z[i]);
-          z[i] = mfma_f32(w4.w, xv[3], z[i]);
+          for (int i = 0; i < TN; ++i) z[i] = mfma<Kind<T>::F16>(*(const s16x8*)(w + (32 * i + col) * S::kWRow + 8 * (q + half)), xv, z[i]);
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < KQ; ++q) {  // 8 q + 4 half ..
+          const float4 x4 = *(const float4*)(xs + (col * S::kChunks + S::place(col, 2 * q + half)) * 16);
+#pragma unroll
+          for (int i = 0; i < TN; ++i) {
+            const float4 w4 = *(const float4*)(w + (32 * i + col) * S::kWRow + 8 * q + 4 * half);
+            z[i] = mfma_f32(w4.x, x4.x, z[i]);
+            z[i] = mfma_f32(w4.y, x4.y, z[i]);
+            z[i] = mfma_f32(w4.z, x4.z, z[i]);
+            z[i] = mfma_f32(w4.w, x4.w, z[i]);
+          }
         }
       }
     }
@@ -411,7 +414,7 @@ __global__ void __launch_bounds__(512) k_narrow(Narrow a) {
 #pragma unroll
             for (int t = 0; t < TK; ++t) {
               const int k = 32 * t + col;  // a row of w is 8 KQ values: where that is 16, lanes 16 .. 31 have none
-              d[t] = mfma_f32(8 * KQ >= 32 || k < 8 * KQ ? w[n * S::kWRow + k] : 0.f, z[i][r], d[t]);
+              d[t] = mfma_f32(8 * KQ >= 32 || k < 8 * KQ ? up(w[n * S::kWRow + k]) : 0.f, z[i][r], d[t]);
             }
           }
         __builtin_amdgcn_wave_barrier();

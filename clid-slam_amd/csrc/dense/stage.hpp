@@ -190,8 +190,8 @@ inline int allow_lds(const void* kernel, int bytes) {
   return CLID_OK;
 }
 
-// n, k <= 64 (narrow.hip; in tiles, 64 -> 64: fp32 98304 rows 51 us against 25, layer and gradients 157 against 68, cross entropy and gradients
-// 212 against 68; bf16 35, 103, 153 against 23, 69, 69.  Only 1000 bf16 rows are as quick in tiles: 7 us against 9)
+// n, k <= 64 (narrow.hip; in tiles, 64 -> 64: fp32 98304 rows 51 us against 25, layer and gradients 157 against 69, cross entropy and gradients
+// 212 against 70; bf16 35, 103, 153 against 16, 64, 56.  Only 1000 bf16 rows are as quick in tiles: 7 us against 8)
 inline bool is_narrow(int32_t k, int32_t n) { return k <= 64 && n <= 64; }
 int narrow_linear(const clid_linear_args* a, hipStream_t s);
 int64_t narrow_linear_bwd_bytes(const clid_linear_bwd_args* a);
