@@ -7,6 +7,7 @@
 // The cross entropy's backward pass makes z again the same way, leaves dz in fp32 (32 rows of it are small) and takes both products on the fp32
 // matrix instruction (16 x 16 x 4), w and dw in 16 bytes a lane of 256 neighbouring ones: with few rows nothing averages a rounding of
 // dz away, and the products cost nothing beside the weight's bytes.
+// Bound by the weight's bytes: 1 x 4096 -> 8192 bf16 silu 13.5 us, label of 1 x 4096 -> 131072 bf16 215 us, both 5.0 TB/s (a large copy: 4.8).
 // Where n is large a wave takes 4 tiles at once (one read of x for four of w) and a block goes through many, keeping running softmax
 // statistics, so that a head of 131072 classes leaves one partial result per block.
 #include "stage.hpp"

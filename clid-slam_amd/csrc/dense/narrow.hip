@@ -529,7 +529,8 @@ __global__ void __launch_bounds__(256) k_narrow_total(const double* sums, int bl
 }
 
 // 32 rows a wave and turn.  Where there is at most one block a CU it has all 8 waves, however few take rows: the others help to bring w and to add
-// up (1000 x 64 -> 64 fp32, layer and gradients: 24 us, 44 without that and with divisions in the sums' last loop).  As many blocks as CUs (two or more a CU where few waves fit one): a block's copy of w serves all its turns,
+// up (1000 x 64 -> 64 fp32, layer and gradients: 24 us, 44 without that and with divisions in the sums' last loop).  As many blocks as CUs (two or
+// more a CU where few waves fit one): a block's copy of w serves all its turns,
 // and no second round of blocks waits behind the first.  Of the waves a block may have, as many as leave the busiest CU the fewest turns:
 // 98304 rows of 64 -> 64 fp32 take two turns of 6 waves (8 waves: half the CUs two turns, the others one).
 struct NarrowGrid {
