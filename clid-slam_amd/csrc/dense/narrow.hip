@@ -4,7 +4,8 @@
 // A wave takes 32 rows at a time; the weight lies in LDS.  z = x w^T on the matrix instruction of x's type, with the rows of w as its row operand:
 // a lane then holds one row m of x and of z, element (i, r) being column 32 i + 8 (r / 4) + 4 (lane / 32) + r % 4.  (32 x 32 x 2 for fp32;
 // 32 x 32 x 16 for 16 bits: 1048576 x 64 -> 64 bf16 gelu 87 us, 3.1 TB/s, label 50, and 140 and 106 by the fp32 one, whose products take 16 times
-// as long.)  A row's softmax is 16 or 32 registers and one exchange between two lanes, with no partial results in memory.  The same
+// as long.  fp32 as bf16 planes, as the tiles have it: 1048576 x 64 -> 21 label 87 us, 70 by the fp32 instruction, as splitting x costs more than the
+// products.)  A row's softmax is 16 or 32 registers and one exchange between two lanes, with no partial results in memory.  The same
 // registers are the column operand of dx = dz w as they are (fp32 instruction; the contraction over n takes its columns in that order, and so
 // does the row operand, read from w in LDS).  dw = dz^T x contracts over m: dz goes through LDS once, x is there already; the sums over a
 // wave's rows stay in accumulators, a block's waves add theirs in LDS, k_narrow_join adds the blocks' in their order.  Nothing is
