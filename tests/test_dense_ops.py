@@ -222,6 +222,36 @@ def test_large_tiles_and_cuts(shape, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape,pad", [((150003, 64, 64), 0), ((150003, 11, 64), 0), ((140001, 64, 21), 1), ((200000, 40, 33), 8)], ids=str)
+def test_many_rows_of_narrow_layers(shape, pad, dtype):
+    """More than 65536 rows: a wave takes several turns of 32, by copies to LDS and (rows that are not whole aligned chunks) through registers."""
+    m, k, n = shape
+    dt, gen = TYPES[dtype], generator(m + k)
+    x = strided(normal(gen, m, k).to(dt), pad, 0).requires_grad_()
+    w, b = (normal(gen, n, k) * k ** -0.5).to(dt).requires_grad_(), normal(gen, n).to(dt).requires_grad_()
+    dy = normal(gen, m, n).to(dt)
+    y = linear_act(x, w, b, activation="gelu")
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(y, [x, w, b], dy))) | {"y": y}
+    for name, (v, tol) in ref.linear(x, w, b, None, "gelu", dy).items():
+        ref.close(got[name], v, tol, name)
+    t = torch.randint(0, n, (m,), generator=gen, device="cuda")
+    t[::3] = -100
+    g = torch.full((), 4096.0, device="cuda")
+    loss = linear_cross_entropy(x, w, b, t)
+    got = dict(zip(("dx", "dw", "db"), torch.autograd.grad(loss, [x, w, b], g))) | {"loss": loss}
+    for name, (v, tol) in ref.cross_entropy(x, w, b, t, -100, "mean", g).items():
+        ref.close(got[name], v, tol, "cross entropy " + name)
+    label, _ = linear_label(x, w, b)
+    _, _, z, ez = ref.logits(x, w, b)
+    top = z.topk(2, dim=1)
+    clear = top.values[:, 0] - top.values[:, 1] > 2 * ez.amax(1)  # k <= 64: 2 ez is under 1e-3, and two largest of 21 and more are rarely that near
+    assert torch.equal(label[clear], top.indices[clear, 0]) and clear.float().mean() > 0.9
+    gx = torch.autograd.grad(linear_act(x, w.detach(), activation="silu"), x, dy)[0]  # dx alone
+    ref.close(gx, *ref.linear(x, w, None, None, "silu", dy)["dx"], "dx alone")
+
+
+@gpu
 @pytest.mark.parametrize("dtype,m", [("bf16", 8192), ("f16", 7000), ("f32", 4096)])
 def test_cross_entropy_in_several_pieces(dtype, m):
     """A backward pass whose dz takes more than one piece of the classes (512 MB of it)."""
