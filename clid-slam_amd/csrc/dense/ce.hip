@@ -252,7 +252,9 @@ int ce_fwd(const clid_ce_args* a, hipStream_t s) {
     if (blocks > 1) hipLaunchKernelGGL(k_count, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (int*)f.counts);
     hipLaunchKernelGGL(k_order, dim3(blocks), dim3(1024), 0, s, a->target, a->rows, a->ignore_index, (const int*)f.counts, v.order, none);
     const int32_t* live = v.order + a->rows;
-    Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, v.order, live), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), live, 0, 1, 0, 0};
+    const Staging x = staging<T>(a->x, a->ldx, a->rows, a->k, f.x, true, v.order, live), w = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
+    stage<T>(x, w, s);
+    Product g = {staged<T>(x), staged<T>(w), a->rows, a->n, up8(a->k), live, 0, 1, 0, 0};
     const int rc = launch_stat<T, false>(g, f.p.size, (const T*)a->bias, a->target, v.order, (float2*)f.part, nullptr, (float*)f.zt, s);
     if (rc != CLID_OK) return rc;
     hipLaunchKernelGGL(k_loss_rows, dim3(f.joins), dim3(512), 0, s, (const float2*)f.part, f.strips, (const float*)f.zt, a->target, v.order, a->rows, a->n,
@@ -310,8 +312,9 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
   hipLaunchKernelGGL(k_scale, dim3(1), dim3(1024), 0, s, a->g, v.total, a->rows, a->reduction, (int)Kind<T>::F16, scale);
   if (a->dx)
     hipLaunchKernelGGL(k_clear_rows<T>, dim3((unsigned)(a->rows < 2048 ? a->rows : 2048)), dim3(256), 0, s, a->target, a->rows, a->ignore_index, a->k, (T*)a->dx);
-  const Operand x = stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s, true, v.order, live);
-  const Operand w = stage<T>(a->w, a->ldw, a->n, a->k, f.w, s);
+  const Staging sx = staging<T>(a->x, a->ldx, a->rows, a->k, f.x, true, v.order, live), sw = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
+  stage<T>(sx, sw, s);
+  const Operand x = staged<T>(sx), w = staged<T>(sw);
   for (int64_t v0 = 0; v0 < a->n; v0 += f.piece) {
     const int64_t nv = a->n - v0 < f.piece ? a->n - v0 : f.piece, ld = padded<T>(nv);
     Operand wv = w;
@@ -367,7 +370,9 @@ struct Label {
 template <typename T>
 int label(const clid_label_args* a, hipStream_t s) {
   const Label<T> f(a);
-  Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
+  const Staging x = staging<T>(a->x, a->ldx, a->rows, a->k, f.x), w = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
+  stage<T>(x, w, s);
+  Product g = {staged<T>(x), staged<T>(w), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
   const int rc = launch_stat<T, true>(g, f.p.size, (const T*)a->bias, nullptr, nullptr, (float2*)f.part, (int32_t*)f.at, nullptr, s);
   if (rc != CLID_OK) return rc;
   const int64_t joins = (a->rows + 15) / 16;

@@ -24,7 +24,9 @@ struct Fwd {
 template <typename T>
 int fwd(const clid_linear_args* a, hipStream_t s) {
   const Fwd<T> f(a);
-  Product g = {stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
+  const Staging x = staging<T>(a->x, a->ldx, a->rows, a->k, f.x), w = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
+  stage<T>(x, w, s);
+  Product g = {staged<T>(x), staged<T>(w), a->rows, a->n, up8(a->k), nullptr, 0, 1, 0, 0};
   LinearOut<T> o = {(const T*)a->bias, (const T*)a->residual, (T*)a->y, (typename KeptZ<T>::Z*)a->z_out, a->ldr, a->n, a->act};
   return launch_out<T, false, false>(g, f.p, o, f.part, s);
 }
@@ -69,13 +71,17 @@ int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
     if (a->db)
       hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
   }
+  Staging x = staging<T>(a->x, a->ldx, a->rows, a->k, f.x), w = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
+  if (!a->dw) x.blocks = 0;
+  if (!a->dx) w.blocks = 0;
+  stage<T>(x, w, s);
   if (a->dx) {
-    Product g = {dz, stage<T>(a->w, a->ldw, a->n, a->k, f.w, s), a->rows, a->k, a->n, nullptr, 0, 1, 0, 0};
+    Product g = {dz, staged<T>(w), a->rows, a->k, a->n, nullptr, 0, 1, 0, 0};
     const int rc = launch_out<T, false, true>(g, f.px, StoreOut<T>{nullptr, (T*)a->dx, nullptr, nullptr, nullptr, a->k}, f.part, s);
     if (rc != CLID_OK) return rc;
   }
   if (a->dw) {
-    Product g = {dz, stage<T>(a->x, a->ldx, a->rows, a->k, f.x, s), a->n, a->k, a->rows, nullptr, 0, 1, 0, 0};
+    Product g = {dz, staged<T>(x), a->n, a->k, a->rows, nullptr, 0, 1, 0, 0};
     return launch_out<T, true, true>(g, f.pw, StoreOut<T>{nullptr, (T*)a->dw, nullptr, nullptr, nullptr, a->k}, f.part, s);
   }
   return CLID_OK;
