@@ -143,9 +143,19 @@ __global__ void __launch_bounds__(256) k_label_join(const float2* part, const in
 
 // scale[0]: what dz is multiplied by as it is stored, scale[1]: what its products are multiplied by.  mean and sum: the one factor
 // belongs to the products, and fp16's dz = p - onehot is stored times 2^10 so that small p keep their bits (|dz| <= 1).  none: the
-// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10.
-__global__ void __launch_bounds__(1024) k_scale(const float* g, const float* total, int64_t rows, int reduction, int half, float* scale) {
+// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10.  All blocks but the first: zeros for the
+// rows of dx that do not count (one launch for both: 333 x 300 -> 200 fp32 loss and gradients 60.8 -> 58.9 us).
+template <typename T>
+__global__ void __launch_bounds__(1024) k_scale(const float* g, const float* total, int64_t rows, int reduction, float* scale, const int64_t* target, int64_t ignore,
+                                                int k, T* dx) {
   __shared__ float ps[16];
+  constexpr bool half = Kind<T>::F16;
+  if (blockIdx.x) {
+    for (int64_t m = (int64_t)(blockIdx.x - 1) * 4 + (threadIdx.x >> 8); m < rows; m += (int64_t)(gridDim.x - 1) * 4)
+      if (target[m] == ignore)
+        for (int c = threadIdx.x & 255; c < k; c += 256) dx[m * k + c] = down<T>(0.f);
+    return;
+  }
   if (reduction != CLID_REDUCE_NONE) {
     if (threadIdx.x == 0) {
       const float f = half ? 1024.f : 1.f;
@@ -170,14 +180,6 @@ __global__ void __launch_bounds__(1024) k_scale(const float* g, const float* tot
   const int by = half && top > 0.f ? (10 - e > 100 ? 100 : 10 - e < -100 ? -100 : 10 - e) : 0;
   scale[0] = ldexpf(1.f, by);
   scale[1] = ldexpf(1.f, -by);
-}
-
-// gradients of the rows that do not count
-template <typename T>
-__global__ void __launch_bounds__(256) k_clear_rows(const int64_t* target, int64_t rows, int64_t ignore, int k, T* dx) {
-  for (int64_t m = blockIdx.x; m < rows; m += gridDim.x)
-    if (target[m] == ignore)
-      for (int c = threadIdx.x; c < k; c += 256) dx[m * k + c] = down<T>(0.f);
 }
 
 template <typename T, int SIZE> constexpr int strip_of() { return Tile<Kind<T>::NP, SIZE>::BN / Tile<Kind<T>::NP, SIZE>::WN; }
@@ -309,9 +311,9 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
   const Saved v(a);
   const int32_t* live = v.order + a->rows;
   float* scale = (float*)f.scale;
-  hipLaunchKernelGGL(k_scale, dim3(1), dim3(1024), 0, s, a->g, v.total, a->rows, a->reduction, (int)Kind<T>::F16, scale);
-  if (a->dx)
-    hipLaunchKernelGGL(k_clear_rows<T>, dim3((unsigned)(a->rows < 2048 ? a->rows : 2048)), dim3(256), 0, s, a->target, a->rows, a->ignore_index, a->k, (T*)a->dx);
+  const int64_t clear = a->dx ? (a->rows + 3) / 4 : 0;
+  hipLaunchKernelGGL(k_scale<T>, dim3((unsigned)(1 + (clear < 512 ? clear : 512))), dim3(1024), 0, s, a->g, v.total, a->rows, a->reduction, scale, a->target,
+                     a->ignore_index, a->k, (T*)a->dx);
   const Staging sx = staging<T>(a->x, a->ldx, a->rows, a->k, f.x, true, v.order, live), sw = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
   stage<T>(sx, sw, s);
   const Operand x = staged<T>(sx), w = staged<T>(sw);
