@@ -143,7 +143,8 @@ __global__ void __launch_bounds__(256) k_label_join(const float2* part, const in
 
 // scale[0]: what dz is multiplied by as it is stored, scale[1]: what its products are multiplied by.  mean and sum: the one factor
 // belongs to the products, and fp16's dz = p - onehot is stored times 2^10 so that small p keep their bits (|dz| <= 1).  none: the
-// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10.  All blocks but the first: zeros for the
+// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10.  (8 loads under way: 1048576 x 64
+// -> 72 fp16 loss and gradients 1.54 -> 1.38 ms.)  All blocks but the first: zeros for the
 // rows of dx that do not count (one launch for both: 333 x 300 -> 200 fp32 loss and gradients 60.8 -> 58.9 us).
 template <typename T>
 __global__ void __launch_bounds__(1024) k_scale(const float* g, const float* total, int64_t rows, int reduction, float* scale, const int64_t* target, int64_t ignore,
@@ -166,6 +167,7 @@ __global__ void __launch_bounds__(1024) k_scale(const float* g, const float* tot
   }
   float top = 0.f;
   if (half)
+#pragma unroll 8
     for (int64_t m = threadIdx.x; m < rows; m += 1024) {
       const float v = fabsf(g[m]);
       top = v <= 3.4028235e38f ? fmaxf(top, v) : top;
