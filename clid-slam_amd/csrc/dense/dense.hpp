@@ -4,8 +4,8 @@
 // Softmax statistics.  A row's statistics over a set of columns are (m, r): the largest z and r = sum over the OTHER columns of
 // exp(z - m).  log sum exp = m + log1p(r), so the log-probability of the largest column is -log1p(r) and the loss of a target t
 // is (m - z_t) + log1p(r): a confident row keeps its relative accuracy where m + log(1 + r) would round it away.  Two sets
-// join as: the larger m wins, r = r_win + (1 + r_lose) exp(m_lose - m_win).  A set of -inf alone has m = -inf, r = 0; one that holds a NaN has
-// r = NaN.
+// join as: the larger m wins, r = r_win + (1 + r_lose) exp(m_lose - m_win).  A set of -inf alone has m = -inf, r = 0; one that holds a NaN or
+// +inf has r = NaN.
 #pragma once
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>

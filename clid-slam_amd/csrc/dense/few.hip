@@ -157,7 +157,7 @@ __global__ void __launch_bounds__(256) k_few_stat(Few a, const T* bias, const in
         if (col >= a.n) break;
         const int at = ((m >> 4) * 16 * NT + n) * kFewRow + (m & 15);
         const float z = sums[at] + sums[kTile + at] + sums[2 * kTile + at] + sums[3 * kTile + at] + (bias ? up(bias[col]) : 0.f);
-        s = join(s, {z, z != z ? z : 0.f, (int)col});
+        s = join(s, {z, z < __builtin_inff() ? 0.f : __builtin_nanf(""), (int)col});  // (+inf - inf or a NaN: no sum is a number)
         if (t == col) zt[m] = z;
       }
     __syncthreads();
