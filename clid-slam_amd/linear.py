@@ -8,6 +8,7 @@ from __future__ import annotations
 import ctypes as C
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -110,6 +111,8 @@ def check_operands(what: str, x, weight, bias=None, residual=None) -> None:
     for name, t in (("x", x), ("weight", weight)):
         if not isinstance(t, torch.Tensor):
             raise RuntimeError(f"{what}: {name} must be a tensor")
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise RuntimeError(f"{what}: make_fx records the tensors that a call makes but not the kernels that fill them")
     if not x.is_cuda:
         raise RuntimeError(f"{what}: x must live on the GPU (got {x.device}); the HIP path has no CPU fallback")
     dtype, shape, wshape = x.dtype, x.shape, weight.shape
@@ -131,12 +134,19 @@ def _like(what, name, t, shape, dtype, device):
         raise RuntimeError(f"{what}: {name} must be {dtype} on {device} like x, got {t.dtype} on {t.device}")
 
 
-def wants_grad(*tensors) -> bool:
+def through_function(*tensors) -> bool:
+    """Whether a call goes through its autograd Function rather than straight to the launch: gradients are wanted; or an operand
+    carries a forward-mode tangent, which the Function refuses (a launch of its own would return a derivative of zero without a word);
+    or torch.jit.trace is recording, which keeps a Function as a node and of a launch nothing."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
-    return False
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                return True
+    return torch._C._is_tracing()
 
 
 def _forward(x, weight, bias, act, residual, keep_z):
@@ -194,23 +204,18 @@ def linear_act(x, weight, bias=None, activation: str = "none", residual=None):
     x [..., k], weight [n, k] (torch.nn.Linear's layout), bias [n], residual [..., n] and y all of one type (float32, bfloat16,
     float16) on one GPU; rows may be a view of a wider buffer.  `activation`: none, relu, leaky_relu (slope 0.01), gelu (erf),
     silu.  Sums are fp32; y is rounded once, after the residual.  Runs on torch's current stream, captures into a graph,
-    differentiates once."""
+    differentiates once, backward only (forward-mode tangents are refused)."""
     act = ACTIVATIONS.get(activation)
     if act is None:
         raise NotImplementedError(f"linear_act: activation must be one of {', '.join(ACTIVATIONS)}, got {activation!r}")
     check_operands("linear_act", x, weight, bias, residual)
-    if wants_grad(x, weight, bias, residual):
+    if through_function(x, weight, bias, residual):
         return _LinearAct.apply(x, weight, bias, residual, act)
     with torch.no_grad():
         return _forward(x, weight, bias, act, residual, False)[0]
 
 
-@torch.no_grad()
-def linear_label(x, weight, bias=None):
-    """(label, log_prob) of z = x weight^T + bias without storing z: label [...] int64 = the lowest class with the largest z (a
-    NaN counts as largest, as in torch.argmax), log_prob [...] float32 = log softmax(z) at it.  Operands as in `linear_act`; not
-    differentiable (the class head's training loss is `loss.linear_cross_entropy`)."""
-    check_operands("linear_label", x, weight, bias)
+def _label(x, weight, bias):
     n, k = weight.shape
     (x2, ldx), (w, ldw) = rows_of(x, k), rows_of(weight, k)
     b = None if bias is None else bias.contiguous()
@@ -222,3 +227,22 @@ def linear_label(x, weight, bias=None):
              LabelArgs(x2.data_ptr(), w.data_ptr(), _lib.ptr(b), label.data_ptr(), log_prob.data_ptr(), ldx, ldw, rows, k, n, DTYPES[x.dtype], 0),
              x.device)
     return label, log_prob
+
+
+class _LinearLabel(torch.autograd.Function):  # for torch.jit.trace alone (through_function)
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        label, log_prob = _label(x, weight, bias)
+        ctx.mark_non_differentiable(label, log_prob)
+        return label, log_prob
+
+
+@torch.no_grad()
+def linear_label(x, weight, bias=None):
+    """(label, log_prob) of z = x weight^T + bias without storing z: label [...] int64 = the lowest class with the largest z (a
+    NaN counts as largest, as in torch.argmax), log_prob [...] float32 = log softmax(z) at it.  Operands as in `linear_act`; not
+    differentiable (the class head's training loss is `loss.linear_cross_entropy`)."""
+    check_operands("linear_label", x, weight, bias)
+    if torch._C._is_tracing():
+        return _LinearLabel.apply(x, weight, bias)
+    return _label(x, weight, bias)

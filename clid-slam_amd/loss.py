@@ -94,7 +94,7 @@ def linear_cross_entropy(x, weight, bias, target, ignore_index: int = -100, redu
     x [..., k], weight [n, k], bias [n] or None of one type (float32, bfloat16, float16) on one GPU; target [...] int64 or int32
     class numbers.  The loss is fp32: a value, or [...] with reduction="none".  Rows with target == ignore_index count for nothing,
     whatever they hold; "mean" divides by the rows that count and is 0 where there are none.  Any other target outside [0, n)
-    makes its row's loss and the gradients that it reaches NaN.  Differentiates once."""
+    makes its row's loss and the gradients that it reaches NaN.  Differentiates once, backward only."""
     if reduction not in linear.REDUCTIONS:
         raise NotImplementedError(f"linear_cross_entropy: reduction must be mean, sum or none, got {reduction!r}")
     linear.check_operands("linear_cross_entropy", x, weight, bias)

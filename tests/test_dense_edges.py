@@ -1,9 +1,12 @@
 """Calls of the dense operators at the edge of what they promise, and results that need more than the tests of whole layers ask for."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import dense_ref as ref
-from clid_slam_amd.linear import linear_label
+from clid_slam_amd import Decoder, HotPathConfig
+from clid_slam_amd import linear as L
+from clid_slam_amd.linear import linear_act, linear_label
 from clid_slam_amd.loss import linear_cross_entropy
 from test_dense_ops import generator, normal
 
@@ -47,3 +50,89 @@ def test_a_logit_of_plus_infinity_is_nan_in_its_row_at_every_size(shape, dtype):
     label, log_prob = linear_label(x, w, b)
     assert (label == n - 1).all() and torch.isnan(log_prob).all()
     assert torch.isnan(linear_cross_entropy(x, w, b, torch.zeros(m, dtype=torch.int64, device="cuda"), reduction="none")).all()
+
+
+# ---- CPU: the launch replaced by a count ---------------------------------------------------------------------------------------
+@pytest.fixture
+def launches(monkeypatch):
+    """The entry points that calls reach, with CPU operands."""
+    seen = []
+
+    class Lib:
+        @staticmethod
+        def clid_ce_saved(args):
+            return 256
+
+    checks = L.check_operands
+
+    def check(what, x, weight, bias=None, residual=None):
+        if not x.is_cuda:  # everything but the refusal of CPU tensors
+            with monkeypatch.context() as m:
+                m.setattr(torch.Tensor, "is_cuda", True)
+                return checks(what, x, weight, bias, residual)
+        return checks(what, x, weight, bias, residual)
+
+    monkeypatch.setattr(L, "check_operands", check)
+    monkeypatch.setattr(L, "load", Lib)
+    monkeypatch.setattr(L, "call", lambda entry, workspace, args, device: seen.append(entry))
+    return seen
+
+
+@pytest.mark.parametrize("which", ["x", "weight", "bias", "residual"])
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused_and_never_lost(launches, which, grad_mode):
+    ops = {"x": torch.randn(4, 8), "weight": torch.randn(5, 8), "bias": torch.randn(5), "residual": torch.randn(4, 5)}
+    target = torch.zeros(4, dtype=torch.int64)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        assert linear_act(**ops).shape == (4, 5)  # no tangent anywhere: an ordinary call
+        ops[which] = forward_ad.make_dual(ops[which], torch.ones_like(ops[which]))
+        with pytest.raises(NotImplementedError, match="jvp"):
+            linear_act(**ops, activation="relu")
+        if which != "residual":
+            with pytest.raises(NotImplementedError, match="jvp"):
+                linear_cross_entropy(ops["x"], ops["weight"], ops["bias"], target)
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")  # (that the trace keeps shapes is what traces do)
+@pytest.mark.parametrize("op", ["linear", "label", "cross_entropy"])
+def test_a_traced_call_launches_at_every_replay(launches, op):
+    """torch.jit.trace records no launch that a tensor's bare pointer is handed to: it would give back memory that nothing has written."""
+    w, target = torch.randn(5, 8), torch.zeros(4, dtype=torch.int64)
+
+    def f(x):
+        if op == "linear":
+            return linear_act(x, w, activation="relu")
+        return linear_label(x, w) if op == "label" else linear_cross_entropy(x, w, None, target)
+
+    with torch.no_grad():
+        traced = torch.jit.trace(f, (torch.randn(4, 8),), check_trace=False)
+        for _ in range(3):
+            before = len(launches)
+            traced(torch.randn(4, 8))
+            assert len(launches) == before + 1
+
+
+@pytest.mark.parametrize("op", ["linear", "label", "cross_entropy"])
+def test_make_fx_is_refused(launches, op):
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    w, target = torch.randn(5, 8), torch.zeros(4, dtype=torch.int64)
+    f = {"linear": lambda x: linear_act(x, w), "label": lambda x: linear_label(x, w)[0], "cross_entropy": lambda x: linear_cross_entropy(x, w, None, target)}[op]
+    with pytest.raises(RuntimeError, match="make_fx"):
+        make_fx(f)(torch.randn(4, 8))
+    assert not launches
+
+
+@gpu
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+def test_a_traced_decoder_answers_as_the_decoder_itself():
+    cfg = HotPathConfig()
+    cfg.device = "cuda"
+    torch.manual_seed(2)
+    dec = Decoder(cfg, 48, 2, 5).requires_grad_(False)
+    gen = generator(3)
+    x = [normal(gen, 200, 11) for _ in range(3)]
+    mlp = torch.jit.trace(lambda v: dec.mlp(v), (x[0],))
+    label = torch.jit.trace(lambda v: dec.sem_label(v), (x[0],))
+    for v in x:
+        assert torch.equal(mlp(v), dec.mlp(v)) and torch.equal(label(v), dec.sem_label(v))
