@@ -143,13 +143,35 @@ __global__ void __launch_bounds__(256) k_label_join(const float2* part, const in
 
 // scale[0]: what dz is multiplied by as it is stored, scale[1]: what its products are multiplied by.  mean and sum: the one factor
 // belongs to the products, and fp16's dz = p - onehot is stored times 2^10 so that small p keep their bits (|dz| <= 1).  none: the
-// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10.  (8 loads under way: 1048576 x 64
-// -> 72 fp16 loss and gradients 1.54 -> 1.38 ms.)  All blocks but the first: zeros for the
+// rows' factors go into dz, fp16's scaled by the power of two that brings the largest to at most 2^10; a row that does not count has no say in it,
+// whatever its factor.  More than kTopRows rows are looked at by blocks of their own first (k_top: 64 -> 72 fp16 loss and gradients of 1048576 rows
+// 1352 us, 2025 by the one block, of 32768 rows 111 and 113, of 16384 rows 78 and 77).  All blocks but the first: zeros for the
 // rows of dx that do not count (one launch for both: 333 x 300 -> 200 fp32 loss and gradients 60.8 -> 58.9 us).
-template <typename T>
-__global__ void __launch_bounds__(1024) k_scale(const float* g, const float* total, int64_t rows, int reduction, float* scale, const int64_t* target, int64_t ignore,
-                                                int k, T* dx) {
+constexpr int64_t kTopRows = 16384;
+__device__ __forceinline__ float largest(const float* g, const int64_t* target, int64_t ignore, int64_t from, int64_t rows, int64_t step) {
+  float top = 0.f;
+#pragma unroll 8
+  for (int64_t m = from; m < rows; m += step) {
+    const float v = fabsf(g[m]);
+    top = v <= 3.4028235e38f && target[m] != ignore ? fmaxf(top, v) : top;
+  }
+  return top;
+}
+__device__ __forceinline__ float block_largest(float top) {  // 1024 threads; the first one's result
   __shared__ float ps[16];
+  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+  if ((threadIdx.x & 63) == 0) ps[threadIdx.x >> 6] = top;
+  __syncthreads();
+  for (int i = 0; i < 16; ++i) top = fmaxf(top, ps[i]);
+  return top;
+}
+__global__ void __launch_bounds__(1024) k_top(const float* g, const int64_t* target, int64_t ignore, int64_t rows, float* tops) {
+  const float top = block_largest(largest(g, target, ignore, (int64_t)blockIdx.x * 1024 + threadIdx.x, rows, (int64_t)gridDim.x * 1024));
+  if (threadIdx.x == 0) tops[blockIdx.x] = top;
+}
+template <typename T>
+__global__ void __launch_bounds__(1024) k_scale(const float* g, const float* total, int64_t rows, int reduction, const float* tops, int n_tops, float* scale,
+                                                const int64_t* target, int64_t ignore, int k, T* dx) {
   constexpr bool half = Kind<T>::F16;
   if (blockIdx.x) {
     for (int64_t m = (int64_t)(blockIdx.x - 1) * 4 + (threadIdx.x >> 8); m < rows; m += (int64_t)(gridDim.x - 1) * 4)
@@ -166,17 +188,8 @@ __global__ void __launch_bounds__(1024) k_scale(const float* g, const float* tot
     return;
   }
   float top = 0.f;
-  if (half)
-#pragma unroll 8
-    for (int64_t m = threadIdx.x; m < rows; m += 1024) {
-      const float v = fabsf(g[m]);
-      top = v <= 3.4028235e38f ? fmaxf(top, v) : top;
-    }
-  for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
-  if ((threadIdx.x & 63) == 0) ps[threadIdx.x >> 6] = top;
-  __syncthreads();
+  if (half) top = block_largest(n_tops ? (int)threadIdx.x < n_tops ? tops[threadIdx.x] : 0.f : largest(g, target, ignore, threadIdx.x, rows, 1024));
   if (threadIdx.x) return;
-  for (int i = 0; i < 16; ++i) top = fmaxf(top, ps[i]);
   int e = 0;
   if (top > 0.f) frexpf(top, &e);  // top < 2^e
   const int by = half && top > 0.f ? (10 - e > 100 ? 100 : 10 - e < -100 ? -100 : 10 - e) : 0;
@@ -283,7 +296,8 @@ struct CeBwd {
   int64_t piece, ld;
   int blocks;
   Plan pz, px, pw;
-  char *x, *w, *dz, *sum, *part, *sums, *scale;
+  int tops;  // blocks of k_top
+  char *x, *w, *dz, *sum, *part, *sums, *scale, *top;
   int64_t bytes;
   explicit CeBwd(const clid_ce_args* a) {
     constexpr int NP = Kind<T>::NP;
@@ -302,6 +316,9 @@ struct CeBwd {
     blocks = row_blocks(a->rows, (int)piece);
     sums = ws.take(a->db ? blocks * piece * 4 : 0);
     scale = ws.take(8);
+    const int64_t t = (a->rows + 2047) / 2048;
+    tops = Kind<T>::F16 && a->reduction == CLID_REDUCE_NONE && a->rows > kTopRows ? (int)(t < 256 ? t : 256) : 0;
+    top = ws.take(tops * 4);
     bytes = ws.used;
   }
 };
@@ -314,8 +331,9 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
   const int32_t* live = v.order + a->rows;
   float* scale = (float*)f.scale;
   const int64_t clear = a->dx ? (a->rows + 3) / 4 : 0;
-  hipLaunchKernelGGL(k_scale<T>, dim3((unsigned)(1 + (clear < 512 ? clear : 512))), dim3(1024), 0, s, a->g, v.total, a->rows, a->reduction, scale, a->target,
-                     a->ignore_index, a->k, (T*)a->dx);
+  if (f.tops) hipLaunchKernelGGL(k_top, dim3(f.tops), dim3(1024), 0, s, a->g, a->target, a->ignore_index, a->rows, (float*)f.top);
+  hipLaunchKernelGGL(k_scale<T>, dim3((unsigned)(1 + (clear < 512 ? clear : 512))), dim3(1024), 0, s, a->g, v.total, a->rows, a->reduction, (const float*)f.top, f.tops, scale,
+                     a->target, a->ignore_index, a->k, (T*)a->dx);
   const Staging sx = staging<T>(a->x, a->ldx, a->rows, a->k, f.x, true, v.order, live), sw = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
   stage<T>(sx, sw, s);
   const Operand x = staged<T>(sx), w = staged<T>(sw);

@@ -136,3 +136,26 @@ def test_a_traced_decoder_answers_as_the_decoder_itself():
     label = torch.jit.trace(lambda v: dec.sem_label(v), (x[0],))
     for v in x:
         assert torch.equal(mlp(v), dec.mlp(v)) and torch.equal(label(v), dec.sem_label(v))
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(300, 72, 66), (2000, 40, 100), (20, 72, 66), (300, 64, 21), (20000, 24, 70)], ids=str)
+def test_factors_of_rows_that_do_not_count_reach_nothing(shape, dtype):
+    """reduction="none": whatever dL/dloss holds for an ignored row, the others' gradients have the same bits."""
+    m, k, n = shape
+    dt, gen = TYPES[dtype], generator(m + k)
+    x, w, b = normal(gen, m, k).to(dt).requires_grad_(), (normal(gen, n, k) * k ** -0.5).to(dt).requires_grad_(), normal(gen, n).to(dt).requires_grad_()
+    t = torch.randint(0, n, (m,), generator=gen, device="cuda")
+    lost = torch.arange(m, device="cuda") % 3 == 1
+    t[lost] = -100
+    g = (normal(gen, m).abs() + 0.5).masked_fill(lost, 0.0)
+    want = ref.cross_entropy(x, w, b, t, -100, "none", g)
+    first = None
+    for other in (0.0, 1e30, -3e38, 1e-30, INF, float("nan")):
+        loss = linear_cross_entropy(x, w, b, t, reduction="none")
+        got = torch.autograd.grad(loss, [x, w, b], torch.where(lost, other, g))
+        for name, v in zip(("dx", "dw", "db"), got):
+            ref.close(v, *want[name], f"{name}, {other}")
+        first = first or got
+        assert all(torch.equal(a, q) for a, q in zip(got, first))
