@@ -120,6 +120,8 @@ def check_operands(what: str, x, weight, bias=None, residual=None) -> None:
         raise RuntimeError(f"{what}: x must be float32, bfloat16 or float16, got {dtype}")
     if len(wshape) != 2 or len(shape) < 1 or shape[-1] != wshape[1] or 0 in wshape:
         raise RuntimeError(f"{what}: x {tuple(shape)} and weight {tuple(wshape)} must be [..., k] and [n, k] with n, k >= 1")
+    if max(wshape) >= 1 << 20:  # (also before a ctypes structure keeps the low 32 bits of it)
+        raise RuntimeError(f"{what}: bad argument: weight {tuple(wshape)} must have n, k < 2^20")
     _like(what, "weight", weight, wshape, dtype, x.device)
     if bias is not None:
         _like(what, "bias", bias, wshape[:1], dtype, x.device)

@@ -159,3 +159,20 @@ def test_factors_of_rows_that_do_not_count_reach_nothing(shape, dtype):
             ref.close(v, *want[name], f"{name}, {other}")
         first = first or got
         assert all(torch.equal(a, q) for a, q in zip(got, first))
+
+
+@pytest.mark.parametrize("k,n", [(1 << 20, 3), ((1 << 32) + 8, 3), (8, (1 << 32) + 3), (1 << 31, 1)], ids=str)
+def test_widths_are_refused_before_they_are_cut_to_32_bits(k, n):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, w = torch.empty(2, k, dtype=torch.bfloat16, device="cuda"), torch.empty(n, k, dtype=torch.bfloat16, device="cuda")
+        t = torch.empty(2, dtype=torch.int64, device="cuda")
+        for f in (lambda: linear_act(x, w), lambda: linear_label(x, w), lambda: linear_cross_entropy(x, w, None, t)):
+            with pytest.raises(RuntimeError, match="bad argument"):
+                f()
+
+
+def test_how_a_width_would_be_cut():
+    """ctypes takes the low 32 bits of a number without a word: what the check above is for."""
+    assert L.LinearArgs(k=(1 << 32) + 8).k == 8
