@@ -248,8 +248,8 @@ struct EpiStat {
       for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][r]);
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float safe = top == neg_inf() ? 0.f : top;
-    // sum of all exp(z - top), the largest one's 1 among them; where the others are less than 2^-6 of it that sum has lost their last
-    // bits, and they are added up again without it
+    // sum of all exp(z - top), the largest one's 1 among them; where the others are less than half of it that sum has lost more of their last
+    // bits than a sum loses anyway, and they are added up again without it
     float rest = 0.f;
 #pragma unroll
     for (int i = 0; i < TN; ++i)
@@ -257,7 +257,7 @@ struct EpiStat {
       for (int r = 0; r < 16; ++r) rest += __builtin_amdgcn_exp2f((acc[i][r] - safe) * 1.4426950408889634f);
     rest += __shfl_xor(rest, 32, 64);
     rest -= 1.f;
-    if (__any(!(rest >= 0.015625f))) {
+    if (__any(!(rest >= 0.5f))) {
       float again = 0.f;
       int same = 0;
 #pragma unroll
@@ -270,7 +270,7 @@ struct EpiStat {
         }
       again += __shfl_xor(again, 32, 64);
       same += __shfl_xor(same, 32, 64);
-      if (!(rest >= 0.015625f)) rest = again + (float)(same - 1);
+      if (!(rest >= 0.5f)) rest = again + (float)(same - 1);
     }
     if (top == neg_inf()) rest = rest == rest ? 0.f : rest;  // nothing finite here: a join counts nothing
     if (top == __builtin_inff()) rest = __builtin_nanf("");

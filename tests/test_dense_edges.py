@@ -176,3 +176,30 @@ def test_widths_are_refused_before_they_are_cut_to_32_bits(k, n):
 def test_how_a_width_would_be_cut():
     """ctypes takes the low 32 bits of a number without a word: what the check above is for."""
     assert L.LinearArgs(k=(1 << 32) + 8).k == 8
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(300, 72, 64), (40, 264, 66), (4096, 80, 96), (300, 8, 50), (20, 72, 64)], ids=str)
+def test_confident_rows_keep_their_relative_accuracy(m, k, n, dtype):
+    """log_prob and loss of rows whose other classes together are 2^-6 to 2^-1 of the largest: log1p of that sum, in which nothing
+    of the largest one's 1 may be rounded away.
+
+    z = -x[m, 0] for every class but the first, exact in every type, so the sum's terms are off by what exp makes of z log2(e) rounded
+    twice (2 u |z|) and its own 2 u; the n of them add (n + 3) u at most, three times that where a sum that holds the 1 is used (down
+    to 1/2 of it), log1p 8 u."""
+    dt = TYPES[dtype]
+    x = torch.zeros(m, k, device="cuda")
+    others = torch.linspace(2.0 ** -6, 0.5, m, device="cuda", dtype=torch.float64) * 1.01
+    x[:, 0] = -torch.log(others / (n - 1))
+    x = x.to(dt)
+    w = torch.zeros(n, k, dtype=dt, device="cuda")
+    w[1:, 0] = -1.0
+    z = x[:, 0].double()
+    want = torch.log1p((n - 1) * torch.exp(-z))
+    tol = (3 * (n + 3) + 2 * z + 16) * ref.U * want
+    label, log_prob = linear_label(x, w)
+    assert not label.any()
+    ref.close(log_prob, -want, tol, "log_prob")
+    loss = linear_cross_entropy(x, w, None, torch.zeros(m, dtype=torch.int64, device="cuda"), reduction="none")
+    ref.close(loss, want, tol, "loss")
