@@ -201,6 +201,11 @@ template <typename T, int SIZE> constexpr int strip_of() { return Tile<Kind<T>::
 template <typename T>
 int strip_width(int size) { return size == 2 ? strip_of<T, 2>() : size == 1 ? strip_of<T, 1>() : strip_of<T, 0>(); }
 
+// rows of a wave
+template <typename T, int SIZE> constexpr int run_of() { return Tile<Kind<T>::NP, SIZE>::BM / Tile<Kind<T>::NP, SIZE>::WM; }
+template <typename T>
+int run_rows(int size) { return size == 2 ? run_of<T, 2>() : size == 1 ? run_of<T, 1>() : run_of<T, 0>(); }
+
 template <typename T, bool LABEL>
 int launch_stat(const Product& g, int size, const T* bias, const int64_t* target, const int32_t* order, float2* part, int32_t* part_at, float* zt, hipStream_t s) {
   constexpr int NP = Kind<T>::NP;
@@ -211,7 +216,7 @@ int launch_stat(const Product& g, int size, const T* bias, const int64_t* target
 template <typename T>
 int launch_dz(const Product& g, int size, const EpiDz<T, 0, Kind<T>::NP>& e, hipStream_t s) {
   constexpr int NP = Kind<T>::NP;
-#define DZ(S) launch_one<T, S, false, false>(g, EpiDz<T, Tile<NP, S>::BN, NP>{e.bias, e.target, e.order, e.stat, e.scale, e.g, e.dz, e.v0, e.n, e.ld}, s)
+#define DZ(S) launch_one<T, S, false, false>(g, EpiDz<T, Tile<NP, S>::BN, NP>{e.bias, e.target, e.order, e.stat, e.scale, e.g, e.dz, e.sums, e.v0, e.n, e.ld}, s)
   return size == 2 ? DZ(2) : size == 1 ? DZ(1) : DZ(0);
 #undef DZ
 }
@@ -294,10 +299,10 @@ int64_t piece_of(const clid_ce_args* a) {
 template <typename T>
 struct CeBwd {
   int64_t piece, ld;
-  int blocks;
   Plan pz, px, pw;
-  int tops;  // blocks of k_top
-  char *x, *w, *dz, *sum, *part, *sums, *scale, *top;
+  int runs, groups, share;  // db: partial sums, joined `share` at a time first where there are many (groups: 0 where not)
+  int tops;                 // blocks of k_top
+  char *x, *w, *dz, *sum, *part, *sums, *joined, *scale, *top;
   int64_t bytes;
   explicit CeBwd(const clid_ce_args* a) {
     constexpr int NP = Kind<T>::NP;
@@ -313,8 +318,11 @@ struct CeBwd {
     sum = ws.take(a->dx && piece < a->n ? a->rows * a->k * 4 : 0);
     const int64_t bx = a->dx ? part_bytes(px, a->rows, a->k) : 0, bw = a->dw ? part_bytes(pw, piece, a->k) : 0;
     part = ws.take(bx > bw ? bx : bw);
-    blocks = row_blocks(a->rows, (int)piece);
-    sums = ws.take(a->db ? blocks * piece * 4 : 0);
+    runs = (int)((a->rows + run_rows<T>(pz.size) - 1) / run_rows<T>(pz.size));
+    share = runs <= 256 * 1024 ? 256 : (runs + 1023) / 1024;
+    groups = runs > 1024 ? (runs + share - 1) / share : 0;
+    sums = ws.take(a->db ? runs * piece * 4 : 0);
+    joined = ws.take(a->db ? groups * piece * 4 : 0);
     scale = ws.take(8);
     const int64_t t = (a->rows + 2047) / 2048;
     tops = Kind<T>::F16 && a->reduction == CLID_REDUCE_NONE && a->rows > kTopRows ? (int)(t < 256 ? t : 256) : 0;
@@ -344,7 +352,7 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
     const Operand dz = {(const uint16_t*)f.dz, ld * NP};
     Product gz = {x, wv, a->rows, nv, up8(a->k), live, 0, 1, 0, 0};
     int rc = launch_dz<T>(gz, f.pz.size, {a->bias ? (const T*)a->bias + v0 : nullptr, a->target, v.order, v.stat, scale,
-                                          a->reduction == CLID_REDUCE_NONE ? a->g : nullptr, (uint16_t*)f.dz, v0, nv, ld}, s);
+                                          a->reduction == CLID_REDUCE_NONE ? a->g : nullptr, (uint16_t*)f.dz, a->db ? (float*)f.sums : nullptr, v0, nv, ld}, s);
     if (rc != CLID_OK) return rc;
     if (a->dx) {
       const bool last = v0 + nv == a->n;
@@ -363,8 +371,15 @@ int ce_bwd(const clid_ce_args* a, hipStream_t s) {
       if (rc != CLID_OK) return rc;
     }
     if (a->db) {
-      hipLaunchKernelGGL(k_colsum<T>, dim3((unsigned)((ld + 255) / 256), f.blocks), dim3(256), 0, s, (const uint16_t*)f.dz, a->rows, live, (int)nv, (int)ld, (float*)f.sums);
-      hipLaunchKernelGGL(k_colsum_join<T>, dim3((unsigned)((nv + 63) / 64)), dim3(1024), 0, s, (const float*)f.sums, f.blocks, (int)nv, (const float*)(scale + 1), (T*)a->db + v0);
+      const dim3 cols((unsigned)((nv + 63) / 64));
+      const int per = run_rows<T>(f.pz.size);
+      const float *alpha = scale + 1, *sums = (const float*)f.sums;
+      if (f.groups) {
+        hipLaunchKernelGGL(k_colsum_join<float>, dim3(cols.x, f.groups), dim3(1024), 0, s, sums, f.runs, f.share, (int)nv, live, per, (const float*)nullptr, (float*)f.joined);
+        hipLaunchKernelGGL(k_colsum_join<T>, cols, dim3(1024), 0, s, (const float*)f.joined, f.groups, f.groups, (int)nv, (const int32_t*)nullptr, 1, alpha, (T*)a->db + v0);
+      } else {
+        hipLaunchKernelGGL(k_colsum_join<T>, cols, dim3(1024), 0, s, sums, f.runs, f.runs, (int)nv, live, per, alpha, (T*)a->db + v0);
+      }
     }
   }
   return CLID_OK;

@@ -69,7 +69,8 @@ int bwd(const clid_linear_bwd_args* a, hipStream_t s) {
     if (a->z_is_y) launch((const T*)a->z);
     else launch((const typename KeptZ<T>::Z*)a->z);
     if (a->db)
-      hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, a->n, (const float*)nullptr, (T*)a->db);
+      hipLaunchKernelGGL(k_colsum_join<T>, dim3((a->n + 63) / 64), dim3(1024), 0, s, (const float*)f.sums, f.blocks, f.blocks, a->n,
+                         (const int32_t*)nullptr, 1, (const float*)nullptr, (T*)a->db);
   }
   Staging x = staging<T>(a->x, a->ldx, a->rows, a->k, f.x), w = staging<T>(a->w, a->ldw, a->n, a->k, f.w);
   if (!a->dw) x.blocks = 0;

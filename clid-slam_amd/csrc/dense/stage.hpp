@@ -142,52 +142,26 @@ __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const Z* 
     part[(int64_t)blockIdx.y * n + col] = s;
   }
 }
-// column sums of planes, as k_dz's: a pass of its own over dz, bound by memory (8192 x 32768 bf16 112 us, 4.8 TB/s; 2048 x 32000 in fp32's planes
-// 69 us, 5.7 TB/s)
+// Partial column sums joined in their order, `share` of them into out[blockIdx.y][n]; with `live` only those of rows that there are, `per` rows
+// each.  64 columns a block, 16 threads a column.
 template <typename T>
-__global__ void __launch_bounds__(256) k_colsum(const uint16_t* src, int64_t rows, const int32_t* live, int n, int np, float* part) {
-  __shared__ float sums[8][256 + 8];
-  if (live) rows = *live < rows ? *live : rows;
-  const int cg = threadIdx.x & 31, rr = threadIdx.x >> 5, c = blockIdx.x * 256 + cg * 8;
-  float sum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  if (c < np)
-    for (int64_t m = (int64_t)blockIdx.y * 8 + rr; m < rows; m += (int64_t)gridDim.y * 8) {
-      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int s = Kind<T>::NP - 1; s >= 0; --s) {
-        union { uint4 w; typename Kind<T>::E t[8]; } u;
-        u.w = *(const uint4*)(src + m * np * Kind<T>::NP + column<Kind<T>::NP>(c) + s * 32);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] += up(u.t[q]);
-      }
-#pragma unroll
-      for (int q = 0; q < 8; ++q) sum[q] += v[q];
-    }
-#pragma unroll
-  for (int q = 0; q < 8; ++q) sums[rr][cg * 8 + q] = sum[q];
-  __syncthreads();
-  const int col = blockIdx.x * 256 + threadIdx.x;
-  if (col < n) {
-    float s = 0.f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) s += sums[r][threadIdx.x];
-    part[(int64_t)blockIdx.y * n + col] = s;
-  }
-}
-// 64 columns a block, 16 threads a column
-template <typename T>
-__global__ void __launch_bounds__(1024) k_colsum_join(const float* part, int blocks, int n, const float* alpha, T* out) {
+__global__ void __launch_bounds__(1024) k_colsum_join(const float* part, int blocks, int share, int n, const int32_t* live, int per, const float* alpha, T* out) {
   __shared__ float p[16][64];
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), g = threadIdx.x >> 6;
+  if (live) {
+    const int64_t there = ((int64_t)*live + per - 1) / per;
+    blocks = there < blocks ? (int)there : blocks;
+  }
+  const int from = blockIdx.y * share, to = from + share < blocks ? from + share : blocks;
   float s = 0.f;
   if (c < n)
 #pragma unroll 4
-    for (int b = g; b < blocks; b += 16) s += part[(int64_t)b * n + c];
+    for (int b = from + g; b < to; b += 16) s += part[(int64_t)b * n + c];
   p[g][threadIdx.x & 63] = s;
   __syncthreads();
   if (g || c >= n) return;
   for (int i = 1; i < 16; ++i) s += p[i][threadIdx.x];
-  out[c] = down<T>((alpha ? *alpha : 1.f) * s);
+  out[(int64_t)blockIdx.y * n + c] = down<T>((alpha ? *alpha : 1.f) * s);
 }
 inline int row_blocks(int64_t rows, int n) {
   const int64_t cols = (n + 255) / 256, want = 2048 / cols + 1, most = (rows + 15) / 16;

@@ -203,3 +203,21 @@ def test_confident_rows_keep_their_relative_accuracy(m, k, n, dtype):
     ref.close(log_prob, -want, tol, "log_prob")
     loss = linear_cross_entropy(x, w, None, torch.zeros(m, dtype=torch.int64, device="cuda"), reduction="none")
     ref.close(loss, want, tol, "loss")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+@pytest.mark.parametrize("m,k,n", [(40, 72, 66), (300, 100, 130), (2049, 64, 500), (4500, 24, 300), (140001, 16, 65), (70, 9, 20011)], ids=str)
+def test_bias_gradient_sums_what_was_not_rounded_yet(m, k, n, reduction, dtype):
+    """db is the sum of dz in fp32, before dz is rounded to the operands' type for the products: as far from 64 bits as a sum in fp32
+    and one rounding of its result."""
+    dt, gen = TYPES[dtype], generator(m + n)
+    x, w, b = normal(gen, m, k).to(dt), (normal(gen, n, k) * k ** -0.5).to(dt), normal(gen, n).to(dt).requires_grad_()
+    t = torch.randint(0, n, (m,), generator=gen, device="cuda")
+    t[::5] = -100
+    g = normal(gen, m).abs() if reduction == "none" else torch.full((), 512.0 if reduction == "mean" else 1.0, device="cuda")
+    loss = linear_cross_entropy(x, w, b, t, reduction=reduction)
+    got = torch.autograd.grad(loss, b, g)[0]
+    v, tol = ref.cross_entropy(x.float(), w.float(), b.detach().float(), t, -100, reduction, g)["db"]
+    ref.close(got, v, ref.rounded(v, tol, dt), "db")
