@@ -32,7 +32,7 @@ template <> __device__ __forceinline__ f16 down<f16>(float v) { return __float2h
 
 __device__ __forceinline__ float neg_inf() { return -__builtin_inff(); }
 
-// ---- activations: act(z) and its slope, in fp32 ------------------------------------------------------------------------
+// ---- activations: act(z) and dy act'(z), in fp32 ------------------------------------------------------------------------
 // Phi(z) by the Chebyshev fit of erfc(x) = t exp(-x^2 + p(t)), t = 2 / (2 + x), of Press et al., Numerical Recipes, 6.2 (relative
 // error 1.2e-7 for x >= 0): one exp, one reciprocal and nine FMAs without a branch, where the library's erf takes two branches.
 __device__ __forceinline__ float normal_cdf(float z) {
@@ -61,16 +61,18 @@ __device__ __forceinline__ float act_value(float z, int act) {
     default: return z;
   }
 }
-__device__ __forceinline__ float act_slope(float z, int act) {
+// dy act'(z).  relu selects, as torch's does: a unit whose z <= 0 hands back 0 whatever it was sent (0 times an overflowed dy would be NaN), and a
+// NaN z hands dy on.
+__device__ __forceinline__ float act_grad(float dy, float z, int act) {
   switch (act) {
-    case CLID_ACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case CLID_ACT_LEAKY_RELU: return z > 0.f ? 1.f : 0.01f;
-    case CLID_ACT_GELU: return fmaf(z * 0.3989422804014327f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f), normal_cdf(z));
+    case CLID_ACT_RELU: return z <= 0.f ? 0.f : dy;
+    case CLID_ACT_LEAKY_RELU: return z > 0.f ? dy : 0.01f * dy;
+    case CLID_ACT_GELU: return dy * fmaf(z * 0.3989422804014327f, __builtin_amdgcn_exp2f(z * z * -0.72134752044448170f), normal_cdf(z));
     case CLID_ACT_SILU: {
       const float p = sigmoid(z);
-      return p * (1.f + z * (1.f - p));
+      return dy * (p * (1.f + z * (1.f - p)));
     }
-    default: return 1.f;
+    default: return dy;
   }
 }
 

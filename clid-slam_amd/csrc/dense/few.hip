@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(256) k_few_linear_dz(const float* dy, int64_t 
     float v = 0.f;
     if (m < rows && col < n) {
       v = dy[m * lddy + col];
-      if (z) v *= act_slope(z[m * n + col], act);
+      if (z) v = act_grad(v, z[m * n + col], act);
     }
     dz[m * np + col] = v;
     all += v;

@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(512) k_narrow(Narrow a) {
           for (int e = 0; e < kEach; ++e)
 #pragma unroll
             for (int q = 0; q < 8; ++q)
-              v[e][q] = m0 + lane / (4 * TN) + e * (16 / TN) < a.rows && c + q < a.n ? v[e][q] * act_slope(y[e][q], act) : 0.f;
+              v[e][q] = m0 + lane / (4 * TN) + e * (16 / TN) < a.rows && c + q < a.n ? act_grad(v[e][q], y[e][q], act) : 0.f;
         });
 #pragma unroll
         for (int e = 0; e < kEach; ++e) {

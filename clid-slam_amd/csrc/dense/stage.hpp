@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const Z* 
         if (t && !two) break;
         if (z) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) v[t][q] = q < count ? v[t][q] * act_slope(y[t][q], act) : 0.f;
+          for (int q = 0; q < 8; ++q) v[t][q] = q < count ? act_grad(v[t][q], y[t][q], act) : 0.f;
         }
 #pragma unroll
         for (int q = 0; q < 8; ++q) sum[q] += v[t][q];

@@ -47,7 +47,7 @@ typedef struct clid_linear_args {
 int64_t clid_linear_workspace(const clid_linear_args* a);
 int clid_linear_fwd(const clid_linear_args* a, void* stream);
 
-/* dz = dy act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz.  z (dense) is z_out of the forward call, or with
+/* dz = dy act'(z) (relu: dy where not z <= 0, else 0), dx = dz w, dw = dz^T x, db = sum over rows of dz.  z (dense) is z_out of the forward call, or with
  * z_is_y (relu and leaky_relu without a residual) its y, whose sign is z's; NULL for CLID_ACT_NONE.  dx, dw, db: NULL where not wanted.
  * dz is rounded to dtype between the products (fp32: not at all). */
 typedef struct clid_linear_bwd_args {

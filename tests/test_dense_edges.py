@@ -221,3 +221,49 @@ def test_bias_gradient_sums_what_was_not_rounded_yet(m, k, n, reduction, dtype):
     got = torch.autograd.grad(loss, b, g)[0]
     v, tol = ref.cross_entropy(x.float(), w.float(), b.detach().float(), t, -100, reduction, g)["db"]
     ref.close(got, v, ref.rounded(v, tol, dt), "db")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("shape", [(40, 16, 24), (5, 100, 70), (33, 100, 72), (300, 130, 70), (2000, 64, 64)], ids=str)
+def test_what_a_dead_relu_unit_is_sent_reaches_nothing(shape, residual, dtype):
+    """relu's backward pass selects: an overflowed dy (infinity, NaN) at a unit whose z <= 0 is 0 and not 0 times infinity."""
+    m, k, n = shape
+    dt, gen = TYPES[dtype], generator(m + k)
+    make = lambda *s: torch.randint(-8, 9, s, generator=gen, device="cuda") / 8  # noqa: E731  (z exact: no z changes its side of the kink)
+    x, w, b = make(m, k).to(dt).requires_grad_(), make(n, k).to(dt).requires_grad_(), make(n).to(dt).requires_grad_()
+    r = normal(gen, m, n).to(dt) if residual else None
+    dy = normal(gen, m, n).to(dt)
+    want = ref.linear(x, w, b, r, "relu", dy)
+    with torch.no_grad():
+        dead = x.double() @ w.double().t() + b.double() <= 0
+    assert dead.any()
+    for sent in (INF, -INF, float("nan")):
+        y = linear_act(x, w, b, activation="relu", residual=r)
+        got = torch.autograd.grad(y, [x, w, b], dy.masked_fill(dead, sent))
+        for name, v in zip(("dx", "dw", "db"), got):
+            ref.close(v, *want[name], f"{name}, {sent}")
+
+
+@gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", [(5, 8, 9), (6, 100, 70), (40, 100, 70)], ids=str)
+def test_activations_of_odd_values_answer_as_torch_does(shape, dtype):
+    """z of NaN, the infinities and zero: values and slopes are numbers, infinities and NaN where torch's own are (in float64)."""
+    m, k, n = shape
+    dt = TYPES[dtype]
+    fs = {"relu": torch.relu, "leaky_relu": torch.nn.functional.leaky_relu, "gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu}
+    for name, f in fs.items():
+        for value in (INF, -INF, float("nan"), 0.0, -0.0):
+            x, w = torch.zeros(m, k, dtype=dt, device="cuda"), torch.zeros(n, k, dtype=dt, device="cuda")
+            x[:, 0], w[:, 0] = value, 1.0
+            b = torch.zeros(n, dtype=dt, device="cuda", requires_grad=True)
+            y = linear_act(x, w, b, activation=name)
+            db = torch.autograd.grad(y, b, torch.ones_like(y))[0]
+            z = torch.full((1,), value, dtype=torch.float64, requires_grad=True)
+            v = f(z)
+            slope = torch.autograd.grad(v, z)[0].item()
+            # (exact numbers all: 0, 1, 1/2; leaky_relu's 0.01 has one rounding to fp32 and one to the type)
+            assert torch.allclose(y.double().cpu(), v.detach().expand(m, n), rtol=0, atol=0, equal_nan=True), (name, value)
+            assert torch.allclose(db.double().cpu(), torch.full((n,), m * slope, dtype=torch.float64), rtol=2.0 ** -8, atol=0, equal_nan=True), (name, value, db[0], slope)
