@@ -269,19 +269,19 @@ template <typename T, int SIZE, bool PKS, bool QKS, class Epi>
 inline int launch_one(Product g, const Epi& epi, hipStream_t s) {
   constexpr int NP = Kind<T>::NP;
   using C = Tile<NP, SIZE>;
-  g.tiles_m = (int)((g.m + C::BM - 1) / C::BM);
   g.tiles_n = (int)((g.n + C::BN - 1) / C::BN);
-  const int64_t blocks = (int64_t)g.tiles_m * g.tiles_n * g.splits;
-  if (blocks * 64 * C::WM * C::WN >= (int64_t(1) << 32)) {
-    clid_set_error("dense product: %lld x %lld results are more than one launch takes", (long long)g.m, (long long)g.n);
-    return CLID_E_SHAPE;
-  }
   constexpr int kLds = tile_lds<NP, C::BM, C::BN, C::BK, C::WM, C::WN, C::STAGES>() + C::BN * 4;
   static_assert(kLds <= 160 * 1024, "a block fits a CU");
   auto k = k_tile<Kind<T>::F16, NP, C::BM, C::BN, C::BK, C::WM, C::WN, C::STAGES, PKS, QKS, Epi>;
   const int rc = allow_lds((const void*)k, kLds);
   if (rc != CLID_OK) return rc;
-  hipLaunchKernelGGL(k, dim3((unsigned)blocks), dim3(64 * C::WM * C::WN), kLds, s, g, epi);
+  // as many rows of tiles a launch as 2^32 threads take (one row of them is under 2^29: n < 2^20, at most 64 splits)
+  const int64_t tiles_m = (g.m + C::BM - 1) / C::BM, each = (int64_t)g.tiles_n * g.splits, most = ((int64_t(1) << 32) - 1) / (each * 64 * C::WM * C::WN);
+  for (int64_t t = 0; t < tiles_m; t += most) {
+    g.first_m = (int)t;
+    g.tiles_m = (int)(tiles_m - t < most ? tiles_m - t : most);
+    hipLaunchKernelGGL(k, dim3((unsigned)(g.tiles_m * each)), dim3(64 * C::WM * C::WN), kLds, s, g, epi);
+  }
   return CLID_OK;
 }
 

@@ -50,7 +50,7 @@ struct Product {
   const int32_t* live;  // how many of m (or of k, live_k) there are on the device; NULL: all
   int live_k;
   int splits;           // k is cut into so many parts, part s of tile t is block t * splits + s
-  int tiles_m, tiles_n;
+  int tiles_m, tiles_n, first_m;  // of this launch: its tiles, and the tile rows before them
 };
 
 template <bool F16>
@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(64 * WM * WN) k_tile(Product g, Epi epi) {
     if (g.live_k) rows_k = live < rows_k ? live : rows_k;
     else rows_m = live < rows_m ? live : rows_m;
   }
-  const int64_t m0 = (int64_t)tm * BM, n0 = (int64_t)tn * BN;
+  const int64_t m0 = (int64_t)(g.first_m + tm) * BM, n0 = (int64_t)tn * BN;
   if (m0 >= rows_m) return;
   const int steps_all = (int)((rows_k + BK - 1) / BK), per = (steps_all + g.splits - 1) / g.splits;
   const int first = split * per, steps = first + per < steps_all ? per : steps_all > first ? steps_all - first : 0;

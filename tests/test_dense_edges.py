@@ -267,3 +267,31 @@ def test_activations_of_odd_values_answer_as_torch_does(shape, dtype):
             # (exact numbers all: 0, 1, 1/2; leaky_relu's 0.01 has one rounding to fp32 and one to the type)
             assert torch.allclose(y.double().cpu(), v.detach().expand(m, n), rtol=0, atol=0, equal_nan=True), (name, value)
             assert torch.allclose(db.double().cpu(), torch.full((n,), m * slope, dtype=torch.float64), rtol=2.0 ** -8, atol=0, equal_nan=True), (name, value, db[0], slope)
+
+
+@gpu
+def test_results_beyond_the_threads_of_one_launch():
+    """2^30 + 300 rows of 257 classes: the tiles are more than 2^32 threads, so one launch after the other takes its share of the rows."""
+    m, k, n = (1 << 30) + 300, 8, 257
+    torch.cuda.empty_cache()
+    if torch.cuda.mem_get_info()[0] < 140 << 30:
+        pytest.skip("needs 140 GB of free memory")
+    x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+    gen = generator(1)
+    w = (torch.arange(n, device="cuda") % 101 / 64)[:, None].repeat(1, k).to(torch.bfloat16)
+    w[:, 1:] = normal(gen, n, k - 1).to(torch.bfloat16)
+    rows = torch.cat([torch.arange(0, m, (1 << 24) + 77, device="cuda"), torch.tensor([m - 301, m - 300, m - 2, m - 1], device="cuda")])
+    x[rows] = normal(gen, len(rows), k).to(torch.bfloat16)
+    label, log_prob = linear_label(x, w)
+    lp = torch.log_softmax(x[rows].double() @ w.double().t(), 1)
+    top = lp.topk(2, dim=1)
+    clear = top.values[:, 0] - top.values[:, 1] > 1e-4
+    assert clear.sum() > 40 and torch.equal(label[rows][clear], top.indices[clear, 0])
+    # z is off by gamma(8) sum |x w| < 100 gamma(8), the statistics by gamma(257)
+    assert (log_prob[rows].double() - top.values[:, 0]).abs().max() <= 200 * ref.gamma(8) + ref.gamma(n) * 8
+    label[rows] = 0
+    assert not label.any()  # all zeros: the lowest class
+    log_prob[rows] = log_prob[1].item()
+    assert (log_prob == log_prob[1]).all()
+    del x, label, log_prob, lp
+    torch.cuda.empty_cache()
