@@ -12,6 +12,12 @@
  *     losses and log-probabilities are fp32;
  *   - `ws` has at least clid_*_workspace() bytes, 256-byte aligned, and holds nothing between calls;
  *   - rows >= 0, k >= 1, n >= 1, each matrix at most 2^40 elements; rows < 2^31, k, n < 2^20.
+ *
+ * Workspaces grow with the rows where n or k is over 64 and there are more than 32 rows: copies of operands that are not 16-bit rows of
+ * whole aligned 16 bytes (fp32: 6 bytes a value; the cross entropy always copies its rows); a layer's backward pass its dz (2 bytes a
+ * value, fp32 6); a class head's statistics 12 bytes (label) or 8 (cross entropy) a row for every 32 or 64 classes.  The cross entropy's backward
+ * pass holds dz of a piece of the classes: at most about 512 MB, but never under 256 classes, that is 512 bytes a row (fp32: 1536) from 1 M
+ * rows (350 k) on, and with more than one piece 4 k bytes a row for dx's sums.  A product whose k is cut adds 4 bytes a result and part.
  */
 #ifndef CLID_DENSE_H
 #define CLID_DENSE_H

@@ -295,3 +295,26 @@ def test_results_beyond_the_threads_of_one_launch():
     assert (log_prob == log_prob[1]).all()
     del x, label, log_prob, lp
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize("rows,k,n", [(40, 100, 65), (2048, 1024, 32000), (8192, 2048, 65536), (300000, 64, 72), (1 << 20, 64, 72), (1 << 22, 64, 300), (5000000, 8, 130000)])
+def test_workspaces_are_as_large_as_the_header_says(rows, k, n, dtype):
+    import ctypes as C
+
+    lib = L.load()
+    a = L.CeArgs(x=4096, w=4096, dx=4096, dw=4096, db=4096, ldx=k, ldw=k, rows=rows, k=k, n=n, dtype=dtype, reduction=1)
+    value = 6 if dtype == 0 else 2
+    k32, n32, slack = (k + 31) // 32 * 32, (n + 31) // 32 * 32, 4096
+    copies = value * (rows + n) * k32
+    forward = lib.clid_ce_workspace(C.byref(a))
+    assert value * rows * k <= forward <= copies + rows * (8 * (-(-n // 32)) + 4) + rows + slack
+    piece = max(512 << 20, value * 256 * rows)
+    backward = lib.clid_ce_bwd_workspace(C.byref(a))
+    dz = backward - copies - (4 * rows * k if piece < value * rows * n32 else 0)
+    # dz itself, k cut into at most 64 parts of the results of dx or dw, 4 bytes a column and run of at least 32 rows for db
+    parts = 64 * 4 * (k + 8) * max(rows, n32)
+    assert dz <= piece * (1 + 4 / (32 * value)) * 1.01 + parts + slack
+    assert backward >= value * rows * (k + min(n, 256))
+    a = L.LabelArgs(x=4096, w=4096, ldx=k, ldw=k, rows=rows, k=k, n=n, dtype=dtype)
+    assert lib.clid_label_workspace(C.byref(a)) <= copies + 12 * rows * (-(-n // 32)) + slack
