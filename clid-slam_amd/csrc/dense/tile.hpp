@@ -5,8 +5,8 @@
 // turned on the way out of LDS (ds_read_b64_tr_b16), so no transposed copy is ever made.
 // fp32 operands come as NP = 3 bf16 planes, hi + mid + lo = v exactly (8 bits each, by truncation), 32 columns' hi, their mid, their lo in
 // turn, so that a row's copy to LDS is 192 neighbouring bytes and not three times 64 (half a cache line each): six plane products
-// (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave out less than 2^-22 of |p q| and run at the bf16 rate, 2.5 PFLOP/s / 6 =
-// 417 TFLOP/s against 157 of the fp32 matrix instructions.
+// (hi hi, hi mid, mid hi, mid mid, hi lo, lo hi) leave out less than 2^-21 of |p q| (mid lo and lo mid: mid is under 2^-7, lo under 2^-15
+// of its number; under 2^-24 on average) and run at the bf16 rate, 2.5 PFLOP/s / 6 = 417 TFLOP/s against 157 of the fp32 matrix instructions.
 //
 // Tiles.  One block computes BM x BN with WM x WN waves, each 32 x 32 x 16 instructions on a (BM / WM) x (BN / WN) part.  Per step
 // of BK along k the block copies both tiles from memory straight to LDS (16 bytes a lane, buffer loads whose bounds check turns

@@ -1,4 +1,6 @@
 """Calls of the dense operators at the edge of what they promise, and results that need more than the tests of whole layers ask for."""
+import math
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
@@ -318,3 +320,57 @@ def test_workspaces_are_as_large_as_the_header_says(rows, k, n, dtype):
     assert backward >= value * rows * (k + min(n, 256))
     a = L.LabelArgs(x=4096, w=4096, ldx=k, ldw=k, rows=rows, k=k, n=n, dtype=dtype)
     assert lib.clid_label_workspace(C.byref(a)) <= copies + 12 * rows * (-(-n // 32)) + slack
+
+
+def whole(gen, bits, *shape):
+    """odd whole numbers of up to `bits` bits, either sign"""
+    return (torch.randint(0, 1 << (bits - 1), shape, generator=gen, device="cuda") * 2 + 1) * (torch.randint(0, 2, shape, generator=gen, device="cuda") * 2 - 1).float()
+
+
+def one_a_column(gen, values, rows):
+    """[rows, len(values)]: values[c] at a row of its own choice in each column, zeros elsewhere; and those rows"""
+    at = torch.randint(0, rows, (len(values),), generator=gen, device="cuda")
+    out = torch.zeros(rows, len(values), device="cuda")
+    out[at, torch.arange(len(values), device="cuda")] = values
+    return out, at
+
+
+# Tiles of 64, 128 and 256 with k whole and cut, for the layer's product (operands' rows along k) and both gradients' (one or both operands' rows
+# across k), then the few-row and the narrow kernels
+@gpu
+@pytest.mark.parametrize("m,k,n", [(40, 72, 70), (4096, 264, 1024), (333, 8200, 260), (8000, 96, 4000), (4096, 1024, 1024), (2100, 2000, 130), (20, 100, 70), (300, 64, 48)], ids=str)
+def test_fp32_products_keep_every_bit_of_their_operands(m, k, n):
+    """One term a sum, whose product fits 24 bits: 12-bit numbers with 12-bit numbers, 24-bit ones with powers of two.  In three bf16
+    parts of 8 bits each that takes hi hi, hi mid, mid hi, mid mid, and hi lo, lo hi."""
+    gen = generator(m + k + n)
+
+    def grads(x, w, dy):
+        x, w = x.requires_grad_(), w.requires_grad_()
+        return torch.autograd.grad(linear_act(x, w), [x, w], dy)
+
+    def power(count):
+        return 2.0 ** torch.randint(-8, 9, (count,), generator=gen, device="cuda")
+
+    for of_x, of_w in ((12, 12), (24, 0), (0, 24)):  # bits; 0: powers of two
+        value = lambda bits, *s: whole(gen, bits, *s) if bits else power(math.prod(s)).view(s)  # noqa: E731
+        # y: x has one value a row, w is full; then the other way about
+        xt, at = one_a_column(gen, value(of_x, m), k)
+        w = value(of_w, n, k)
+        assert torch.equal(linear_act(xt.t().contiguous(), w).double(), xt.sum(0).double()[:, None] * w.double()[:, at].t())
+        wt, at = one_a_column(gen, value(of_w, n), k)
+        x = value(of_x, m, k)
+        assert torch.equal(linear_act(x, wt.t().contiguous()).double(), x.double()[:, at] * wt.sum(0).double())
+        # dx: dy has one value a row, w is full; w has one value a column, dy is full
+        dyt, at = one_a_column(gen, value(of_x, m), n)
+        w = value(of_w, n, k)
+        assert torch.equal(grads(torch.zeros(m, k, device="cuda"), w, dyt.t().contiguous())[0].double(), dyt.sum(0).double()[:, None] * w.double()[at])
+        w, at = one_a_column(gen, value(of_w, k), n)
+        dy = value(of_x, m, n)
+        assert torch.equal(grads(torch.zeros(m, k, device="cuda"), w, dy)[0].double(), dy.double()[:, at] * w.sum(0).double())
+        # dw: dy has one value a column, x is full; x has one value a column, dy is full
+        dy, at = one_a_column(gen, value(of_w, n), m)
+        x = value(of_x, m, k)
+        assert torch.equal(grads(x, torch.zeros(n, k, device="cuda"), dy)[1].double(), dy.sum(0).double()[:, None] * x.double()[at])
+        x, at = one_a_column(gen, value(of_x, k), m)
+        dy = value(of_w, m, n)
+        assert torch.equal(grads(x, torch.zeros(n, k, device="cuda"), dy)[1].double(), (dy.double()[at] * x.sum(0).double()[:, None]).t())
