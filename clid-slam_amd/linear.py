@@ -108,8 +108,8 @@ def rows_of(t: torch.Tensor, width: int):
 
 def check_operands(what: str, x, weight, bias=None, residual=None) -> None:
     """x [..., k], weight [n, k], bias [n], residual [..., n]: on one GPU, of one of the three types."""
-    for name, t in (("x", x), ("weight", weight)):
-        if not isinstance(t, torch.Tensor):
+    for name, t in (("x", x), ("weight", weight), ("bias", bias), ("residual", residual)):
+        if not isinstance(t, torch.Tensor) and (t is not None or name in ("x", "weight")):
             raise RuntimeError(f"{what}: {name} must be a tensor")
     if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
         raise RuntimeError(f"{what}: make_fx records the tensors that a call makes but not the kernels that fill them")

@@ -374,3 +374,12 @@ def test_fp32_products_keep_every_bit_of_their_operands(m, k, n):
         x, at = one_a_column(gen, value(of_x, k), m)
         dy = value(of_w, m, n)
         assert torch.equal(grads(x, torch.zeros(n, k, device="cuda"), dy)[1].double(), (dy.double()[at] * x.sum(0).double()[:, None]).t())
+
+
+def test_operands_that_are_no_tensors_are_named(launches):
+    x, w = torch.zeros(4, 8), torch.zeros(5, 8)
+    for name, call in (("bias", lambda: linear_act(x, w, 0.5)), ("residual", lambda: linear_act(x, w, residual=1.0)), ("bias", lambda: linear_label(x, w, [0.0] * 5)),
+                       ("bias", lambda: linear_cross_entropy(x, w, 0, torch.zeros(4, dtype=torch.int64))), ("weight", lambda: linear_act(x, None))):
+        with pytest.raises(RuntimeError, match=f"{name} must be a tensor"):
+            call()
+    assert not launches
