@@ -249,7 +249,8 @@ struct EpiStat {
     top = fmaxf(top, __shfl_xor(top, 32, 64));
     const float safe = top == neg_inf() ? 0.f : top;
     // sum of all exp(z - top), the largest one's 1 among them; where the others are less than half of it that sum has lost more of their last
-    // bits than a sum loses anyway, and they are added up again without it
+    // bits than a sum loses anyway, and they are added up again without it (down to 2^-6 only, which lost 6 bits: 8192 x 2048 -> 65536 bf16
+    // 1.67 ms either way, 1048576 x 64 -> 72 fp16 with random logits 0.21 and 0.22)
     float rest = 0.f;
 #pragma unroll
     for (int i = 0; i < TN; ++i)

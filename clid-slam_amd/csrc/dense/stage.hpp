@@ -98,8 +98,10 @@ inline void stage(const Staging& a, const Staging& b, hipStream_t s) {
   if (a.blocks + b.blocks) hipLaunchKernelGGL(k_stage<T>, dim3(a.blocks + b.blocks), dim3(256), 0, s, a, b);
 }
 
-// dz = dy act'(z) -> planes with rows of np values (dst may be NULL: the sums alone), and its column sums over blocks of rows ->
-// part[row block][n].  A block takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows.  Bound by memory: 8192 x 4096 bf16 (dy, z and
+// dz = dy act'(z) -> planes with rows of np values (dst may be NULL: the sums alone), and its column sums over blocks of rows, before any
+// rounding -> part[row block][n].  16-bit dz has one rounding here, since the matrix instruction takes both operands in 16 bits: dx and dw are then
+// off by 0.00235 where one rounding of the results gives 0.00166 (8192 x 4096 -> 4096 bf16, relative to the norm); in two parts, which would have no
+// more than that, both products run twice (762 us -> about 1230).  A block takes 256 columns (8 a thread) and every gridDim.y-th run of 8 rows.  Bound by memory: 8192 x 4096 bf16 (dy, z and
 // dz 67 MB each) 47 us, 4.2 TB/s.
 template <typename T, typename Z>
 __global__ void __launch_bounds__(256) k_dz(const T* dy, int64_t lddy, const Z* z, int64_t rows, int n, int act, uint16_t* dst, int np, float* part) {
@@ -188,7 +190,8 @@ inline int allow_lds(const void* kernel, int bytes) {
 }
 
 // n, k <= 64 (narrow.hip; in tiles, 64 -> 64: fp32 98304 rows 51 us against 25, layer and gradients 157 against 69, cross entropy and gradients
-// 212 against 70; bf16 35, 103, 153 against 16, 64, 56.  Only 1000 bf16 rows are as quick in tiles: 7 us against 8)
+// 212 against 70; bf16 35, 103, 153 against 16, 64, 56.  Only 1000 bf16 rows are as quick in tiles: 7 us against 8.  The border
+// is what the registers hold, not where both are even: 1048576 rows, cross entropy and gradients in fp16, 64 -> 64 here 314 us, 64 -> 72 in tiles 1316)
 inline bool is_narrow(int32_t k, int32_t n) { return k <= 64 && n <= 64; }
 int narrow_linear(const clid_linear_args* a, hipStream_t s);
 int64_t narrow_linear_bwd_bytes(const clid_linear_bwd_args* a);
