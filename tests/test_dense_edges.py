@@ -383,3 +383,40 @@ def test_operands_that_are_no_tensors_are_named(launches):
         with pytest.raises(RuntimeError, match=f"{name} must be a tensor"):
             call()
     assert not launches
+
+
+@gpu
+@pytest.mark.parametrize("m,k,n,dtype,reduction", [(300, 72, 66, "bf16", "mean"), (20000, 24, 70, "f16", "none"), (300, 64, 21, "f32", "mean"), (20, 100, 70, "f32", "sum"),
+                                                   (2049, 64, 500, "f32", "none")])
+def test_a_captured_step_follows_its_targets(m, k, n, dtype, reduction):
+    """How many rows count is read on the device: a replay on other targets (none, all, some ignored, factors with them) is the eager result."""
+    dt, gen = TYPES[dtype], generator(m)
+    x, w, b = normal(gen, m, k).to(dt), (normal(gen, n, k) * k ** -0.5).to(dt), normal(gen, n).to(dt)
+    t, g = torch.randint(0, n, (m,), generator=gen, device="cuda"), normal(gen, m) if reduction == "none" else torch.full((), 8.0, device="cuda")
+
+    def step():
+        leaves = [v.detach().requires_grad_() for v in (x, w, b)]
+        loss = linear_cross_entropy(*leaves, t, reduction=reduction)
+        return [loss.detach(), *torch.autograd.grad(loss, leaves, g)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        step()
+    s.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        out = step()
+    for share in (0.5, 1.0, 0.0, 0.9, 0.1):
+        t.copy_(torch.randint(0, n, (m,), generator=gen, device="cuda"))
+        t[torch.rand(m, generator=gen, device="cuda") < share] = -100
+        if reduction == "none":
+            g.copy_(normal(gen, m))
+        want = step()
+        for v in out:
+            v.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, q) for a, q in zip(out, want)), share
+        if share == 1.0:
+            assert not any(v.any() for v in out)
